@@ -951,6 +951,10 @@ hxq_error_t decompress_sync(hxq_tensor_t *t, void *d_out, int bf16, float *l2)
 
 }  // namespace
 
+namespace hxq {
+void count_launches(unsigned n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
+}  // namespace hxq
+
 // ===========================================================================
 // Internal interface used by the C host library (hxq_internal.h)
 

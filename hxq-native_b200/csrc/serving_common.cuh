@@ -1,0 +1,125 @@
+// serving_common.cuh -- pieces shared by the serving operators (kv_cache.cu,
+// kv_attention.cu, lora.cu).  Internal header.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstdint>
+
+#include "hxq_cuda.h"
+#include "hxq_serving.h"
+
+namespace hxq {
+
+// Adds to hxq_cuda_launch_count (hxq_cuda_rt.cu).
+void count_launches(unsigned n);
+
+namespace serving {
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static __device__ __forceinline__ float to(float v) { return v; }
+    static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static __device__ __forceinline__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Elem<__half> {
+    static __device__ __forceinline__ float to(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
+
+// One code as the value it stands for (before its scale).
+template <int FMT> __device__ __forceinline__ float code_value(uint8_t c)
+{
+    if (FMT == HXQ_KV_INT8) return (float)(int8_t)c;
+    __nv_fp8_e4m3 v;
+    v.__x = c;
+    return (float)v;
+}
+
+// The nearest code (ties to even); int8 takes NaN to 0.
+template <int FMT> __device__ __forceinline__ uint8_t nearest_code(float v)
+{
+    if (FMT == HXQ_KV_INT8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(v)));
+    return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ void flag(uint32_t *status, uint32_t bit)
+{
+    if (status) atomicOr(status, bit);
+}
+
+// Programmatic dependent launch: the next kernel of the stream may begin its
+// prologue / this kernel's reads of its predecessor's results may begin.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+inline hxq_error_t launched(unsigned n = 1)
+{
+    if (cudaGetLastError() != cudaSuccess) return HXQ_ERR_CUDA;
+    count_launches(n);
+    return HXQ_OK;
+}
+
+inline int sm_count()
+{
+    int sms = 148, dev = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+// Raise a kernel's dynamic shared memory limit, once per device (`ready`:
+// one bit per device, a static of the kernel's launcher).
+template <typename K> cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t> &ready)
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (ready.load(std::memory_order_acquire) >> dev & 1u) return cudaSuccess;
+    if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)) != cudaSuccess) return e;
+    ready.fetch_or(1ull << dev, std::memory_order_acq_rel);
+    return cudaSuccess;
+}
+
+// A launch that may begin before the kernel in front of it on the stream
+// has ended; the kernel calls wait_previous before it reads or writes memory.
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Host checks of a cache descriptor.
+inline hxq_error_t check_cache(const hxq_kv_cache_t *c)
+{
+    if (!c || !c->k || !c->v || !c->k_scales || !c->v_scales) return HXQ_ERR_NULL_PTR;
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return HXQ_ERR_INVALID_DIM;
+    if (c->block_tokens == 0 || c->block_tokens % 16 != 0 || c->block_tokens > 256) return HXQ_ERR_INVALID_DIM;
+    if (c->n_blocks == 0 || c->n_heads == 0 || c->n_heads > 65535) return HXQ_ERR_INVALID_ARG;
+    if ((uint64_t)c->n_blocks * c->block_tokens >= (1ull << 31)) return HXQ_ERR_INVALID_ARG;
+    if (c->format != HXQ_KV_INT8 && c->format != HXQ_KV_E4M3) return HXQ_ERR_INVALID_ARG;
+    if ((((uintptr_t)c->k | (uintptr_t)c->v) & 15u) != 0 || (((uintptr_t)c->k_scales | (uintptr_t)c->v_scales) & 3u) != 0)
+        return HXQ_ERR_INVALID_ARG;
+    return HXQ_OK;
+}
+
+}  // namespace serving
+}  // namespace hxq

@@ -40,6 +40,9 @@ HXQ_BACKEND_AUTO, HXQ_BACKEND_CPU, HXQ_BACKEND_CUDA, HXQ_BACKEND_METAL, HXQ_BACK
 HXQ_OUT_F32, HXQ_OUT_BF16 = 0, 1
 HXQ_IMAGE_STREAMED, HXQ_IMAGE_MATMUL = 1, 2
 HXQ_AFFINE_PATH_AUTO, HXQ_AFFINE_PATH_GEMV, HXQ_AFFINE_PATH_TC_GEMV, HXQ_AFFINE_PATH_GEMM = 0, 1, 2, 3
+HXQ_ELEM_F32, HXQ_ELEM_BF16, HXQ_ELEM_F16 = 0, 1, 2
+HXQ_KV_INT8, HXQ_KV_E4M3 = 0, 1
+HXQ_LORA_TILE = 64
 MAX_BATCH = 64
 
 P = C.c_void_p
@@ -80,6 +83,30 @@ class AffineTensor(C.Structure):
     _fields_ = [("indices", P), ("scales", P), ("offsets", P), ("bias", P),
                 ("out_features", C.c_uint32), ("in_features", C.c_uint32),
                 ("group_size", C.c_uint32)]
+
+
+class KvCacheDesc(C.Structure):
+    """hxq_kv_cache_t (include/hxq_serving.h); device pointers."""
+    _fields_ = [("k", P), ("v", P), ("k_scales", P), ("v_scales", P),
+                ("n_blocks", C.c_uint32), ("n_heads", C.c_uint32), ("block_tokens", C.c_uint32),
+                ("head_dim", C.c_uint32), ("format", C.c_uint32)]
+
+
+class KvAttention(C.Structure):
+    """hxq_kv_attention_t (include/hxq_serving.h); device pointers."""
+    _fields_ = [("q", P), ("out", P), ("lse", P),
+                ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64),
+                ("out_stride_t", C.c_int64), ("out_stride_h", C.c_int64),
+                ("starts", P), ("lens", P), ("table", P),
+                ("n_requests", C.c_uint32), ("n_rows", C.c_uint32), ("n_heads", C.c_uint32),
+                ("table_width", C.c_uint32), ("max_new", C.c_uint32), ("window", C.c_uint32),
+                ("scale", C.c_float), ("elem", C.c_int), ("causal", C.c_int)]
+
+
+class LoraDesc(C.Structure):
+    """hxq_lora_t (include/hxq_serving.h); device pointers."""
+    _fields_ = [("a", P), ("b", P), ("scales", P), ("n_adapters", C.c_uint32), ("rank", C.c_uint32),
+                ("in_features", C.c_uint32), ("out_features", C.c_uint32)]
 
 
 TP = C.POINTER(HxqTensor)
@@ -153,6 +180,19 @@ SIGNATURES = {
     "hxq_cuda_peer_wait": (C.c_int, [P, C.c_uint32, P, P, P]),
     "hxq_cuda_image_has_matmul_tables": (C.c_int, [P]),
     "hxq_cuda_vq_matmul_path": (C.c_int, [P, P, C.c_uint32, P, C.c_uint32, C.c_int, P]),
+    # include/hxq_serving.h
+    "hxq_cuda_kv_plan": (C.c_int, [P, P, C.c_uint32, P, C.c_uint32, C.c_uint32, P, C.c_uint32, P, P, P, P, C.c_uint32,
+                                   P, P, P]),
+    "hxq_cuda_kv_append": (C.c_int, [C.POINTER(KvCacheDesc), P, P, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                                     P, C.c_uint32, P, P]),
+    "hxq_cuda_kv_read": (C.c_int, [C.POINTER(KvCacheDesc), P, C.c_uint32, P, P, C.c_int, P, P]),
+    "hxq_cuda_kv_attention_workspace": (C.c_size_t, [C.POINTER(KvCacheDesc), C.POINTER(KvAttention)]),
+    "hxq_cuda_kv_attention": (C.c_int, [C.POINTER(KvCacheDesc), C.POINTER(KvAttention), P, C.c_size_t, P, P]),
+    "hxq_lora_tiles": (C.c_uint32, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    "hxq_cuda_lora_plan": (C.c_int, [P, P, C.c_uint32, C.c_uint32, C.c_uint32, P, P, P, P]),
+    "hxq_cuda_lora_workspace": (C.c_size_t, [C.POINTER(LoraDesc), C.c_uint32, C.c_uint32]),
+    "hxq_cuda_lora": (C.c_int, [C.POINTER(LoraDesc), P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_uint32, C.c_uint32,
+                                P, P, P, C.c_size_t, P]),
     # Lloyd's algorithm (hxq_lloyd.h, hxq_cuda.h)
     "hxq_lloyd_reassign": (C.c_int, [P, P, P, C.c_size_t, C.c_int, C.c_int, P]),
     "hxq_lloyd_assign_only": (C.c_int, [P, P, P, C.c_size_t, C.c_int, C.c_int]),

@@ -22,6 +22,9 @@ import ctypes as C
 import torch
 
 from . import (HXQ_IMAGE_MATMUL, HXQ_OUT_BF16, HXQ_OUT_F32, AffineTensor, Tensor, check, lib)
+from .serving import KvCache, LoraAdapters, LoraPlan
+from .serving import kv_plan as _kv_plan
+from .serving import lora_plan as _lora_plan
 
 _DT = {torch.float32: HXQ_OUT_F32, torch.bfloat16: HXQ_OUT_BF16}
 
@@ -92,6 +95,60 @@ def _(x, codes, scales, offsets, bias, group_size):
     return x.new_empty((*x.shape[:-1], codes.shape[0]), dtype=torch.float32)
 
 
+# -- serving operators (hxq_b200.serving; the same calls on flat tensor
+# arguments, for graphs that are traced) --------------------------------------
+
+@torch.library.custom_op("hxq::kv_plan", mutates_args=("table",))
+def kv_plan(new: torch.Tensor, cached: torch.Tensor, table: torch.Tensor, free: torch.Tensor, block_tokens: int,
+            n_slots: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """starts, lens, slots, positions, taken; enters new blocks in table."""
+    # an operator's results may not share memory
+    return tuple(t.clone() for t in _kv_plan(new, cached, table, free, block_tokens, n_slots))
+
+
+@kv_plan.register_fake
+def _(new, cached, table, free, block_tokens, n_slots):
+    B = new.shape[0]
+    return tuple(new.new_empty(n) for n in (B + 1, B, n_slots, n_slots, 1))
+
+
+@torch.library.custom_op("hxq::kv_append", mutates_args=("k_codes", "v_codes", "k_scales", "v_scales"))
+def kv_append(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, k: torch.Tensor,
+              v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise rows of k and v into their slots of an 8-bit cache."""
+    KvCache(k_codes, v_codes, k_scales, v_scales).append(k, v, slots)
+
+
+@kv_append.register_fake
+def _(k_codes, v_codes, k_scales, v_scales, k, v, slots):
+    return None
+
+
+@torch.library.custom_op("hxq::kv_attention", mutates_args=())
+def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                 starts: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, max_new: int, scale: float, window: int,
+                 causal: bool) -> torch.Tensor:
+    """Attention of q [rows, heads, head_dim] over an 8-bit cache."""
+    return KvCache(k_codes, v_codes, k_scales, v_scales).attention(q, starts, lens, table, max_new, scale, window, causal)
+
+
+@kv_attention.register_fake
+def _(q, k_codes, v_codes, k_scales, v_scales, starts, lens, table, max_new, scale, window, causal):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("hxq::lora", mutates_args=())
+def lora(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, starts: torch.Tensor,
+         adapters: torch.Tensor) -> torch.Tensor:
+    """y + scale (x A^T) B^T of each request's adapter."""
+    return LoraAdapters(a, b, scales).add(y, x, _lora_plan(starts, adapters, a.shape[0], x.shape[0]))
+
+
+@lora.register_fake
+def _(y, x, a, b, scales, starts, adapters):
+    return y.new_empty(y.shape)
+
+
 class HxqLinear(torch.nn.Module):
     """A linear layer (no bias) whose weight is an HXQ tensor kept compressed
     on the GPU: 12-bit 2D-VQ tensors run the fused VQ matmul, other modes
@@ -125,10 +182,20 @@ class HxqLinear(torch.nn.Module):
     def weight(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return dequant(self.image, self.out_features, self.in_features, dtype)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, adapters: LoraAdapters | None = None, plan: LoraPlan | None = None) -> torch.Tensor:
+        """x @ W.T in fp32; with `adapters` (of this projection's rows) and the
+        step's plan (hxq_b200.serving.lora_plan), plus each token's adapter."""
         if self.fused:
-            return vq_matmul(x.to(torch.bfloat16), self.image, self.out_features)
-        return torch.matmul(x.float(), self.weight(torch.float32).t())
+            y = vq_matmul(x.to(torch.bfloat16), self.image, self.out_features)
+        else:
+            y = torch.matmul(x.float(), self.weight(torch.float32).t())
+        if adapters is None:
+            return y
+        if plan is None:
+            raise ValueError("adapters need the step's plan")
+        flat = y.view(-1, self.out_features)
+        adapters.add(flat, x.reshape(-1, self.in_features).to(torch.bfloat16), plan, out=flat)
+        return y
 
     def __del__(self):
         img = getattr(self, "_img", None)
