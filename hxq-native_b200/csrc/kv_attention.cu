@@ -36,7 +36,6 @@ constexpr int kRows = 16;        // rows of a tile
 constexpr int kGran = 64;        // keys of a granule
 constexpr int kWarpsA = 4;
 constexpr int kThreadsA = kWarpsA * 32;
-constexpr uint32_t kMaxParts = 128;   // most parts of a unit that the second kernel joins
 
 template <int D> struct Geo {
     static constexpr int kVB = D >= 128 ? 16 : 8;      // bytes of a lane's copy of a value row
@@ -51,7 +50,6 @@ template <int D> struct Geo {
     static constexpr int kMerge = kWarpsA * kRows * (D + kPad) * 4;
     static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQSmem;
     static constexpr int kCtas = D == 256 ? 2 : 3;
-    static constexpr int kPartFloats = kRows * D + 2 * kRows;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src)
@@ -69,28 +67,6 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void *src)
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Granules of tile t of a request, and the first one's number.
-__device__ __forceinline__ uint32_t tile_grans(const AttnArgs &a, const Req &r, uint32_t t, uint32_t &first)
-{
-    uint32_t lo, hi;
-    key_range(a, r, t * kRows, min((t + 1) * kRows, r.rows), lo, hi);
-    first = lo / kGran;
-    const uint32_t last = (hi + kGran - 1) / kGran;
-    return last > first ? last - first : 1u;   // a tile that sees nothing still writes its rows
-}
-
-__device__ __forceinline__ uint64_t req_grans(const AttnArgs &a, const Req &r, uint32_t &most)
-{
-    uint64_t sum = 0;
-    uint32_t first;
-    for (uint32_t t = 0; t * kRows < r.rows; ++t) {
-        const uint32_t n = tile_grans(a, r, t, first);
-        sum += n;
-        most = max(most, n);
-    }
-    return sum;
-}
-
 template <typename QT> __device__ __forceinline__ uint32_t to_f16x2(uint32_t w, float m)
 {
     const QT *e = reinterpret_cast<const QT *>(&w);
@@ -103,101 +79,24 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
 {
     using G = Geo<D>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t sh_scan[kWarpsA];
-    __shared__ uint32_t sh_most[kWarpsA];
-    __shared__ uint32_t sh_b;
-    __shared__ uint64_t sh_off;
+    __shared__ RangeShared<kWarpsA> sh;
     __shared__ float sh_m[kWarpsA][kRows], sh_l[kWarpsA][kRows];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
     let_next_start();
 
-    // this CTA's range [x, x1) of all granules, and the request it begins in
-    uint64_t x, x1;
-    uint32_t b;
-    uint64_t off;
-    {
-        const uint32_t per = (a.B + kThreadsA - 1) / kThreadsA, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-        uint64_t mine = 0;
-        uint32_t most = 1;
-        for (uint32_t i = b0; i < b1; ++i) {
-            mine += req_grans(a, load_req(a, i), most) * a.H;
-            if (blockIdx.x == 0 && a.row_min == 0) flag_req(a, i);
-        }
-        uint64_t incl = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint64_t u = __shfl_up_sync(~0u, incl, d);
-            if (lane >= (uint32_t)d) incl += u;
-        }
-        most = __reduce_max_sync(~0u, most);
-        if (lane == 31) {
-            sh_scan[warp] = incl;
-            sh_most[warp] = most;
-        }
-        if (tid == 0) { sh_b = a.B; sh_off = 0; }
-        __syncthreads();
-        uint64_t total = 0, before = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < kWarpsA; ++w) {
-            if (w < warp) before += sh_scan[w];
-            total += sh_scan[w];
-            most = max(most, sh_most[w]);
-        }
-        const uint64_t least = max(1u, (most + kMaxParts - 1) / kMaxParts);   // granules a CTA takes at least
-        uint64_t n = (total + least - 1) / least;
-        n = n < gridDim.x ? n : gridDim.x;
-        if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
-        if (blockIdx.x >= n) return;
-        x = total * blockIdx.x / n;
-        x1 = total * (blockIdx.x + 1) / n;
-        incl += before;
-        if (incl - mine <= x && x < incl) {
-            uint64_t at = incl - mine;
-            for (uint32_t i = b0; i < b1; ++i) {
-                const uint64_t w = req_grans(a, load_req(a, i), most) * a.H;
-                if (x < at + w) {
-                    sh_b = i;
-                    sh_off = x - at;
-                    break;
-                }
-                at += w;
-            }
-        }
-        __syncthreads();
-        b = sh_b;
-        off = sh_off;
-        // for the parts of a unit that ends behind this range
-        sh_scan[0] = total;
-        sh_scan[1] = n;
-    }
-
+    if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    Range range;
+    if (!find_range<kWarpsA, kRows, kGran>(a, sh, true, range)) return;
     const uint32_t ring = pipe::smem_u32(smem) + warp * (G::kStages * G::kSlot);
     uint4 *qs = reinterpret_cast<uint4 *>(smem + (G::kSmem - G::kQSmem));
     float *merge = reinterpret_cast<float *>(smem);
     const uint32_t bh_bytes = a.P * D;
 
-    while (x < x1 && b < a.B) {
-        const Req r = load_req(a, b);
-        uint32_t most = 0;
-        const uint64_t sum = req_grans(a, r, most);
-        if (off >= sum * a.H) {
-            off -= sum * a.H;
-            ++b;
-            continue;
-        }
-        const uint32_t h = (uint32_t)(off / sum);
-        uint32_t rem = (uint32_t)(off % sum), tile = 0, first, n;
-        while (true) {
-            n = tile_grans(a, r, tile, first);
-            if (rem < n) break;
-            rem -= n;
-            ++tile;
-        }
-        const uint32_t take = (uint32_t)min((uint64_t)(n - rem), x1 - x);
-        uint32_t lo, hi;
-        const uint32_t r0 = tile * kRows, r1 = min(r0 + kRows, r.rows);
-        key_range(a, r, r0, r1, lo, hi);
-        const uint32_t key0 = (first + rem) * kGran + warp * 16;   // this warp's first 16 keys
+    Segment seg;
+    while (next_segment<kRows, kGran>(a, range, seg)) {
+        const Req &r = seg.r;
+        const uint32_t h = seg.h, take = seg.take, hi = seg.hi, r0 = seg.r0, r1 = seg.r1;
+        const uint32_t key0 = (seg.first + seg.rem) * kGran + warp * 16;   // this warp's first 16 keys
 
         // ---- Q: rows g and g + 8, in the order in which codes arrive
         uint32_t qf[G::kQSmem ? 1 : D / 16][4];
@@ -271,7 +170,7 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
             for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
         uint32_t valid = 0;   // bit s: the step in stage s has a block inside the cache
-        const int32_t *row = a.table + (size_t)b * a.width;
+        const int32_t *row = a.table + (size_t)seg.b * a.width;
         auto entry = [&](uint32_t j) -> int32_t {
             const uint32_t key = key0 + j * kGran;
             return j < take && key < hi ? __ldg(row + key / a.P) : -1;
@@ -475,8 +374,8 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
                 mine[(g + (e >> 1) * 8) * (D + G::kPad) + d + (2 * q + (e & 1)) * G::kVB] = o[t][e] * wt[e >> 1];
         }
         __syncthreads();
-        const bool whole = rem == 0 && take == n;
-        float *part = a.part + (size_t)(2 * blockIdx.x + (rem == 0 ? 1 : 0)) * G::kPartFloats;
+        const bool whole = seg.rem == 0 && take == seg.n;
+        float *part = a.part + (size_t)(2 * blockIdx.x + (seg.rem == 0 ? 1 : 0)) * part_floats<kRows, D>();
         for (uint32_t i = tid; i < kRows * (D / 4); i += kThreadsA) {
             const uint32_t rr = i / (D / 4), d = (i % (D / 4)) * 4;
             if (r0 + rr >= r1) break;
@@ -511,84 +410,41 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
                 }
             }
         }
-        if (rem == 0 && take < n && tid == 0) {
-            // the unit's last granule is n - take behind this range's end: which CTA has it
-            const uint64_t total = sh_scan[0], ctas = sh_scan[1], end = x + n;
-            uint64_t c = blockIdx.x + 1;
-            while (total * (c + 1) / ctas < end) ++c;
-            a.desc[blockIdx.x] = make_int4((int)(c - blockIdx.x + 1), (int)b, (int)h, (int)tile);
-        }
+        if (seg.rem == 0 && take < seg.n && tid == 0) a.desc[blockIdx.x] = cut_unit(range, seg);
         __syncthreads();   // the ring is free again
-        x += take;
-        off += take;
     }
 }
 
-// Joins the parts of the unit that CTA blockIdx.x began and did not finish:
-// its own second slot, then the first slots of the CTAs behind it, in order.
 template <int D, typename QT> __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a)
 {
-    using G = Geo<D>;
     wait_previous();
-    const int4 d = a.desc[blockIdx.x];
-    if (d.x == 0) return;
-    const Req r = load_req(a, (uint32_t)d.y);
-    const uint32_t row = (uint32_t)d.w * kRows + blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= min(((uint32_t)d.w + 1) * kRows, r.rows)) return;
-    const uint32_t rr = row % kRows;
-    const float *first = a.part + (size_t)(2 * blockIdx.x + 1) * G::kPartFloats;
-    const float *rest = a.part + (size_t)(2 * (blockIdx.x + 1)) * G::kPartFloats;
-    const size_t step = 2 * G::kPartFloats;
-    auto part = [&](int i) { return i == 0 ? first : rest + (size_t)(i - 1) * step; };
-    float top = -INFINITY;
-    for (int i = lane; i < d.x; i += 32) top = fmaxf(top, part(i)[kRows * D + rr]);
-#pragma unroll
-    for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, m));
-    constexpr int N = D / 32;
-    float v[N], sum = 0.0f;
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < d.x; ++i) {
-        const float *p = part(i);
-        const float m = p[kRows * D + rr], w = top == -INFINITY ? 1.0f : ex2(m - top);
-        sum += p[kRows * D + kRows + rr] * w;
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] += p[rr * D + j * 32 + lane] * w;
-    }
-    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const uint32_t tok = r.q0 + row / a.G, head = (uint32_t)d.z * a.G + row % a.G;
-    QT *dst = static_cast<QT *>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
-#pragma unroll
-    for (int j = 0; j < N; ++j) dst[j * 32 + lane] = Elem<QT>::from(v[j] * f);
-    if (a.lse && lane == 0)
-        a.lse[(size_t)tok * a.Hq + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+    join_row<kRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
 }
 
-template <int D, int FMT, typename QT> cudaError_t launch_one(const AttnArgs &a, uint32_t grid, cudaStream_t s)
+template <int D, int FMT, typename QT> cudaError_t launch_one(const AttnArgs &a, uint32_t grid, bool join, cudaStream_t s)
 {
     auto kernel = attn_mma_kernel<D, FMT, QT>;
     static std::atomic<uint64_t> ready{0};
     cudaError_t e = allow_smem(kernel, Geo<D>::kSmem, ready);
     if (e != cudaSuccess) return e;
     kernel<<<grid, kThreadsA, Geo<D>::kSmem, s>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if ((e = cudaGetLastError()) != cudaSuccess || !join) return e;
     return launch_behind(attn_join_kernel<D, QT>, dim3(grid, kRows / 4), dim3(128), 0, s, a);
 }
 
-template <int D> cudaError_t launch_dim(const AttnArgs &a, uint32_t fmt, int elem, uint32_t grid, cudaStream_t s)
+template <int D> cudaError_t launch_dim(const AttnArgs &a, uint32_t fmt, int elem, uint32_t grid, bool join, cudaStream_t s)
 {
     if (elem == HXQ_ELEM_BF16)
-        return fmt == HXQ_KV_INT8 ? launch_one<D, HXQ_KV_INT8, __nv_bfloat16>(a, grid, s)
-                                  : launch_one<D, HXQ_KV_E4M3, __nv_bfloat16>(a, grid, s);
-    return fmt == HXQ_KV_INT8 ? launch_one<D, HXQ_KV_INT8, __half>(a, grid, s)
-                              : launch_one<D, HXQ_KV_E4M3, __half>(a, grid, s);
+        return fmt == HXQ_KV_INT8 ? launch_one<D, HXQ_KV_INT8, __nv_bfloat16>(a, grid, join, s)
+                                  : launch_one<D, HXQ_KV_E4M3, __nv_bfloat16>(a, grid, join, s);
+    return fmt == HXQ_KV_INT8 ? launch_one<D, HXQ_KV_INT8, __half>(a, grid, join, s)
+                              : launch_one<D, HXQ_KV_E4M3, __half>(a, grid, join, s);
 }
 
-cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, uint32_t grid, cudaStream_t s)
+cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, uint32_t grid, bool join, cudaStream_t s)
 {
-    return D == 64 ? launch_dim<64>(a, fmt, elem, grid, s)
-                   : D == 128 ? launch_dim<128>(a, fmt, elem, grid, s) : launch_dim<256>(a, fmt, elem, grid, s);
+    return D == 64 ? launch_dim<64>(a, fmt, elem, grid, join, s)
+                   : D == 128 ? launch_dim<128>(a, fmt, elem, grid, join, s) : launch_dim<256>(a, fmt, elem, grid, join, s);
 }
 
 uint32_t attn_mma_ctas_per_sm(uint32_t D)
@@ -611,7 +467,28 @@ hxq_error_t check_attention(const hxq_kv_cache_t *c, const hxq_kv_attention_t *p
     return HXQ_OK;
 }
 
-size_t part_bytes(uint32_t D) { return ((size_t)kRows * D + 2 * kRows) * sizeof(float) * 2; }
+// Workspace: a word group for every CTA, then the partial results, of this
+// kernel and of the one for many rows.
+struct AttnLayout {
+    uint32_t ctas, tc_ctas;
+    size_t part, tc_desc, tc_part, bytes;
+};
+
+// Requests with more rows than this go to the tcgen05 kernel.
+constexpr uint32_t kFewRows = 64;
+
+AttnLayout attn_layout(uint32_t D, uint64_t most_rows)
+{
+    AttnLayout l;
+    const uint32_t sms = (uint32_t)sm_count();
+    l.ctas = sms * attn_mma_ctas_per_sm(D);
+    l.tc_ctas = D != 256 && most_rows > kFewRows ? sms : 0;
+    l.part = l.ctas * sizeof(int4);
+    l.tc_desc = l.part + (size_t)l.ctas * 2 * (kRows * D + 2 * kRows) * sizeof(float);
+    l.tc_part = l.tc_desc + l.tc_ctas * sizeof(int4);
+    l.bytes = l.tc_part + (size_t)l.tc_ctas * 2 * (kTcRows * D + 2 * kTcRows) * sizeof(float);
+    return l;
+}
 
 }  // namespace serving
 }  // namespace hxq
@@ -623,8 +500,7 @@ extern "C" {
 size_t hxq_cuda_kv_attention_workspace(const hxq_kv_cache_t *cache, const hxq_kv_attention_t *args)
 {
     if (check_attention(cache, args) != HXQ_OK) return 0;
-    const size_t ctas = (size_t)sm_count() * attn_mma_ctas_per_sm(cache->head_dim);
-    return ctas * (sizeof(int4) + part_bytes(cache->head_dim));
+    return attn_layout(cache->head_dim, (uint64_t)args->max_new * (args->n_heads / cache->n_heads)).bytes;
 }
 
 hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_attention_t *args, void *d_workspace,
@@ -638,7 +514,8 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     if ((((uintptr_t)args->d_q | (uintptr_t)d_workspace) & 15u) != 0 || ((args->q_stride_t | args->q_stride_h) & 7) != 0 ||
         ((uintptr_t)args->d_out & 1u) != 0)
         return HXQ_ERR_INVALID_ARG;
-    if (workspace_bytes < hxq_cuda_kv_attention_workspace(cache, args)) return HXQ_ERR_INVALID_ARG;
+    const AttnLayout lay = attn_layout(cache->head_dim, (uint64_t)args->max_new * (args->n_heads / cache->n_heads));
+    if (workspace_bytes < lay.bytes) return HXQ_ERR_INVALID_ARG;
     AttnArgs a;
     a.q = args->d_q;
     a.out = args->d_out;
@@ -668,14 +545,28 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     a.row_min = 0;
     a.row_max = 0xffffffffu;
     a.scale_log2 = args->scale * 1.4426950408889634f;
-    const uint32_t grid = (uint32_t)sm_count() * attn_mma_ctas_per_sm(cache->head_dim);
-    a.desc = static_cast<int4 *>(d_workspace);
-    a.part = reinterpret_cast<float *>(a.desc + grid);
-    if (launch_attn_mma(a, cache->head_dim, cache->format, args->elem, grid, static_cast<cudaStream_t>(stream)) != cudaSuccess) {
+    uint8_t *ws = static_cast<uint8_t *>(d_workspace);
+    a.desc = reinterpret_cast<int4 *>(ws);
+    a.part = reinterpret_cast<float *>(ws + lay.part);
+    // Few rows of a request: this file's kernel. More: the tcgen05 kernel (64
+    // is where a tile of 16 rows reads the keys four times over; that kernel
+    // takes 128 rows at a time). Without rows of the other kind a launch ends
+    // after its scan of the lengths.
+    if (lay.tc_ctas) a.row_max = kFewRows;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = launch_attn_mma(a, cache->head_dim, cache->format, args->elem, lay.ctas, true, s);
+    if (e == cudaSuccess && lay.tc_ctas) {
+        a.row_min = kFewRows;
+        a.row_max = 0xffffffffu;
+        a.desc = reinterpret_cast<int4 *>(ws + lay.tc_desc);
+        a.part = reinterpret_cast<float *>(ws + lay.tc_part);
+        e = launch_attn_tc(a, cache->head_dim, cache->format, args->elem, lay.tc_ctas, s);
+    }
+    if (e != cudaSuccess) {
         cudaGetLastError();
         return HXQ_ERR_CUDA;
     }
-    return launched(2);
+    return launched(lay.tc_ctas ? 4 : 2);
 }
 
 }  // extern "C"
