@@ -34,6 +34,7 @@ namespace serving {
 
 constexpr int kRows = 16;        // rows of a tile
 constexpr int kGran = 64;        // keys of a granule
+constexpr int kFixed = 2;        // granules that a unit costs by itself
 constexpr int kWarpsA = 4;
 constexpr int kThreadsA = kWarpsA * 32;
 
@@ -48,7 +49,8 @@ template <int D> struct Geo {
     static constexpr int kRing = kWarpsA * kStages * kSlot;
     static constexpr int kPad = 4;
     static constexpr int kMerge = kWarpsA * kRows * (D + kPad) * 4;
-    static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQSmem;
+    static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQSmem;   // at least the scan's 4 (B + 1) bytes
+    static_assert(kSmem >= 4 * (HXQ_ATTENTION_MAX_REQUESTS + 1), "room for the scan");
     static constexpr int kCtas = D == 256 ? 2 : 3;
 };
 
@@ -86,17 +88,18 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
 
     if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     Range range;
-    if (!find_range<kWarpsA, kRows, kGran>(a, sh, true, range)) return;
+    if (!find_range<kWarpsA, kRows, kGran, kFixed>(a, sh, reinterpret_cast<uint32_t *>(smem), true, range)) return;
+    __syncthreads();   // the sums in front of the requests are read: the ring may be filled
     const uint32_t ring = pipe::smem_u32(smem) + warp * (G::kStages * G::kSlot);
     uint4 *qs = reinterpret_cast<uint4 *>(smem + (G::kSmem - G::kQSmem));
     float *merge = reinterpret_cast<float *>(smem);
     const uint32_t bh_bytes = a.P * D;
 
     Segment seg;
-    while (next_segment<kRows, kGran>(a, range, seg)) {
+    while (next_segment<kRows, kGran, kFixed>(a, range, seg)) {
         const Req &r = seg.r;
         const uint32_t h = seg.h, take = seg.take, hi = seg.hi, r0 = seg.r0, r1 = seg.r1;
-        const uint32_t key0 = (seg.first + seg.rem) * kGran + warp * 16;   // this warp's first 16 keys
+        const uint32_t key0 = seg.key0 + warp * 16;   // this warp's first 16 keys
 
         // ---- Q: rows g and g + 8, in the order in which codes arrive
         uint32_t qf[G::kQSmem ? 1 : D / 16][4];
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
             for (int i = 0; i < 2; ++i) {
                 const uint32_t row = r0 + g + 8 * i;
                 const bool in = row < r1;
-                const uint32_t tok = in ? row / a.G : 0, head = h * a.G + (in ? row % a.G : 0);
+                const uint32_t tok = in ? token_of(a, row) : 0, head = h * a.G + (in ? row - tok * a.G : 0);
                 pos[i] = in ? (a.causal ? (int32_t)((int64_t)r.len - r.n + tok) : (int32_t)r.len - 1) : -1;
                 const QT *p = static_cast<const QT *>(a.q) + (int64_t)(r.q0 + tok) * a.q_st + (int64_t)head * a.q_sh;
                 uint32_t top = 0;
@@ -156,8 +159,8 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
             }
             if (G::kQSmem) __syncthreads();
         }
-        const int32_t pos_first = a.causal ? (int32_t)((int64_t)r.len - r.n + r0 / a.G) : (int32_t)r.len - 1;
-        const int32_t pos_last = a.causal ? (int32_t)((int64_t)r.len - r.n + (r1 - 1) / a.G) : (int32_t)r.len - 1;
+        const int32_t pos_first = a.causal ? (int32_t)((int64_t)r.len - r.n + token_of(a, r0)) : (int32_t)r.len - 1;
+        const int32_t pos_last = a.causal ? (int32_t)((int64_t)r.len - r.n + token_of(a, r1 - 1)) : (int32_t)r.len - 1;
         // a row sees keys above its floor: its position less the window, -1 without one
         auto key_floor = [&](int32_t at) { return a.window ? (int32_t)max((int64_t)at - (int64_t)a.window, (int64_t)-1) : -1; };
         const int32_t floor_last = key_floor(pos_last), floors[2] = {key_floor(pos[0]), key_floor(pos[1])};
@@ -173,7 +176,8 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
         const int32_t *row = a.table + (size_t)seg.b * a.width;
         auto entry = [&](uint32_t j) -> int32_t {
             const uint32_t key = key0 + j * kGran;
-            return j < take && key < hi ? __ldg(row + key / a.P) : -1;
+            uint32_t slot;
+            return j < take && key < hi ? __ldg(row + block_of(a, key, slot)) : -1;
         };
         auto issue = [&](uint32_t j, uint32_t stage, int32_t blk) {
             const uint32_t key = key0 + j * kGran;
@@ -183,7 +187,9 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
             valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
             if (ok) {
                 const size_t bh = (size_t)(uint32_t)blk * a.H + h;
-                const size_t base = bh * bh_bytes + (size_t)(key % a.P) * D;
+                uint32_t slot;
+                block_of(a, key, slot);
+                const size_t base = bh * bh_bytes + (size_t)slot * D;
                 const uint32_t dst = ring + stage * G::kSlot + lane * 16;
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt)
@@ -374,8 +380,8 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
                 mine[(g + (e >> 1) * 8) * (D + G::kPad) + d + (2 * q + (e & 1)) * G::kVB] = o[t][e] * wt[e >> 1];
         }
         __syncthreads();
-        const bool whole = seg.rem == 0 && take == seg.n;
-        float *part = a.part + (size_t)(2 * blockIdx.x + (seg.rem == 0 ? 1 : 0)) * part_floats<kRows, D>();
+        const bool whole = seg.begins && take == seg.n;
+        float *part = a.part + (size_t)(2 * blockIdx.x + (seg.begins ? 1 : 0)) * part_floats<kRows, D>();
         for (uint32_t i = tid; i < kRows * (D / 4); i += kThreadsA) {
             const uint32_t rr = i / (D / 4), d = (i % (D / 4)) * 4;
             if (r0 + rr >= r1) break;
@@ -393,7 +399,7 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
 #pragma unroll
             for (int w = 0; w < kWarpsA; ++w) sum += top == -INFINITY ? sh_l[w][rr] : sh_l[w][rr] * ex2(sh_m[w][rr] - top);
             if (whole) {
-                const uint32_t tok = r.q0 + (r0 + rr) / a.G, head = h * a.G + (r0 + rr) % a.G;
+                const uint32_t tk = token_of(a, r0 + rr), tok = r.q0 + tk, head = h * a.G + (r0 + rr - tk * a.G);
                 const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
                 QT *dst = static_cast<QT *>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + d;
                 dst[0] = Elem<QT>::from(v.x * f);
@@ -410,7 +416,7 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
                 }
             }
         }
-        if (seg.rem == 0 && take < seg.n && tid == 0) a.desc[blockIdx.x] = cut_unit(range, seg);
+        if (seg.begins && take < seg.n && tid == 0) a.desc[blockIdx.x] = cut_unit(range, seg);
         __syncthreads();   // the ring is free again
     }
 }
@@ -538,6 +544,8 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     a.H = cache->n_heads;
     a.G = args->n_heads / cache->n_heads;
     a.P = cache->block_tokens;
+    a.pmul = a.P == 16 ? 0u : (uint32_t)(((1ull << 32) + a.P / 16 - 1) / (a.P / 16));
+    a.gmul = a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G);
     a.n_blocks = cache->n_blocks;
     a.width = args->table_width;
     a.window = args->window;

@@ -18,6 +18,8 @@ struct AttnArgs {
     uint32_t *status;
     uint32_t B, T, Hq, H, G, P, n_blocks, width, window;
     uint32_t causal;
+    uint32_t pmul;               // 2^32 / (P / 16), rounded up; 0 for P = 16
+    uint32_t gmul;               // 2^32 / G, rounded up; 0 for G = 1
     uint32_t row_min, row_max;   // requests with row_min < rows <= row_max are this launch's
     float scale_log2;            // scale * log2(e)
     float *part;                 // partial results
@@ -44,6 +46,23 @@ __device__ __forceinline__ Req load_req(const AttnArgs &a, uint32_t b)
     return r;
 }
 
+// row / G: the product with the rounded-up inverse is right or one too large.
+__device__ __forceinline__ uint32_t token_of(const AttnArgs &a, uint32_t row)
+{
+    if (a.gmul == 0) return row;
+    const uint32_t q = __umulhi(row, a.gmul);
+    return q - (q * a.G > row);
+}
+
+// Block of a request that a 16-aligned key is in, and its slot there
+// (exact: key / 16 < 2^27, P / 16 <= 16).
+__device__ __forceinline__ uint32_t block_of(const AttnArgs &a, uint32_t key, uint32_t &slot)
+{
+    const uint32_t k16 = key >> 4, b = a.pmul ? __umulhi(k16, a.pmul) : k16;
+    slot = (k16 - b * (a.P >> 4)) << 4;
+    return b;
+}
+
 // Called by one CTA of a launch: what was out of range is recorded.
 __device__ __forceinline__ void flag_req(const AttnArgs &a, uint32_t b)
 {
@@ -56,14 +75,14 @@ __device__ __forceinline__ void flag_req(const AttnArgs &a, uint32_t b)
 __device__ __forceinline__ void key_range(const AttnArgs &a, const Req &r, uint32_t r0, uint32_t r1, uint32_t &lo,
                                           uint32_t &hi)
 {
-    const int64_t before = (int64_t)r.len - r.n;   // position of the request's first row
+    const int32_t before = (int32_t)r.len - (int32_t)r.n;   // position of the request's first row
     lo = 0;
     hi = r.len;
     if (a.causal) {
-        const int64_t last = before + (r1 - 1) / a.G + 1;
-        hi = last < 0 ? 0u : last < (int64_t)r.len ? (uint32_t)last : r.len;
+        const int32_t last = before + (int32_t)token_of(a, r1 - 1) + 1;
+        hi = (uint32_t)min(max(last, 0), (int32_t)r.len);
         if (a.window) {
-            const int64_t first = before + r0 / a.G - (int64_t)a.window + 1;
+            const int64_t first = (int64_t)before + token_of(a, r0) - a.window + 1;
             lo = first > 0 ? (uint32_t)first : 0u;
         }
     }
@@ -72,7 +91,8 @@ __device__ __forceinline__ void key_range(const AttnArgs &a, const Req &r, uint3
 
 // The work of a launch: units (request, cache head, tile of ROWS rows) end to
 // end, each as many granules of KEYS keys as its rows may see (one if none:
-// the rows are written all the same), cut into one range for every CTA.
+// the rows are written all the same) behind FIXED ones that stand for the
+// time a unit costs by itself, cut into one range for every CTA.
 template <int ROWS, int KEYS> __device__ __forceinline__ uint32_t tile_grans(const AttnArgs &a, const Req &r, uint32_t t, uint32_t &first)
 {
     uint32_t lo, hi;
@@ -82,83 +102,114 @@ template <int ROWS, int KEYS> __device__ __forceinline__ uint32_t tile_grans(con
     return last > first ? last - first : 1u;
 }
 
-template <int ROWS, int KEYS> __device__ __forceinline__ uint64_t req_grans(const AttnArgs &a, const Req &r, uint32_t &most)
-{
-    uint64_t sum = 0;
-    uint32_t first;
-    for (uint32_t t = 0; t * ROWS < r.rows; ++t) {
-        const uint32_t n = tile_grans<ROWS, KEYS>(a, r, t, first);
-        sum += n;
-        most = max(most, n);
-    }
-    return sum;
-}
-
 // Most parts of a unit that the joining kernel adds up.
 constexpr uint32_t kMaxParts = 128;
 
 template <int WARPS> struct RangeShared {
     uint64_t scan[WARPS];
     uint32_t most[WARPS];
-    uint32_t b;
+    uint32_t b, tile;
     uint64_t off;
 };
 
-// A position in the work: granule x of all, granule off of request b's.
+// A position in the work: granule x of all, up to x1 for this CTA; request b,
+// tile, cache head h, granule rem of that unit's n.
 struct Range {
-    uint64_t x, x1, off, total, ctas;
-    uint32_t b;
+    uint64_t x, x1, total, ctas;
+    Req r;
+    uint32_t b, tile, h, n, first, rem;
 };
 
-// This CTA's range, by a block scan over the requests; false: it has none.
-// `record`: whether what is out of range is recorded (one launch of a call).
-template <int WARPS, int ROWS, int KEYS>
-__device__ __forceinline__ bool find_range(const AttnArgs &a, RangeShared<WARPS> &sh, bool record, Range &out)
+// This CTA's range; false: it has none. Requests' tiles are numbered through
+// (a block scan, the sums in `pre`, B + 1 words of shared memory), then every
+// thread counts the granules of some consecutive tiles (another scan), so a
+// single long prompt is counted by all threads.  Heads of a tile follow each
+// other.  `record`: whether what is out of range is recorded (one launch of a
+// call).
+template <int WARPS, int ROWS, int KEYS, int FIXED>
+__device__ __forceinline__ bool find_range(const AttnArgs &a, RangeShared<WARPS> &sh, uint32_t *pre, bool record, Range &out)
 {
     constexpr uint32_t N = WARPS * 32;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t per = (a.B + N - 1) / N, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-    uint64_t mine = 0;
-    uint32_t most = 1;
-    for (uint32_t i = b0; i < b1; ++i) {
-        mine += req_grans<ROWS, KEYS>(a, load_req(a, i), most) * a.H;
-        if (record && blockIdx.x == 0) flag_req(a, i);
-    }
-    uint64_t incl = mine;
+    auto scan = [&](uint64_t mine, uint64_t &total) {   // the sum in front of this thread
+        uint64_t incl = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const uint64_t u = __shfl_up_sync(~0u, incl, d);
-        if (lane >= (uint32_t)d) incl += u;
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint64_t u = __shfl_up_sync(~0u, incl, d);
+            if (lane >= (uint32_t)d) incl += u;
+        }
+        if (lane == 31) sh.scan[warp] = incl;
+        __syncthreads();
+        uint64_t before = 0;
+        total = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < WARPS; ++w) {
+            if (w < warp) before += sh.scan[w];
+            total += sh.scan[w];
+        }
+        return before + incl - mine;
+    };
+    uint64_t tiles;
+    {
+        const uint32_t per = (a.B + N - 1) / N, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+        uint32_t mine = 0;
+        for (uint32_t i = b0; i < b1; ++i) {
+            mine += (load_req(a, i).rows + ROWS - 1) / ROWS;
+            if (record && blockIdx.x == 0) flag_req(a, i);
+        }
+        uint32_t at = (uint32_t)scan(mine, tiles);
+        for (uint32_t i = b0; i < b1; ++i) {
+            pre[i] = at;
+            at += (load_req(a, i).rows + ROWS - 1) / ROWS;
+        }
+        if (tid == 0) { pre[a.B] = (uint32_t)tiles; sh.b = a.B; }
+        __syncthreads();
+    }
+    if (tiles == 0) return false;
+    const uint32_t per = ((uint32_t)tiles + N - 1) / N, p0 = min(tid * per, (uint32_t)tiles), p1 = min(p0 + per, (uint32_t)tiles);
+    uint32_t lo = 0, most = 1, first;
+    uint64_t mine = 0;
+    if (p0 < p1) {
+        uint32_t hi = a.B;   // the last request with pre <= p0: it has tiles
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (pre[mid] <= p0) lo = mid;
+            else hi = mid;
+        }
+        Req r = load_req(a, lo);
+        for (uint32_t p = p0, b = lo; p < p1; ++p) {
+            if (p >= pre[b + 1]) {
+                while (p >= pre[b + 1]) ++b;
+                r = load_req(a, b);
+            }
+            const uint32_t n = FIXED + tile_grans<ROWS, KEYS>(a, r, p - pre[b], first);
+            mine += (uint64_t)n * a.H;
+            most = max(most, n);
+        }
     }
     most = __reduce_max_sync(~0u, most);
-    if (lane == 31) {
-        sh.scan[warp] = incl;
-        sh.most[warp] = most;
-    }
-    if (tid == 0) { sh.b = a.B; sh.off = 0; }
-    __syncthreads();
-    uint64_t total = 0, before = 0;
+    if (lane == 31) sh.most[warp] = most;
+    uint64_t at = scan(mine, out.total);
 #pragma unroll
-    for (uint32_t w = 0; w < WARPS; ++w) {
-        if (w < warp) before += sh.scan[w];
-        total += sh.scan[w];
-        most = max(most, sh.most[w]);
-    }
-    const uint64_t least = max(1u, (most + kMaxParts - 1) / kMaxParts);   // granules a CTA takes at least
-    uint64_t n = (total + least - 1) / least;
+    for (uint32_t w = 0; w < WARPS; ++w) most = max(most, sh.most[w]);
+    const uint64_t least = (most + kMaxParts - 1) / kMaxParts;   // granules a CTA takes at least
+    uint64_t n = (out.total + least - 1) / least;
     n = n < gridDim.x ? n : gridDim.x;
     if (blockIdx.x >= n) return false;
-    out.x = total * blockIdx.x / n;
-    out.x1 = total * (blockIdx.x + 1) / n;
-    out.total = total;
+    out.x = out.total * blockIdx.x / n;
+    out.x1 = out.total * (blockIdx.x + 1) / n;
     out.ctas = n;
-    incl += before;
-    if (incl - mine <= out.x && out.x < incl) {
-        uint64_t at = incl - mine;
-        for (uint32_t i = b0; i < b1; ++i) {
-            const uint64_t w = req_grans<ROWS, KEYS>(a, load_req(a, i), most) * a.H;
+    if (at <= out.x && out.x < at + mine) {
+        Req r = load_req(a, lo);
+        for (uint32_t p = p0, b = lo; p < p1; ++p) {
+            if (p >= pre[b + 1]) {
+                while (p >= pre[b + 1]) ++b;
+                r = load_req(a, b);
+            }
+            const uint64_t w = (uint64_t)(FIXED + tile_grans<ROWS, KEYS>(a, r, p - pre[b], first)) * a.H;
             if (out.x < at + w) {
-                sh.b = i;
+                sh.b = b;
+                sh.tile = p - pre[b];
                 sh.off = out.x - at;
                 break;
             }
@@ -167,55 +218,69 @@ __device__ __forceinline__ bool find_range(const AttnArgs &a, RangeShared<WARPS>
     }
     __syncthreads();
     out.b = sh.b;
-    out.off = sh.off;
+    if (out.b >= a.B) return false;   // never: the ranges cover all granules
+    out.tile = sh.tile;
+    out.r = load_req(a, out.b);
+    out.n = FIXED + tile_grans<ROWS, KEYS>(a, out.r, out.tile, out.first);
+    out.h = (uint32_t)(sh.off / out.n);
+    out.rem = (uint32_t)(sh.off - (uint64_t)out.h * out.n);
     return true;
 }
 
 // The part of a unit that a range has next.
 struct Segment {
     Req r;
-    uint32_t b, h, tile, first, rem, n, take, r0, r1, lo, hi;   // granules first + rem .. + take of the unit's n
+    uint32_t b, h, tile, key0, take, r0, r1, lo, hi, n;   // granules from key key0 on, of the unit's n
+    bool begins;                                          // with the unit's first granule
+    uint64_t end;                                         // of the unit, in the numbering of all granules
 };
 
-template <int ROWS, int KEYS> __device__ __forceinline__ bool next_segment(const AttnArgs &a, Range &w, Segment &s)
+template <int ROWS, int KEYS, int FIXED> __device__ __forceinline__ bool next_segment(const AttnArgs &a, Range &w, Segment &s)
 {
     while (w.x < w.x1 && w.b < a.B) {
-        s.r = load_req(a, w.b);
-        uint32_t most = 0;
-        const uint64_t sum = req_grans<ROWS, KEYS>(a, s.r, most);
-        if (w.off >= sum * a.H) {
-            w.off -= sum * a.H;
-            ++w.b;
-            continue;
-        }
+        // granules of keys among those that are left, of the unit's n
+        const uint32_t from = w.rem > FIXED ? w.rem - FIXED : 0u, step = (uint32_t)min((uint64_t)(w.n - w.rem), w.x1 - w.x);
+        const uint32_t to = w.rem + step > FIXED ? w.rem + step - FIXED : 0u;
+        s.r = w.r;
         s.b = w.b;
-        s.h = (uint32_t)(w.off / sum);
-        s.rem = (uint32_t)(w.off - s.h * sum);
-        s.tile = 0;
-        while (true) {
-            s.n = tile_grans<ROWS, KEYS>(a, s.r, s.tile, s.first);
-            if (s.rem < s.n) break;
-            s.rem -= s.n;
-            ++s.tile;
+        s.h = w.h;
+        s.tile = w.tile;
+        s.n = w.n - FIXED;
+        s.begins = from == 0;
+        s.key0 = (w.first + from) * KEYS;
+        s.take = to - from;
+        w.x += step;
+        w.rem += step;
+        s.end = w.x + (w.n - w.rem);
+        if (w.rem == w.n && w.x < w.x1) {
+            w.rem = 0;
+            if (++w.h == a.H) {
+                w.h = 0;
+                if (++w.tile * ROWS >= w.r.rows) {
+                    w.tile = 0;
+                    while (++w.b < a.B) {
+                        w.r = load_req(a, w.b);
+                        if (w.r.rows) break;
+                    }
+                }
+                if (w.b < a.B) w.n = FIXED + tile_grans<ROWS, KEYS>(a, w.r, w.tile, w.first);
+            }
         }
-        s.take = (uint32_t)min((uint64_t)(s.n - s.rem), w.x1 - w.x);
+        if (s.take == 0) continue;   // the range ends before the unit's first keys: the next CTA begins it
         s.r0 = s.tile * ROWS;
         s.r1 = min(s.r0 + ROWS, s.r.rows);
         key_range(a, s.r, s.r0, s.r1, s.lo, s.hi);
-        w.x += s.take;
-        w.off += s.take;
         return true;
     }
     return false;
 }
 
 // For the joining kernel, when a segment begins a unit and does not end it:
-// how many ranges the unit lies in. (w is already behind the segment.)
+// how many ranges, from this one on, the unit lies in.
 __device__ __forceinline__ int4 cut_unit(const Range &w, const Segment &s)
 {
-    const uint64_t end = w.x - s.take + s.n;
     uint64_t c = blockIdx.x + 1;
-    while (w.total * (c + 1) / w.ctas < end) ++c;
+    while (w.total * (c + 1) / w.ctas < s.end) ++c;
     return make_int4((int)(c - blockIdx.x + 1), (int)s.b, (int)s.h, (int)s.tile);
 }
 
@@ -231,6 +296,32 @@ __device__ __forceinline__ float lg2(float x)
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two fp32 at a time.
+__device__ __forceinline__ uint64_t pack2(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b)
@@ -306,7 +397,7 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const int4 *desc, co
         for (int j = 0; j < N; ++j) v[j] += p[rr * D + j * 32 + lane] * w;
     }
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const uint32_t tok = r.q0 + row / a.G, head = (uint32_t)d.z * a.G + row % a.G;
+    const uint32_t tk = token_of(a, row), tok = r.q0 + tk, head = (uint32_t)d.z * a.G + (row - tk * a.G);
     QT *dst = static_cast<QT *>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
 #pragma unroll
     for (int j = 0; j < N; ++j) dst[j * 32 + lane] = Elem<QT>::from(v[j] * f);

@@ -5,24 +5,26 @@
 // inside the exponent and the row sums.  A CTA takes 256 rows (tokens x heads
 // of a group) of one (request, cache head), two tiles of 128, against 128 keys
 // at a time:
-//   warps 0-7   one row per thread (tile = warp / 4): Q scaled into f16 and
-//               into shared memory once, then for every 128 keys the scores
-//               out of tensor memory, exp2, weights back into tensor memory
-//               as f16 over the scores' columns; at the end the row out;
-//   warps 8-11  codes: global memory -> registers (one step ahead) -> f16 ->
+//   warps 0-15  two threads a row (tile = warp / 8), each for half of the keys:
+//               Q scaled into f16 and into shared memory once, then for every
+//               128 keys the scores out of tensor memory, exp2, weights back
+//               into tensor memory as f16 over the scores' columns; at the
+//               end the row out, through Q's place so that stores coalesce;
+//   warps 16-19 codes: shared memory (as they are in the cache) -> f16 ->
 //               shared memory, keys [key][dim] and values transposed
-//               [dim][key], both K-major with 128-byte swizzle; the block
-//               scales of every 16 keys;
-//   warp 12     one thread issues S = Q K^T (both operands in shared memory)
-//               and O += P V (P in tensor memory).
+//               [dim][key], both K-major with 128-byte swizzle;
+//   warp 20     one thread issues S = Q K^T (both operands in shared memory)
+//               and O += P V (P in tensor memory);
+//   warp 21     a lane for every 16 keys looks up their block, copies its
+//               codes to shared memory (cp.async.bulk) and its scales;
+//   warp 22     one thread cuts the CTA's range into segments for the others.
 // The two tiles take turns: while one is at its exponentials, the tensor
 // cores work for the other.  Tensor memory: S/P of tile t at column 128 t,
 // O of tile t at 256 + 128 t, all 512 columns, one CTA an SM.
 //
-// The running maximum is lazy: weights are taken against the maximum so far
-// and only where one would pass 2^8 (f16 holds 2^16) is it raised and O
-// rescaled, which after the first keys is rare, so that the rescale needs no
-// warps of its own and the scores are read from tensor memory once.
+// The running maximum is lazy: it is raised, and O rescaled, only where a
+// weight would pass 2^8 (f16 holds 2^16), which after the first keys is rare,
+// so that the rescale needs no warps of its own.
 //
 // Work is cut and joined as in kv_attention.cu, with granules of 128 keys.
 // Every wait is bounded; one that runs out is recorded and the CTA unwinds.
@@ -35,18 +37,27 @@ namespace serving {
 
 constexpr int kKeys = 128;                 // keys of a step
 constexpr int kTile = 128;                 // rows of a tile
-constexpr int kSoftWarps = 8, kConvWarps = 4;
-constexpr int kWarpsT = kSoftWarps + kConvWarps + 1;
+constexpr int kFixedT = 2;                 // steps that a unit costs by itself
+constexpr int kSoftWarps = 16, kConvWarps = 4;
+constexpr int kMmaWarp = kSoftWarps + kConvWarps, kLoadWarp = kMmaWarp + 1, kPlanWarp = kMmaWarp + 2;
+constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups; the last warp has nothing to do
+// Registers: launched with 80 a thread, 61,440 in all; the rows' threads hold
+// 64 scores. 512 x 96 + 128 x 56 + 128 x 40 = 61,440.
+constexpr int kRegsSoft = 96, kRegsConv = 56, kRegsRest = 40;
 constexpr int kThreadsT = kWarpsT * 32;
-constexpr int kScaleSlots = 4;
+constexpr int kScaleSlots = 4, kSegSlots = 2;
 constexpr float kRaise = 8.0f;             // log2 of the largest weight before the maximum is raised
 
 template <int D> struct TcGeo {
     static constexpr int kQ = kTile * D * 2;           // bytes of a tile of Q
     static constexpr int kK = kKeys * D * 2;           // of a step's keys, and of its values
-    static constexpr int kOffK = 2 * kQ, kOffV = kOffK + 2 * kK, kOffS = kOffV + 2 * kK;
-    static constexpr int kOffBar = kOffS + kScaleSlots * 8 * 16;
-    static constexpr int kSmem = kOffBar + 256 + 1024;
+    static constexpr int kRaw = kKeys * D;             // bytes of their codes
+    static constexpr int kOffK = 2 * kQ, kOffV = kOffK + 2 * kK, kOffRaw = kOffV + 2 * kK, kOffS = kOffRaw + 2 * kRaw;
+    static constexpr int kOffSeg = kOffS + kScaleSlots * 8 * 16, kOffBar = kOffSeg + kSegSlots * 64;
+    static constexpr int kOffTop = kOffBar + 320;      // a float for every row of both tiles and halves
+    static constexpr int kSmem = kOffTop + 2 * 2 * kTile * 4;
+    static_assert(kSmem <= 232448, "shared memory");
+    static_assert(kOffS - 1024 >= 4 * (HXQ_ATTENTION_MAX_REQUESTS + 1) && sizeof(RangeShared<kWarpsT>) <= 1024, "room for the scan");
     static constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
     static constexpr uint32_t kIdescPV = (1u << 4) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 };
@@ -81,29 +92,46 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t (&v)[32])
+__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t *v)
 {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-        "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr)
-        : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
+                 "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+                 "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
+                 "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(taddr)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t *v)
 {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-        "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+                 "%32};" ::"r"(taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+                 "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
+                 "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
+                 "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 : "memory");
+}
+
+__device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tm_st8(uint32_t taddr, const uint32_t *v)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w)
@@ -112,54 +140,84 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 }
 
 struct Bars {
-    uint64_t q_full[2], s_full[2], p_full[2], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2], drained;
-    uint32_t tmem, abort;
+    uint64_t q_full[2], s_full[2], p_full[2], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t rawk_full, rawk_empty, rawv_full, rawv_empty, seg_full[kSegSlots], seg_empty[kSegSlots], drained;
+    uint32_t tmem;
+    uint32_t live[2], zero[2][8];   // of a raw step (by its parity): keys within the range (0: no more steps), value groups that count as 0
 };
+static_assert(sizeof(Bars) <= 320, "room for the barriers");
 
-// Bounded wait; false once it, or another one of the CTA, has run out.
-struct Waiter {
-    Bars *bars;
-    uint32_t *status;
-    __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity) const
-    {
-        if (pipe::mbar_try(bar, parity)) return true;
-        const uint64_t t0 = clock64();
-        while (!pipe::mbar_try(bar, parity)) {
-            if (*(volatile uint32_t *)&bars->abort) return false;
-            if (clock64() - t0 > pipe::kWaitCycles) {
-                *(volatile uint32_t *)&bars->abort = 1u;
-                flag(status, HXQ_SERVING_TIMEOUT);
-                return false;
-            }
-        }
-        return true;
-    }
+// What the warps need of a segment; take 0: no more of them.
+struct SegInfo {
+    uint32_t take, take0;            // steps, and those that tile 0 takes part in
+    uint32_t key0, hi, r0, r1, q0, h, b;
+    int32_t before;                  // position of the request's first row
+    uint32_t len, whole;
+    int4 cut;                        // for the joining kernel, where the segment begins a unit and doesn't end it
 };
+static_assert(sizeof(SegInfo) == 64, "a slot");
 
-// A step of 128 keys within the CTA's range, for the converters, which run
-// ahead of the other warps.
-struct Cursor {
-    Range range;
-    Segment seg;
-    uint32_t j;
-    bool ok;
-    __device__ __forceinline__ void next(const AttnArgs &a)
-    {
-        if (!ok) return;
-        if (++j >= seg.take) {
-            ok = next_segment<kTcRows, kKeys>(a, range, seg);
-            j = 0;
+// Bounded wait (2^21 tries of up to a microsecond, in which the thread is
+// suspended); false if it ran out.
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
+        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t@p bra DONE_%=;\n\t"
+        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 2097152;\n\t@q bra AGAIN_%=;\n"
+        "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(pipe::smem_u32(bar)), "r"(parity), "r"(1000u)
+        : "memory");
+    return ok != 0;
+}
+
+__device__ __forceinline__ void named_sync(uint32_t id, uint32_t threads)
+{
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Largest of 16 scores.
+__device__ __forceinline__ float largest16(const uint32_t *s)
+{
+    float m[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+        m[i] = fmaxf(fmaxf(__uint_as_float(s[3 * i]), __uint_as_float(s[3 * i + 1])), __uint_as_float(s[3 * i + 2]));
+    return fmaxf(fmaxf(fmaxf(m[0], m[1]), m[2]), fmaxf(fmaxf(m[3], m[4]), __uint_as_float(s[15])));
+}
+
+// Weights of 16 scores, as f16 pairs (MASK: 0 for keys that the row may not
+// see, whatever the scales of their block); their sum is returned.
+template <bool MASK>
+__device__ __forceinline__ float weigh16(const uint32_t *s, float f, float off, uint32_t *p, int32_t key, int32_t pos, int32_t floor)
+{
+    const uint64_t f2 = pack2(f, f), off2 = pack2(off, off);
+    uint64_t sum2 = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+        float2 t = unpack2(fma2(pack2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), f2, off2));
+        if (MASK) {
+            if (key + i > pos || key + i <= floor) t.x = -INFINITY;
+            if (key + i + 1 > pos || key + i + 1 <= floor) t.y = -INFINITY;
         }
+        const float w0 = ex2(t.x), w1 = ex2(t.y);
+        sum2 = i == 0 ? pack2(w0, w1) : add2(sum2, pack2(w0, w1));
+        const __half2 h = __floats2half2_rn(w0, w1);
+        p[i / 2] = *reinterpret_cast<const uint32_t *>(&h);
     }
-};
+    const float2 sum = unpack2(sum2);
+    return sum.x + sum.y;
+}
 
 template <int D, int FMT, typename QT>
 __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_constant__ AttnArgs a)
 {
     using G = TcGeo<D>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = smem_raw + ((1024u - (pipe::smem_u32(smem_raw) & 1023u)) & 1023u);
-    __shared__ RangeShared<kWarpsT> sh;
+    extern __shared__ __align__(1024) uint8_t smem[];   // the kernel has no other shared memory: it begins on 1024
+    RangeShared<kWarpsT> &sh = *reinterpret_cast<RangeShared<kWarpsT> *>(smem + G::kOffS - 1024);
+    SegInfo *segs = reinterpret_cast<SegInfo *>(smem + G::kOffSeg);
     Bars *bars = reinterpret_cast<Bars *>(smem + G::kOffBar);
     float4 *scales = reinterpret_cast<float4 *>(smem + G::kOffS);   // [slot][16-key group]: ks, log2 vs, 1 / vs
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -167,23 +225,30 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
 
     if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     Range range;
-    if (!find_range<kWarpsT, kTcRows, kKeys>(a, sh, false, range)) return;
+    if (!find_range<kWarpsT, kTcRows, kKeys, kFixedT>(a, sh, reinterpret_cast<uint32_t *>(smem), false, range)) return;
     if (tid == 0) {
         for (int t = 0; t < 2; ++t) {
-            pipe::mbar_init(&bars->q_full[t], kTile);
+            pipe::mbar_init(&bars->q_full[t], 2 * kTile);
             pipe::mbar_init(&bars->s_full[t], 1);
-            pipe::mbar_init(&bars->p_full[t], kTile);
+            pipe::mbar_init(&bars->p_full[t], 2 * kTile);
             pipe::mbar_init(&bars->o_done[t], 1);
             pipe::mbar_init(&bars->k_full[t], kConvWarps * 32);
             pipe::mbar_init(&bars->k_empty[t], 1);
             pipe::mbar_init(&bars->v_full[t], kConvWarps * 32);
             pipe::mbar_init(&bars->v_empty[t], 1);
         }
+        pipe::mbar_init(&bars->rawk_full, 8);
+        pipe::mbar_init(&bars->rawk_empty, kConvWarps);
+        pipe::mbar_init(&bars->rawv_full, 8);
+        pipe::mbar_init(&bars->rawv_empty, kConvWarps);
+        for (int i = 0; i < kSegSlots; ++i) {
+            pipe::mbar_init(&bars->seg_full[i], 1);
+            pipe::mbar_init(&bars->seg_empty[i], kSoftWarps + 2);   // the rows' warps, loads, products
+        }
         pipe::mbar_init(&bars->drained, 1);
-        bars->abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kWarpsT - 1) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pipe::smem_u32(&bars->tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -191,148 +256,151 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
     __syncthreads();
     fence_after();
     const uint32_t tmem = bars->tmem;
-    const Waiter wait{bars, a.status};
 
+    bool ok = true;
     if (warp < kSoftWarps) {
         // ------------------------------------------------------- rows
-        const uint32_t t = warp >> 2, rr = tid & (kTile - 1);          // tile, row of it
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
+        const uint32_t t = warp >> 3, hf = warp >> 2 & 1u, rr = tid & (kTile - 1);   // tile, half of the keys, row of the tile
         const uint32_t lanes = (warp & 3u) << 21;                      // this warp's 32 lanes of tensor memory
-        const uint32_t tS = tmem + lanes + t * 128u, tO = tmem + lanes + 256u + t * 128u;
-        uint32_t n_q = 0, n_s = 0;                                     // Q tiles and steps so far
+        const uint32_t tS = tmem + lanes + t * 128u + hf * 64u, tP = tmem + lanes + t * 128u + hf * 32u;
+        const uint32_t tO = tmem + lanes + 256u + t * 128u + hf * (D / 2);
+        const uint32_t pair = 1 + t * 4 + (warp & 3u), whole_tile = 9 + t;           // named barriers: 64 and 256 threads
+        float *tops = reinterpret_cast<float *>(smem + G::kOffTop) + t * 2 * kTile;
+        const uint32_t qt = base + t * G::kQ;
+        uint32_t n_s = 0;                                              // steps of this tile so far
         uint32_t step0 = 0;                                            // CTA's steps before this segment
-        Segment seg;
-        bool ok = true;
-        while (ok && next_segment<kTcRows, kKeys>(a, range, seg)) {
-            const Req &r = seg.r;
-            if (t == 1 && seg.r1 - seg.r0 <= (uint32_t)kTile) {
+        for (uint32_t si = 0;; ++si) {
+            const SegInfo &seg = segs[si % kSegSlots];
+            ok = __all_sync(~0u, wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u));
+            if (!ok || seg.take == 0) break;
+            const uint32_t take = t == 0 ? seg.take0 : seg.take, key_first = seg.key0;
+            const uint32_t tr0 = seg.r0 + t * kTile, r1 = seg.r1;
+            if (tr0 >= r1) {
                 step0 += seg.take;
+                __syncwarp();
+                if (lane == 0) pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
                 continue;
             }
-            const uint32_t tr0 = seg.r0 + t * kTile, tr1 = min(tr0 + kTile, seg.r1), row = tr0 + rr;
-            const bool in = row < tr1;
-            const int32_t before = (int32_t)((int64_t)r.len - r.n);
-            auto position = [&](uint32_t rw) { return a.causal ? before + (int32_t)(rw / a.G) : (int32_t)r.len - 1; };
+            const uint32_t tr1 = min(tr0 + kTile, r1);
+            const int32_t before = seg.before, last = (int32_t)seg.len - 1;
+            auto position = [&](uint32_t rw) { return a.causal ? before + (int32_t)token_of(a, rw) : last; };
             auto key_floor = [&](int32_t at) { return a.window ? (int32_t)max((int64_t)at - (int64_t)a.window, (int64_t)-1) : -1; };
-            const int32_t pos_first = position(tr0), pos_last = position(tr1 - 1), pos = in ? position(row) : pos_last;
+            const int32_t pos_first = position(tr0), pos_last = position(tr1 - 1), pos = tr0 + rr < tr1 ? position(tr0 + rr) : pos_last;
             const int32_t floor_last = key_floor(pos_last), floor = key_floor(pos);
-            const uint32_t tok = r.q0 + (in ? row / a.G : 0), head = seg.h * a.G + (in ? row % a.G : 0);
-            float fac;
+            // Q: a row's largest into [2^14, 2^15), 0 and non-finite rows as they are. D / 8 lanes a row.
             {
-                // Q: the row's largest into [2^14, 2^15), 0 and non-finite rows as they are
-                const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const QT *>(a.q) + (int64_t)tok * a.q_st + (int64_t)head * a.q_sh);
-                uint4 v[D / 8];
-                uint32_t top = 0;
+                constexpr uint32_t kLanes = D / 8, kRowsQ = 32 / kLanes;
+                const uint32_t c = lane % kLanes;
+                uint4 vs[16 / kRowsQ];
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    v[c] = in ? __ldg(p + c) : make_uint4(0, 0, 0, 0);
-                    const QT *e = reinterpret_cast<const QT *>(&v[c]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(fabsf(Elem<QT>::to(e[i]))));
+                for (uint32_t i = 0; i < 16 / kRowsQ; ++i) {
+                    const uint32_t row = tr0 + (warp & 7u) * 16 + i * kRowsQ + lane / kLanes;
+                    vs[i] = make_uint4(0, 0, 0, 0);
+                    if (row < tr1) {
+                        const uint32_t tk = token_of(a, row);
+                        vs[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const QT *>(a.q) + (int64_t)(seg.q0 + tk) * a.q_st +
+                                                                      (int64_t)(seg.h * a.G + (row - tk * a.G)) * a.q_sh) + c);
+                    }
                 }
-                const int32_t e2 = (int32_t)(top >> 23) - 127;
-                const int32_t shift = (top == 0 || e2 == 128) ? 0 : max(-100, min(100, 14 - e2));
-                const float m = __uint_as_float((uint32_t)(127 + shift) << 23);
-                fac = a.scale_log2 * __uint_as_float((uint32_t)(127 - shift) << 23);
-                const uint32_t dst = base + t * G::kQ + rr * 128u;
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const QT *e = reinterpret_cast<const QT *>(&v[c]);
+                for (uint32_t i = 0; i < 16 / kRowsQ; ++i) {
+                    const uint32_t r = (warp & 7u) * 16 + i * kRowsQ + lane / kLanes;
+                    const uint4 v = vs[i];
+                    const QT *e = reinterpret_cast<const QT *>(&v);
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) top = max(top, __float_as_uint(fabsf(Elem<QT>::to(e[u]))));
+#pragma unroll
+                    for (uint32_t d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+                    const int32_t e2 = (int32_t)(top >> 23) - 127;
+                    const int32_t shift = (top == 0 || e2 == 128) ? 0 : max(-100, min(100, 14 - e2));
+                    const float m = __uint_as_float((uint32_t)(127 + shift) << 23);
                     uint32_t w[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const __half2 h = __floats2half2_rn(Elem<QT>::to(e[2 * i]) * m, Elem<QT>::to(e[2 * i + 1]) * m);
-                        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+                    for (int u = 0; u < 4; ++u) {
+                        const __half2 h = __floats2half2_rn(Elem<QT>::to(e[2 * u]) * m, Elem<QT>::to(e[2 * u + 1]) * m);
+                        w[u] = *reinterpret_cast<const uint32_t *>(&h);
                     }
-                    sts128(dst + (c >> 3) * (kTile * 128u) + (((c & 7) ^ (rr & 7)) << 4), w[0], w[1], w[2], w[3]);
+                    sts128(qt + (c >> 3) * (kTile * 128u) + r * 128u + (((c & 7u) ^ (r & 7u)) << 4), w[0], w[1], w[2], w[3]);
+                    if (c == 0) tops[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - shift) << 23);
                 }
                 pipe::async_proxy_fence();
                 pipe::mbar_arrive(&bars->q_full[t]);
-                ++n_q;
             }
+            named_sync(whole_tile, 2 * kTile);
+            const float fac = tops[rr];
+            named_sync(whole_tile, 2 * kTile);
             float M = -INFINITY, l = 0.0f;
-            for (uint32_t j = 0; j < seg.take; ++j) {
-                const uint32_t key0 = (seg.first + seg.rem + j) * kKeys;
+            for (uint32_t j = 0; j < take; ++j) {
+                const uint32_t key0 = key_first + j * kKeys + hf * 64u;
                 ok = __all_sync(~0u, wait(&bars->s_full[t], n_s & 1u));
                 if (!ok) break;
                 fence_after();
-                const float4 *sc = scales + ((step0 + j) & (kScaleSlots - 1)) * 8;
-                const bool all = (int32_t)(key0 + kKeys - 1) <= pos_first && (int32_t)key0 > floor_last;
-                uint32_t p[kKeys / 2];
-                float add = 0.0f, top = -INFINITY;
-                const bool begin = __any_sync(~0u, M == -INFINITY);
-                // weights against the maximum so far; only the largest score
-                // while some row has none yet
-                auto pass = [&](bool only_top) {
-                    const float ms = M == -INFINITY ? 0.0f : M;
-                    add = 0.0f;
-                    top = -INFINITY;
+                const float4 *sc = scales + ((step0 + j) & (kScaleSlots - 1)) * 8 + hf * 4;
+                const bool all = (int32_t)(key0 + 63) <= pos_first && (int32_t)key0 > floor_last;
+                uint32_t s[64];
+                tm_ld32(tS, s);
+                tm_ld32(tS + 32, s + 32);
+                wait_ld();
+                float top = -INFINITY;
+                // scales are not negative; NaN is passed over here
+                if (all) {
 #pragma unroll
-                    for (int c = 0; c < kKeys / 32; ++c) {
-                        uint32_t s[32];
-                        tm_ld32(tS + c * 32, s);
-                        wait_ld();
+                    for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaf(largest16(s + g * 16), fac * sc[g].x, sc[g].y));
+                } else {
 #pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const float4 b = sc[c * 2 + g];
-                            const float f = fac * b.x, off = b.y - ms;
-                            float sum = 0.0f;
+                    for (int g = 0; g < 4; ++g) {
+                        float m = -INFINITY;
 #pragma unroll
-                            for (int i = 0; i < 16; i += 2) {
-                                float t0 = fmaf(__uint_as_float(s[g * 16 + i]), f, off);
-                                float t1 = fmaf(__uint_as_float(s[g * 16 + i + 1]), f, off);
-                                if (!all) {
-                                    const int32_t k = (int32_t)(key0 + c * 32 + g * 16 + i);
-                                    if (k > pos || k <= floor) t0 = -INFINITY;
-                                    if (k + 1 > pos || k + 1 <= floor) t1 = -INFINITY;
-                                }
-                                top = fmaxf(top, fmaxf(t0, t1));
-                                if (!only_top) {
-                                    const float w0 = ex2(t0), w1 = ex2(t1);
-                                    sum += w0 + w1;
-                                    const __half2 h = __floats2half2_rn(w0, w1);
-                                    p[(c * 32 + g * 16 + i) / 2] = *reinterpret_cast<const uint32_t *>(&h);
-                                }
-                            }
-                            // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
-                            add += sum == 0.0f ? 0.0f : sum * b.z;
+                        for (int i = 0; i < 16; ++i) {
+                            const int32_t key = (int32_t)key0 + g * 16 + i;
+                            if (key <= pos && key > floor) m = fmaxf(m, __uint_as_float(s[g * 16 + i]));
                         }
+                        top = fmaxf(top, fmaf(m, fac * sc[g].x, sc[g].y));
                     }
-                };
-                // raise the maximum to the largest score seen
-                auto raise = [&]() {
-                    const float to = fmaxf(M, top == -INFINITY ? M : top + (M == -INFINITY ? 0.0f : M));
-                    const float al = to == -INFINITY ? 1.0f : ex2(M - to);
+                }
+                // and of the other half's
+                tops[hf * kTile + rr] = top;
+                named_sync(pair, 64);
+                top = fmaxf(top, tops[(hf ^ 1u) * kTile + rr]);
+                if (__any_sync(~0u, top > M + kRaise)) {
+                    // raise the maximum (all rows of the warp; the other half's warp does the same), O and l with it
+                    const float to = fmaxf(M, top), al = to == -INFINITY ? 1.0f : ex2(M - to);
                     M = to;
                     l *= al;
                     if (j > 0) {
                         ok = __all_sync(~0u, wait(&bars->o_done[t], (n_s - 1) & 1u));
-                        if (!ok) return;
+                        if (!ok) break;
                         fence_after();
+#pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
-                            uint32_t o[32];
-                            tm_ld32(tO + c * 32, o);
+                            uint32_t o[16];
+                            tm_ld16(tO + c * 16, o);
                             wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                            tm_st32(tO + c * 32, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
+                            tm_st8(tO + c * 16, o);
+                            tm_st8(tO + c * 16 + 8, o + 8);
                         }
                         wait_st();
                     }
-                };
-                if (begin) {
-                    pass(true);
-                    raise();
-                    if (!ok) break;
                 }
-                pass(false);
-                if (__any_sync(~0u, top > kRaise)) {
-                    raise();
-                    if (!ok) break;
-                    pass(false);
+                const float ms = M == -INFINITY ? 0.0f : M;
+                // weights as f16 over the scores' first columns (both halves have read theirs)
+                uint32_t p[32];
+                if (all) {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) l += weigh16<false>(s + g * 16, fac * sc[g].x, sc[g].y - ms, p + g * 8, 0, 0, 0) * sc[g].z;
+                } else {
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const float sum = weigh16<true>(s + g * 16, fac * sc[g].x, sc[g].y - ms, p + g * 8, (int32_t)key0 + g * 16, pos, floor);
+                        // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
+                        l += sum == 0.0f ? 0.0f : sum * sc[g].z;
+                    }
                 }
-                l += add;
-                tm_st32(tS, p);
-                tm_st32(tS + 32, p + 32);
+                tm_st32(tP, p);
                 wait_st();
                 fence_before();
                 pipe::mbar_arrive(&bars->p_full[t]);
@@ -343,204 +411,297 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             ok = __all_sync(~0u, wait(&bars->o_done[t], (n_s - 1) & 1u));
             if (!ok) break;
             fence_after();
-            const bool whole = seg.rem == 0 && seg.take == seg.n;
+            // the products are done: Q's place takes the halves' sums, then the rows on their way out
+            float *sums = reinterpret_cast<float *>(smem + t * G::kQ);
+            sums[hf * kTile + rr] = l;
+            named_sync(whole_tile, 2 * kTile);
+            l = sums[rr] + sums[kTile + rr];
+            named_sync(whole_tile, 2 * kTile);
+            const uint32_t whole = seg.whole, q0 = seg.q0, head0 = seg.h * a.G;
+            // rows of this warp, 16-byte columns: [half of a row's 16][row][8, swizzled] for heads of 128, [row][8] for 64
+            auto place = [&](uint32_t r, uint32_t c) {   // c: column within this half's
+                return D == 128 ? qt + hf * (kTile * 128u) + r * 128u + ((c ^ (r & 7u)) << 4)
+                                : qt + r * 128u + (((hf * 4 + c) ^ (r & 7u)) << 4);
+            };
+            constexpr uint32_t kCols = D / 16, kRowsO = 32 / kCols;    // 16-byte columns of a half row; rows a warp moves at a time
+            const uint32_t rw = (warp & 3u) * 32, lr = lane / kCols, lc = lane % kCols;
             if (whole) {
                 const float f = l == 0.0f ? 0.0f : 1.0f / l;
-                QT *dst = static_cast<QT *>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
-                const bool wide = (((uintptr_t)dst) & 15u) == 0;
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tm_ld32(tO + c * 32, o);
+#pragma unroll 1
+                for (uint32_t c = 0; c < D / 32; ++c) {
+                    uint32_t o[16], w[8];
+                    tm_ld16(tO + c * 16, o);
                     wait_ld();
-                    if (in) {
-                        QT e[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) e[i] = Elem<QT>::from(__uint_as_float(o[i]) * f);
-                        if (wide) {
+                    for (int i = 0; i < 8; ++i) {
+                        QT e[2] = {Elem<QT>::from(__uint_as_float(o[2 * i]) * f), Elem<QT>::from(__uint_as_float(o[2 * i + 1]) * f)};
+                        w[i] = *reinterpret_cast<const uint32_t *>(e);
+                    }
+                    sts128(place(rr, 2 * c), w[0], w[1], w[2], w[3]);
+                    sts128(place(rr, 2 * c + 1), w[4], w[5], w[6], w[7]);
+                }
+                __syncwarp();
+#pragma unroll 1
+                for (uint32_t i = 0; i < 32; i += kRowsO) {
+                    const uint32_t r = rw + i + lr, row = tr0 + r;
+                    if (row < tr1) {
+                        const uint32_t tk = token_of(a, row);
+                        const uint4 v = pipe::lds128(place(r, lc));
+                        QT *dst = static_cast<QT *>(a.out) + (int64_t)(q0 + tk) * a.o_st + (int64_t)(head0 + row - tk * a.G) * a.o_sh +
+                                  hf * (D / 2) + lc * 8;
+                        if ((((uintptr_t)dst) & 15u) == 0) *reinterpret_cast<uint4 *>(dst) = v;
+                        else {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(dst + c * 32)[i] = reinterpret_cast<const uint4 *>(e)[i];
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) dst[c * 32 + i] = e[i];
+                            for (int u = 0; u < 8; ++u) dst[u] = reinterpret_cast<const QT *>(&v)[u];
                         }
                     }
                 }
-                if (in && a.lse)
-                    a.lse[(size_t)tok * a.Hq + head] = l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.69314718055994531f;
+                if (hf == 0 && a.lse && tr0 + rr < tr1) {
+                    const uint32_t tk = token_of(a, tr0 + rr);
+                    a.lse[(size_t)(q0 + tk) * a.Hq + head0 + (tr0 + rr - tk * a.G)] =
+                        l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.69314718055994531f;
+                }
             } else {
-                float *part = a.part + (size_t)(2 * blockIdx.x + (seg.rem == 0 ? 1 : 0)) * part_floats<kTcRows, D>();
-                const uint32_t pr = t * kTile + rr;
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tm_ld32(tO + c * 32, o);
-                    wait_ld();
-                    if (in) {
+                float *part = a.part + (size_t)(2 * blockIdx.x + (seg.cut.x ? 1 : 0)) * part_floats<kTcRows, D>();
+#pragma unroll 1
+                for (uint32_t k = 0; k < 2; ++k) {   // a quarter of the row's columns at a time
+#pragma unroll 1
+                    for (uint32_t c = 0; c < D / 64; ++c) {
+                        uint32_t o[16];
+                        tm_ld16(tO + k * (D / 4) + c * 16, o);
+                        wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            reinterpret_cast<uint4 *>(part + (size_t)pr * D + c * 32)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (uint32_t i = 0; i < 4; ++i) sts128(place(rr, 4 * c + i), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
+                    __syncwarp();
+#pragma unroll 1
+                    for (uint32_t i = 0; i < 32; i += kRowsO) {
+                        const uint32_t r = rw + i + lr;
+                        if (tr0 + r < tr1)
+                            *reinterpret_cast<uint4 *>(part + (size_t)(t * kTile + r) * D + hf * (D / 2) + k * (D / 4) + lc * 4) =
+                                pipe::lds128(place(r, lc));
+                    }
+                    __syncwarp();
                 }
-                if (in) {
-                    part[kTcRows * D + pr] = M;
-                    part[kTcRows * D + kTcRows + pr] = l;
+                if (hf == 0 && tr0 + rr < tr1) {
+                    part[kTcRows * D + t * kTile + rr] = M;
+                    part[kTcRows * D + kTcRows + t * kTile + rr] = l;
                 }
-                if (seg.rem == 0 && tid == 0) a.desc[blockIdx.x] = cut_unit(range, seg);
+                if (seg.cut.x && tid == 0) a.desc[blockIdx.x] = seg.cut;
             }
+            __syncwarp();
+            if (lane == 0) pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
             fence_before();   // O is read before the next segment's products, which wait for its weights
+            named_sync(whole_tile, 2 * kTile);   // every row is on its way out: Q's place is free
         }
     } else if (warp < kSoftWarps + kConvWarps) {
         // ------------------------------------------------------- codes
-        const uint32_t ct = tid - kSoftWarps * 32, cw = ct >> 5;
-        constexpr int kLanesK = D / 16;                       // lanes of a key row (16 codes each)
-        constexpr int kNK = kKeys * kLanesK / 128;            // key loads of a thread: 8 or 4
-        constexpr int kLanesV = D / 4;                        // lanes of a value row (4 codes each)
-        constexpr int kNV = 16 * kLanesV / 128;               // groups of 8 value rows of a thread: 4 or 2
-        const uint32_t kc = lane % kLanesK, kr = cw * (32 / kLanesK) + lane / kLanesK;   // K: piece, row of every load
-        const uint32_t vd = (lane % kLanesV) * 4, vg = cw * (32 / kLanesV) + lane / kLanesV;   // V: first dim, group of every load
-        // values: position i of a word holds dim vd + (i + turn) % 4, so that the
-        // 8 lanes of a store phase write 8 different 16-byte columns
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConv));
+        const uint32_t cw = warp - kSoftWarps;
+        // Keys: a lane takes 8 codes, one 16-byte column; the lanes of a row
+        // side by side, 1024 / D rows at a time, so row & 7 stays
+        constexpr uint32_t kLanesK = D / 8, kRowsK = 32 / kLanesK;
+        const uint32_t kc = lane % kLanesK, kr = cw * kRowsK + lane / kLanesK;
+        const uint32_t k_src = base + G::kOffRaw + kr * D + kc * 8;
+        const uint32_t k_dst = (kc >> 3) * (kKeys * 128u) + kr * 128u + (((kc & 7u) ^ (kr & 7u)) << 4);
+        constexpr int kNK = kKeys / (4 * kRowsK);              // 16 or 8 loads a step
+        // Values: a lane takes 4 dims of 8 keys. Position i of a word holds dim
+        // vd + (i + turn) % 4, so that the 8 lanes of a store phase write 8
+        // different 16-byte columns; in heads of 64 the upper lanes take
+        // their keys in the order 1, 0, 3, 2, .. to read the other banks
+        constexpr uint32_t kLanesV = D / 4;
+        constexpr int kNV = 16 * kLanesV / 128;                // 4 or 2 groups of 8 keys a step
+        const uint32_t vd = (lane % kLanesV) * 4, vg = cw * (32 / kLanesV) + lane / kLanesV, swap = lane / kLanesV;
         const uint32_t turn = (lane >> 1) & 3u;
-        const uint32_t k0 = turn, k1 = (turn + 1) & 3u, k2 = (turn + 2) & 3u, k3 = (turn + 3) & 3u;
-        const uint32_t selA = k0 | (k0 + 4) << 4 | k1 << 8 | (k1 + 4) << 12, selB = k2 | (k2 + 4) << 4 | k3 << 8 | (k3 + 4) << 12;
-        const uint32_t vdim[4] = {vd + k0, vd + k1, vd + k2, vd + k3};
-        constexpr uint32_t kStepK = kKeys / kNK, kStepV = 16 / kNV;   // rows, groups between a thread's loads
-
-        Cursor cur{range, {}, 0, true};
-        cur.ok = next_segment<kTcRows, kKeys>(a, cur.range, cur.seg);
-        Cursor nxt = cur;
-        int32_t ek[kNK], ev[kNV], es = -1;
-        uint4 kw[kNK];
-        uint32_t vw[kNV][8];
-        float vs_of[kNV], s_k = 0.0f, s_v = 0.0f;
-        bool s_ok = false;
-        // table entries of a step's rows
-        auto entries = [&](const Cursor &c) {
-            if (!c.ok) return;
-            const uint32_t key0 = (c.seg.first + c.seg.rem + c.j) * kKeys;
-            const int32_t *row = a.table + (size_t)c.seg.b * a.width;
-            auto entry = [&](uint32_t key) -> int32_t { return key < c.seg.hi ? __ldg(row + key / a.P) : -1; };
+        uint32_t sel[2], v_dst[4];
 #pragma unroll
-            for (int i = 0; i < kNK; ++i) ek[i] = entry(key0 + i * kStepK + (kr & ~15u));
-#pragma unroll
-            for (int i = 0; i < kNV; ++i) ev[i] = entry(key0 + (i * kStepV + vg) * 8);
-            if (ct < 8) {
-                es = entry(key0 + ct * 16);
-                if (key0 + ct * 16 < c.seg.hi && (uint32_t)es >= a.n_blocks) flag(a.status, HXQ_SERVING_BAD_BLOCK);
-            }
-        };
-        auto load_k = [&](const Cursor &c) {
-            if (!c.ok) return;
-            const uint32_t key0 = (c.seg.first + c.seg.rem + c.j) * kKeys;
-#pragma unroll
-            for (int i = 0; i < kNK; ++i) {
-                const uint32_t key = key0 + i * kStepK + kr;
-                kw[i] = make_uint4(0, 0, 0, 0);
-                if ((uint32_t)ek[i] < a.n_blocks)
-                    kw[i] = __ldg(reinterpret_cast<const uint4 *>(a.k + (((size_t)(uint32_t)ek[i] * a.H + c.seg.h) * a.P + key % a.P) * D + kc * 16));
-            }
-            s_ok = (uint32_t)es < a.n_blocks;
-            if (ct < 8 && s_ok) {
-                s_k = __ldg(a.ks + (size_t)(uint32_t)es * a.H + c.seg.h);
-                s_v = __ldg(a.vs + (size_t)(uint32_t)es * a.H + c.seg.h);
-            }
-        };
-        auto load_v = [&](const Cursor &c) {
-            if (!c.ok) return;
-            const uint32_t key0 = (c.seg.first + c.seg.rem + c.j) * kKeys;
-#pragma unroll
-            for (int i = 0; i < kNV; ++i) {
-                const uint32_t key = key0 + (i * kStepV + vg) * 8;
-                const bool in = (uint32_t)ev[i] < a.n_blocks;
-                const size_t bh = (size_t)(in ? (uint32_t)ev[i] : 0u) * a.H + c.seg.h;
-                vs_of[i] = in ? __ldg(a.vs + bh) : 0.0f;
-#pragma unroll
-                for (int u = 0; u < 8; ++u)
-                    vw[i][u] = in ? __ldg(reinterpret_cast<const uint32_t *>(a.v + (bh * a.P + key % a.P + u) * D + vd)) : 0u;
-            }
-        };
-        entries(cur);
-        load_k(cur);
-        load_v(cur);
-        nxt.next(a);
-        entries(nxt);
-        bool ok = true;
-        for (uint32_t it = 0; cur.ok; ++it) {
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t k = (turn + i) & 3u, dim = vd + k;
+            const uint32_t pair = swap ? (k + 4) | k << 4 : k | (k + 4) << 4;   // bytes k of the two keys
+            sel[i >> 1] = (i & 1) ? sel[i >> 1] | pair << 8 : pair;
+            v_dst[i] = dim * 128u + ((vg & 7u) ^ (dim & 7u)) * 16u;
+        }
+        constexpr uint32_t kStepV = 16 / kNV;                  // groups between a lane's
+        const uint32_t v_src = base + G::kOffRaw + G::kRaw + vg * 8 * D + vd;
+        for (uint32_t it = 0;; ++it) {
             const uint32_t st = it & 1u, par = (it >> 1) & 1u;
-            const uint32_t key0 = (cur.seg.first + cur.seg.rem + cur.j) * kKeys, hi = cur.seg.hi;
+            ok = __all_sync(~0u, wait(&bars->rawk_full, it & 1u));
+            if (!ok) break;
+            const uint32_t live = bars->live[st];
+            if (live == 0) break;
             if (it >= 2) ok = __all_sync(~0u, wait(&bars->k_empty[st], par ^ 1u));
             if (!ok) break;
-            const uint32_t kb = base + G::kOffK + st * G::kK;
+            const uint32_t kb = base + G::kOffK + st * G::kK + k_dst;
 #pragma unroll
             for (int i = 0; i < kNK; ++i) {
-                const uint32_t row = i * kStepK + kr, w[4] = {kw[i].x, kw[i].y, kw[i].z, kw[i].w};
-                uint32_t h[8];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) codes_to_f16<FMT>(w[u], h[2 * u], h[2 * u + 1]);
-                // 16 codes: two 16-byte columns; odd column first in the second half of a row of 128, away from the
-                // first half's even ones
-                const uint32_t half = kc >> 2, c0 = (kc & 3u) * 2, odd = half;
-                const uint32_t dst = kb + half * (kKeys * 128u) + row * 128u;
-                const uint32_t a0 = dst + (((c0 + odd) ^ (row & 7u)) << 4), a1 = dst + (((c0 + (odd ^ 1u)) ^ (row & 7u)) << 4);
-                sts128(a0, odd ? h[4] : h[0], odd ? h[5] : h[1], odd ? h[6] : h[2], odd ? h[7] : h[3]);
-                sts128(a1, odd ? h[0] : h[4], odd ? h[1] : h[5], odd ? h[2] : h[6], odd ? h[3] : h[7]);
-            }
-            if (ct < 8) {
-                float4 b = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);   // keys outside: no weight
-                if (s_ok) {
-                    bool zero;
-                    b.x = s_k;
-                    value_scale(s_v, b.y, b.z, zero);
-                }
-                scales[(it & (kScaleSlots - 1)) * 8 + ct] = b;
+                uint2 w = pipe::lds64(k_src + i * (4 * kRowsK * D));
+                if (live < kKeys && ((kr + i * 4 * kRowsK) & ~15u) >= live) w = make_uint2(0, 0);   // not copied
+                uint32_t h[4];
+                codes_to_f16<FMT>(w.x, h[0], h[1]);
+                codes_to_f16<FMT>(w.y, h[2], h[3]);
+                sts128(kb + i * (4 * kRowsK * 128u), h[0], h[1], h[2], h[3]);
             }
             pipe::async_proxy_fence();
             pipe::mbar_arrive(&bars->k_full[st]);
-            load_k(nxt);
+            __syncwarp();
+            if (lane == 0) pipe::mbar_arrive(&bars->rawk_empty);
+            ok = __all_sync(~0u, wait(&bars->rawv_full, it & 1u));
+            if (!ok) break;
             if (it >= 2) ok = __all_sync(~0u, wait(&bars->v_empty[st], par ^ 1u));
             if (!ok) break;
             const uint32_t vb = base + G::kOffV + st * G::kK;
 #pragma unroll
             for (int i = 0; i < kNV; ++i) {
-                const uint32_t grp = i * kStepV + vg, key = key0 + grp * 8;
-                const bool drop = vs_of[i] < 7.8886090522101181e-31f;   // blocks below 2^-100 count as 0
-                if (drop || key + 8 > hi) {
+                const uint32_t grp = i * kStepV + vg;
+                uint32_t w[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) w[u] = pipe::lds32(v_src + i * (kStepV * 8 * D) + (D == 64 ? u ^ swap : u) * D);
+                const bool drop = bars->zero[st][grp >> 1] != 0;
+                if (drop || grp * 8 + 8 > live) {
+                    // blocks that count as 0, and slots behind the last key, which may hold anything
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
-                        if (drop || key + u >= hi) vw[i][u] = 0;   // slots behind the last key may hold anything
+                        if (drop || grp * 8 + (D == 64 ? u ^ swap : u) >= live) w[u] = 0;
                 }
                 uint32_t o[4][4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    codes_to_f16<FMT>(__byte_perm(vw[i][2 * u], vw[i][2 * u + 1], selA), o[0][u], o[1][u]);
-                    codes_to_f16<FMT>(__byte_perm(vw[i][2 * u], vw[i][2 * u + 1], selB), o[2][u], o[3][u]);
+                    codes_to_f16<FMT>(__byte_perm(w[2 * u], w[2 * u + 1], sel[0]), o[0][u], o[1][u]);
+                    codes_to_f16<FMT>(__byte_perm(w[2 * u], w[2 * u + 1], sel[1]), o[2][u], o[3][u]);
                 }
-                const uint32_t dst = vb + (grp >> 3) * (D * 128u);
+                // groups i * kStepV + vg: the next half of the keys, and the other four columns of a half
+                const uint32_t dst = vb + ((i * kStepV) >> 3) * (D * 128u), flip = ((i * kStepV) & 7u) << 4;
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    sts128(dst + vdim[u] * 128u + (((grp & 7u) ^ (vdim[u] & 7u)) << 4), o[u][0], o[u][1], o[u][2], o[u][3]);
+                for (int u = 0; u < 4; ++u) sts128(dst + (v_dst[u] ^ flip), o[u][0], o[u][1], o[u][2], o[u][3]);
             }
             pipe::async_proxy_fence();
             pipe::mbar_arrive(&bars->v_full[st]);
-            load_v(nxt);
-            cur = nxt;
-            nxt.next(a);
-            entries(nxt);
+            __syncwarp();
+            if (lane == 0) pipe::mbar_arrive(&bars->rawv_empty);
         }
-    } else if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+        if (warp == kLoadWarp && lane < 8) {
+            // --------------------------------------------------- loads
+            uint32_t it = 0;
+            for (uint32_t si = 0; ok; ++si) {
+                ok = wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u);
+                if (!ok) break;
+                const SegInfo seg = segs[si % kSegSlots];
+                __syncwarp(0xffu);
+                if (lane == 0) pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
+                if (seg.take == 0) break;
+                const int32_t *row = a.table + (size_t)seg.b * a.width;
+                uint32_t slot;
+                // the block of the next step is looked up while this one's copies are under way
+                auto entry = [&](uint32_t j) -> int32_t {
+                    const uint32_t key = seg.key0 + j * kKeys + lane * 16;
+                    return j < seg.take && key < seg.hi ? __ldg(row + block_of(a, key, slot)) : -1;
+                };
+                auto zeros = [&](uint8_t *dst) {   // in place of a block outside the cache
+                    for (int i = 0; i < D; ++i) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0, 0, 0, 0);
+                    pipe::async_proxy_fence();
+                };
+                int32_t next = entry(0);
+                for (uint32_t j = 0; j < seg.take; ++j, ++it) {
+                    const int32_t blk = next;
+                    const uint32_t key0 = seg.key0 + j * kKeys, key = key0 + lane * 16;
+                    const bool in = key < seg.hi && (uint32_t)blk < a.n_blocks;
+                    if (key < seg.hi && !in) flag(a.status, HXQ_SERVING_BAD_BLOCK);
+                    float4 b = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);   // keys outside: no weight
+                    bool zero = true;
+                    const size_t bh = (size_t)(in ? (uint32_t)blk : 0u) * a.H + seg.h;
+                    block_of(a, key, slot);
+                    const size_t src = (bh * a.P + slot) * D;
+                    if (in) {
+                        b.x = __ldg(a.ks + bh);
+                        value_scale(__ldg(a.vs + bh), b.y, b.z, zero);
+                    }
+                    next = entry(j + 1);
+                    if (it >= 1) ok = wait(&bars->rawk_empty, (it - 1) & 1u);
+                    if (!ok) break;
+                    scales[(it & (kScaleSlots - 1)) * 8 + lane] = b;
+                    bars->zero[it & 1u][lane] = zero;
+                    if (lane == 0) bars->live[it & 1u] = min((uint32_t)kKeys, seg.hi > key0 ? seg.hi - key0 : 1u);
+                    uint8_t *dst = smem + G::kOffRaw + lane * 16 * D;
+                    if (in) {
+                        pipe::mbar_expect_tx(&bars->rawk_full, 16 * D);
+                        pipe::bulk_g2s(dst, a.k + src, 16 * D, &bars->rawk_full);
+                    } else {
+                        if (key < seg.hi) zeros(dst);
+                        pipe::mbar_arrive(&bars->rawk_full);
+                    }
+                    if (it >= 1) ok = wait(&bars->rawv_empty, (it - 1) & 1u);
+                    if (!ok) break;
+                    if (in) {
+                        pipe::mbar_expect_tx(&bars->rawv_full, 16 * D);
+                        pipe::bulk_g2s(dst + G::kRaw, a.v + src, 16 * D, &bars->rawv_full);
+                    } else {
+                        if (key < seg.hi) zeros(dst + G::kRaw);
+                        pipe::mbar_arrive(&bars->rawv_full);
+                    }
+                }
+            }
+            // the end of the work
+            if (ok && it >= 1) ok = wait(&bars->rawk_empty, (it - 1) & 1u);
+            if (ok) {
+                if (lane == 0) bars->live[it & 1u] = 0;
+                pipe::mbar_arrive(&bars->rawk_full);
+            }
+            // copies under way end before the CTA does
+            if (!ok) {
+                const uint64_t t0 = clock64();
+                while (clock64() - t0 < 20000000ull) {}
+            }
+        } else if (warp == kPlanWarp && lane == 0) {
+            // --------------------------------------------------- segments
+            Segment seg;
+            for (uint32_t si = 0; ok; ++si) {
+                const bool more = next_segment<kTcRows, kKeys, kFixedT>(a, range, seg);
+                if (si >= kSegSlots) ok = wait(&bars->seg_empty[si % kSegSlots], (si / kSegSlots & 1u) ^ 1u);
+                if (!ok) break;
+                SegInfo &d = segs[si % kSegSlots];
+                d.take = more ? seg.take : 0;
+                if (more) {
+                    uint32_t lo, hi0;
+                    key_range(a, seg.r, seg.r0, min(seg.r0 + kTile, seg.r1), lo, hi0);
+                    const uint32_t n0 = hi0 > seg.key0 ? (hi0 - seg.key0 + kKeys - 1) / kKeys : 1u;
+                    d.take0 = seg.r1 - seg.r0 > (uint32_t)kTile ? min(n0, seg.take) : seg.take;
+                    d.key0 = seg.key0;
+                    d.hi = seg.hi;
+                    d.r0 = seg.r0;
+                    d.r1 = seg.r1;
+                    d.q0 = seg.r.q0;
+                    d.h = seg.h;
+                    d.b = seg.b;
+                    d.before = (int32_t)seg.r.len - (int32_t)seg.r.n;
+                    d.len = seg.r.len;
+                    d.whole = seg.begins && seg.take == seg.n;
+                    d.cut = seg.begins && seg.take < seg.n ? cut_unit(range, seg) : make_int4(0, 0, 0, 0);
+                }
+                pipe::mbar_arrive(&bars->seg_full[si % kSegSlots]);
+                if (!more) break;
+            }
+        } else if (warp == kMmaWarp && lane == 0) {
         // ------------------------------------------------------- products
         uint32_t it = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-        Segment seg;
-        bool ok = true;
+        // descriptors address 16-byte units
+        const uint64_t q_desc = desc_sw128(base), k_desc = desc_sw128(base + G::kOffK), v_desc = desc_sw128(base + G::kOffV);
         auto qk = [&](uint32_t t, uint32_t st) {
-            const uint32_t qa = base + t * G::kQ, kb = base + G::kOffK + st * G::kK;
+            const uint64_t qa = q_desc + t * (G::kQ >> 4), kb = k_desc + st * (G::kK >> 4);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
-                tc_mma_ss(tmem + t * 128u, desc_sw128(qa + (kk >> 2) * (kTile * 128u) + (kk & 3) * 32u),
-                          desc_sw128(kb + (kk >> 2) * (kKeys * 128u) + (kk & 3) * 32u), G::kIdescQK, kk != 0);
+                tc_mma_ss(tmem + t * 128u, qa + ((kk >> 2) * (kTile * 8) + (kk & 3) * 2), kb + ((kk >> 2) * (kKeys * 8) + (kk & 3) * 2),
+                          G::kIdescQK, kk != 0);
             tc_commit(&bars->s_full[t]);
         };
-        while (ok && next_segment<kTcRows, kKeys>(a, range, seg)) {
-            const uint32_t tiles = seg.r1 - seg.r0 > (uint32_t)kTile ? 2u : 1u;
+        for (uint32_t si = 0; ok; ++si) {
+            ok = wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u);
+            if (!ok) break;
+            const uint32_t take = segs[si % kSegSlots].take, take0 = segs[si % kSegSlots].take0;
+            const uint32_t tiles = segs[si % kSegSlots].r1 - segs[si % kSegSlots].r0 > (uint32_t)kTile ? 2u : 1u;
+            pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
+            if (take == 0) break;
             ok = wait(&bars->k_full[it & 1u], (it >> 1) & 1u);
             for (uint32_t t = 0; ok && t < tiles; ++t) {
                 ok = wait(&bars->q_full[t], n_q[t]++ & 1u);
@@ -550,29 +711,23 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             }
             if (!ok) break;
             tc_commit(&bars->k_empty[it & 1u]);
-            for (uint32_t j = 0; ok && j < seg.take; ++j, ++it) {
+            for (uint32_t j = 0; ok && j < take; ++j, ++it) {
                 const uint32_t st = it & 1u, sn = (it + 1) & 1u;
-                for (uint32_t t = 0; t < tiles; ++t) {
-                    ok = wait(&bars->p_full[t], n_p[t]++ & 1u) && (t != 0 || wait(&bars->v_full[st], (it >> 1) & 1u));
+                ok = wait(&bars->v_full[st], (it >> 1) & 1u) && (j + 1 >= take || wait(&bars->k_full[sn], ((it + 1) >> 1) & 1u));
+                for (uint32_t t = j < take0 ? 0 : 1; ok && t < tiles; ++t) {
+                    ok = wait(&bars->p_full[t], n_p[t]++ & 1u);
                     if (!ok) break;
                     fence_after();
-                    const uint32_t vb = base + G::kOffV + st * G::kK;
+                    const uint64_t vb = v_desc + st * (G::kK >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        tc_mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + kk * 8u,
-                                  desc_sw128(vb + (kk >> 2) * (D * 128u) + (kk & 3) * 32u), G::kIdescPV, (j | kk) != 0);
+                        tc_mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + kk * 8u, vb + ((kk >> 2) * (D * 8) + (kk & 3) * 2),
+                                  G::kIdescPV, (j | kk) != 0);
                     tc_commit(&bars->o_done[t]);
-                    if (t == tiles - 1) tc_commit(&bars->v_empty[st]);
-                    if (j + 1 < seg.take) {
-                        if (t == 0) {
-                            ok = wait(&bars->k_full[sn], ((it + 1) >> 1) & 1u);
-                            if (!ok) break;
-                            fence_after();
-                        }
-                        qk(t, sn);
-                        if (t == tiles - 1) tc_commit(&bars->k_empty[sn]);
-                    }
+                    if (j + 1 < (t == 0 ? take0 : take)) qk(t, sn);
                 }
+                if (ok) tc_commit(&bars->v_empty[st]);
+                if (ok && j + 1 < take) tc_commit(&bars->k_empty[sn]);
             }
         }
         if (!ok) {
@@ -581,11 +736,13 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             const uint64_t t0 = clock64();
             while (!pipe::mbar_try(&bars->drained, 0) && clock64() - t0 < pipe::kWaitCycles) {}
         }
+        }
     }
+    if (!ok) flag(a.status, HXQ_SERVING_TIMEOUT);
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == kWarpsT - 1) {
+    if (warp == kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
