@@ -42,8 +42,8 @@ constexpr int kSoftWarps = 16, kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps, kLoadWarp = kMmaWarp + 1, kPlanWarp = kMmaWarp + 2;
 constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups; the last warp has nothing to do
 // Registers: launched with 80 a thread, 61,440 in all; the rows' threads hold
-// 64 scores. 512 x 96 + 128 x 56 + 128 x 40 = 61,440.
-constexpr int kRegsSoft = 96, kRegsConv = 56, kRegsRest = 40;
+// 32 scores at a time. 512 x 88 + 128 x 64 + 128 x 64 = 61,440.
+constexpr int kRegsSoft = 88, kRegsConv = 64, kRegsRest = 64;
 constexpr int kThreadsT = kWarpsT * 32;
 constexpr int kScaleSlots = 4, kSegSlots = 2;
 constexpr float kRaise = 8.0f;             // log2 of the largest weight before the maximum is raised
@@ -105,15 +105,12 @@ __device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t *v)
                  : "memory");
 }
 
-__device__ __forceinline__ void tm_st32(uint32_t taddr, const uint32_t *v)
+__device__ __forceinline__ void tm_st16(uint32_t taddr, const uint32_t *v)
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-                 "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
-                 "%32};" ::"r"(taddr),
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+                 "%13, %14, %15, %16};" ::"r"(taddr),
                  "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-                 "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
-                 "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-                 "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+                 "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                  : "memory");
 }
 
@@ -124,13 +121,6 @@ __device__ __forceinline__ void tm_ld16(uint32_t taddr, uint32_t (&v)[16])
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
                  "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                  : "r"(taddr)
-                 : "memory");
-}
-
-__device__ __forceinline__ void tm_st8(uint32_t taddr, const uint32_t *v)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
-                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 
@@ -263,7 +253,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
         const uint32_t t = warp >> 3, hf = warp >> 2 & 1u, rr = tid & (kTile - 1);   // tile, half of the keys, row of the tile
         const uint32_t lanes = (warp & 3u) << 21;                      // this warp's 32 lanes of tensor memory
-        const uint32_t tS = tmem + lanes + t * 128u + hf * 64u, tP = tmem + lanes + t * 128u + hf * 32u;
+        const uint32_t tS = tmem + lanes + t * 128u + hf * 64u;
         const uint32_t tO = tmem + lanes + 256u + t * 128u + hf * (D / 2);
         const uint32_t pair = 1 + t * 4 + (warp & 3u), whole_tile = 9 + t;           // named barriers: 64 and 256 threads
         float *tops = reinterpret_cast<float *>(smem + G::kOffTop) + t * 2 * kTile;
@@ -339,25 +329,23 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 fence_after();
                 const float4 *sc = scales + ((step0 + j) & (kScaleSlots - 1)) * 8 + hf * 4;
                 const bool all = (int32_t)(key0 + 63) <= pos_first && (int32_t)key0 > floor_last;
-                uint32_t s[64];
-                tm_ld32(tS, s);
-                tm_ld32(tS + 32, s + 32);
-                wait_ld();
                 float top = -INFINITY;
                 // scales are not negative; NaN is passed over here
-                if (all) {
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t s[32];
+                    tm_ld32(tS + c * 32, s);
+                    wait_ld();
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaf(largest16(s + g * 16), fac * sc[g].x, sc[g].y));
-                } else {
+                    for (int g = 0; g < 2; ++g) {
+                        if (!all) {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        float m = -INFINITY;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int32_t key = (int32_t)key0 + g * 16 + i;
-                            if (key <= pos && key > floor) m = fmaxf(m, __uint_as_float(s[g * 16 + i]));
+                            for (int i = 0; i < 16; ++i) {
+                                const int32_t key = (int32_t)key0 + c * 32 + g * 16 + i;
+                                if (key > pos || key <= floor) s[g * 16 + i] = 0xff800000u;   // -infinity
+                            }
                         }
-                        top = fmaxf(top, fmaf(m, fac * sc[g].x, sc[g].y));
+                        top = fmaxf(top, fmaf(largest16(s + g * 16), fac * sc[c * 2 + g].x, sc[c * 2 + g].y));
                     }
                 }
                 // and of the other half's
@@ -380,27 +368,33 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                             wait_ld();
 #pragma unroll
                             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * al);
-                            tm_st8(tO + c * 16, o);
-                            tm_st8(tO + c * 16 + 8, o + 8);
+                            tm_st16(tO + c * 16, o);
                         }
                         wait_st();
                     }
                 }
                 const float ms = M == -INFINITY ? 0.0f : M;
-                // weights as f16 over the scores' first columns (both halves have read theirs)
-                uint32_t p[32];
-                if (all) {
+                // weights as f16 over the first half of this half's columns: 32 scores are read, then 16 columns written
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t s[32], p[16];
+                    tm_ld32(tS + c * 32, s);
+                    wait_ld();
+                    if (all) {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) l += weigh16<false>(s + g * 16, fac * sc[g].x, sc[g].y - ms, p + g * 8, 0, 0, 0) * sc[g].z;
-                } else {
+                        for (int g = 0; g < 2; ++g)
+                            l += weigh16<false>(s + g * 16, fac * sc[c * 2 + g].x, sc[c * 2 + g].y - ms, p + g * 8, 0, 0, 0) * sc[c * 2 + g].z;
+                    } else {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const float sum = weigh16<true>(s + g * 16, fac * sc[g].x, sc[g].y - ms, p + g * 8, (int32_t)key0 + g * 16, pos, floor);
-                        // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
-                        l += sum == 0.0f ? 0.0f : sum * sc[g].z;
+                        for (int g = 0; g < 2; ++g) {
+                            const float sum = weigh16<true>(s + g * 16, fac * sc[c * 2 + g].x, sc[c * 2 + g].y - ms, p + g * 8,
+                                                            (int32_t)key0 + c * 32 + g * 16, pos, floor);
+                            // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
+                            l += sum == 0.0f ? 0.0f : sum * sc[c * 2 + g].z;
+                        }
                     }
+                    tm_st16(tS + c * 16, p);
                 }
-                tm_st32(tP, p);
                 wait_st();
                 fence_before();
                 pipe::mbar_arrive(&bars->p_full[t]);
@@ -721,7 +715,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     const uint64_t vb = v_desc + st * (G::kK >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        tc_mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + kk * 8u, vb + ((kk >> 2) * (D * 8) + (kk & 3) * 2),
+                        tc_mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + (kk >> 2) * 64u + (kk & 3) * 8u, vb + ((kk >> 2) * (D * 8) + (kk & 3) * 2),
                                   G::kIdescPV, (j | kk) != 0);
                     tc_commit(&bars->o_done[t]);
                     if (j + 1 < (t == 0 ? take0 : take)) qk(t, sn);
