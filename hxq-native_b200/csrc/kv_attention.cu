@@ -11,16 +11,21 @@
 // nothing.  q is scaled per row by a power of two into f16's range (bf16
 // values down to 2^-39 of the row's largest are exact).
 //
-// A CTA of four warps takes 16 rows (tokens x heads of a group) of one
-// (request, cache head) against 64 keys at a time, 16 keys a warp: m16n8k16
-// products, Q and the output accumulators in registers, every warp its own
-// running maximum and sums, joined at the end of a segment.  A lane's share
-// of a key row is 16 consecutive bytes: the order of the head's dimensions
-// inside a product is free as long as Q has the same, so codes go from a
-// lane's own 16-byte copies (cp.async into slots that no other lane reads: no
-// barrier in the loop) through a byte permute into the fragments.
+// A CTA of four warps takes 8 or 16 rows (tokens x heads of a group) of one
+// (request, cache head) against 64 keys at a time, 16 keys a warp, every warp
+// with its own running maximum and sums, joined at the end of a segment.  The
+// products are m16n8k16 with keys, then dimensions, on the side of 16 and rows
+// on that of 8 (S^T = K Q^T, O^T = V^T P^T): one request's group of heads
+// fills the small side, so a decode step of up to 8 heads a group wastes
+// nothing of it.  A lane's share of a key row is 16 consecutive bytes: the
+// order of the head's dimensions inside a product is free as long as Q has
+// the same, so codes go from a lane's own 16-byte copies (cp.async into slots
+// that no other lane reads: no barrier in the loop) through a byte permute
+// into the fragments; the weights turn round with movmatrix.  The maximum is
+// raised only where a weight would pass 2^8 (f16 holds 2^16): a vote a step
+// instead of a reduction.
 //
-// The keys of all (request, head, 16 rows) are laid end to end in granules of
+// The keys of all (request, head, tile of rows) are laid end to end in granules of
 // 64 and cut into equal ranges, one per CTA; a range that ends inside a unit
 // leaves a partial result (16 rows) in the workspace, and a second kernel
 // joins the parts of each cut unit in order.  Every CTA derives the cut from
@@ -32,26 +37,24 @@
 namespace hxq {
 namespace serving {
 
-constexpr int kRows = 16;        // rows of a tile
+constexpr int kMostRows = 16;    // rows of a partial result's slot; a tile has 8 NT of them
 constexpr int kGran = 64;        // keys of a granule
 constexpr int kFixed = 2;        // granules that a unit costs by itself
 constexpr int kWarpsA = 4;
 constexpr int kThreadsA = kWarpsA * 32;
+constexpr float kRaiseA = 8.0f;  // log2 of the largest weight before the maximum is raised
 
 template <int D> struct Geo {
     static constexpr int kVB = D >= 128 ? 16 : 8;      // bytes of a lane's copy of a value row
     static constexpr int kVC = D / (8 * kVB);          // copies of a value row per lane
     static constexpr int kKC = D / 64;                 // copies of a key row per lane
-    static constexpr int kStepBytes = 32 * D;          // K and V of 16 keys
-    static constexpr int kSlot = kStepBytes + 32 * 8;  // plus the two scales per lane
-    static constexpr int kStages = D == 64 ? 6 : D == 128 ? 4 : 3;
-    static constexpr int kQSmem = D == 256 ? 32 * D : 0;   // Q fragments in shared memory
+    static constexpr int kSlot = 32 * D + 32 * 8;      // K and V of 16 keys, and the two scales per lane
+    static constexpr int kStages = D == 64 ? 4 : 3;
     static constexpr int kRing = kWarpsA * kStages * kSlot;
     static constexpr int kPad = 4;
-    static constexpr int kMerge = kWarpsA * kRows * (D + kPad) * 4;
-    static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kQSmem;   // at least the scan's 4 (B + 1) bytes
+    static constexpr int kMerge = kWarpsA * kMostRows * (D + kPad) * 4;
+    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
     static_assert(kSmem >= 4 * (HXQ_ATTENTION_MAX_REQUESTS + 1), "room for the scan");
-    static constexpr int kCtas = D == 256 ? 2 : 3;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src)
@@ -76,132 +79,74 @@ template <typename QT> __device__ __forceinline__ uint32_t to_f16x2(uint32_t w, 
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-template <int D, int FMT, typename QT>
-__global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(const __grid_constant__ AttnArgs a)
+__device__ __forceinline__ uint32_t turn8x8(uint32_t v)
+{
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+
+// CTAs an SM: as many as the accumulators' registers allow.
+__host__ __device__ constexpr uint32_t ctas_per_sm(uint32_t D, bool few) { return D == 256 ? 2u : D == 128 && !few ? 3u : 4u; }
+
+template <int D, int FMT, typename QT, int NT>
+__global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_kernel(const __grid_constant__ AttnArgs a)
 {
     using G = Geo<D>;
+    constexpr int kRows = 8 * NT;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RangeShared<kWarpsA> sh;
     __shared__ float sh_m[kWarpsA][kRows], sh_l[kWarpsA][kRows];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
     let_next_start();
-
     if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     Range range;
     if (!find_range<kWarpsA, kRows, kGran, kFixed>(a, sh, reinterpret_cast<uint32_t *>(smem), true, range)) return;
     __syncthreads();   // the sums in front of the requests are read: the ring may be filled
+
     const uint32_t ring = pipe::smem_u32(smem) + warp * (G::kStages * G::kSlot);
-    uint4 *qs = reinterpret_cast<uint4 *>(smem + (G::kSmem - G::kQSmem));
     float *merge = reinterpret_cast<float *>(smem);
-    const uint32_t bh_bytes = a.P * D;
+    const uint32_t k_lane = g * D + q * 16, v_lane = 2 * q * D + g * G::kVB;   // of a 16-key piece
 
     Segment seg;
     while (next_segment<kRows, kGran, kFixed>(a, range, seg)) {
         const Req &r = seg.r;
         const uint32_t h = seg.h, take = seg.take, hi = seg.hi, r0 = seg.r0, r1 = seg.r1;
         const uint32_t key0 = seg.key0 + warp * 16;   // this warp's first 16 keys
-
-        // ---- Q: rows g and g + 8, in the order in which codes arrive
-        uint32_t qf[G::kQSmem ? 1 : D / 16][4];
-        float fac[2];
-        int32_t pos[2];
-        {
-            uint32_t raw[2][D / 16][2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t row = r0 + g + 8 * i;
-                const bool in = row < r1;
-                const uint32_t tok = in ? token_of(a, row) : 0, head = h * a.G + (in ? row - tok * a.G : 0);
-                pos[i] = in ? (a.causal ? (int32_t)((int64_t)r.len - r.n + tok) : (int32_t)r.len - 1) : -1;
-                const QT *p = static_cast<const QT *>(a.q) + (int64_t)(r.q0 + tok) * a.q_st + (int64_t)head * a.q_sh;
-                uint32_t top = 0;
-#pragma unroll
-                for (int c = 0; c < G::kKC; ++c)
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const uint4 v = in ? __ldg(reinterpret_cast<const uint4 *>(p + c * 64 + q * 16) + w)
-                                           : make_uint4(0, 0, 0, 0);
-                        raw[i][c * 4 + w * 2][0] = v.x;
-                        raw[i][c * 4 + w * 2][1] = v.y;
-                        raw[i][c * 4 + w * 2 + 1][0] = v.z;
-                        raw[i][c * 4 + w * 2 + 1][1] = v.w;
-                    }
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const QT *e = reinterpret_cast<const QT *>(&raw[i][s][w]);
-                        top = max(top, __float_as_uint(fabsf(Elem<QT>::to(e[0]))));
-                        top = max(top, __float_as_uint(fabsf(Elem<QT>::to(e[1]))));
-                    }
-                top = max(top, __shfl_xor_sync(~0u, top, 1));
-                top = max(top, __shfl_xor_sync(~0u, top, 2));
-                // 2^(14 - exponent of the largest): into [2^14, 2^15); 0 and non-finite rows as they are
-                const int32_t e = (int32_t)(top >> 23) - 127;
-                const int32_t sh = (top == 0 || e == 128) ? 0 : max(-100, min(100, 14 - e));
-                const float m = __uint_as_float((uint32_t)(127 + sh) << 23);
-                fac[i] = a.scale_log2 * __uint_as_float((uint32_t)(127 - sh) << 23);
-#pragma unroll
-                for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) raw[i][s][w] = to_f16x2<QT>(raw[i][s][w], m);
-            }
-#pragma unroll
-            for (int s = 0; s < D / 16; ++s) {
-                if (G::kQSmem) {
-                    if (warp == 0) qs[s * 32 + lane] = make_uint4(raw[0][s][0], raw[1][s][0], raw[0][s][1], raw[1][s][1]);
-                } else {
-                    qf[s % (G::kQSmem ? 1 : D / 16)][0] = raw[0][s][0];
-                    qf[s % (G::kQSmem ? 1 : D / 16)][1] = raw[1][s][0];
-                    qf[s % (G::kQSmem ? 1 : D / 16)][2] = raw[0][s][1];
-                    qf[s % (G::kQSmem ? 1 : D / 16)][3] = raw[1][s][1];
-                }
-            }
-            if (G::kQSmem) __syncthreads();
-        }
-        const int32_t pos_first = a.causal ? (int32_t)((int64_t)r.len - r.n + token_of(a, r0)) : (int32_t)r.len - 1;
-        const int32_t pos_last = a.causal ? (int32_t)((int64_t)r.len - r.n + token_of(a, r1 - 1)) : (int32_t)r.len - 1;
+        const int32_t before = (int32_t)r.len - (int32_t)r.n;
+        auto position = [&](uint32_t row) { return a.causal ? before + (int32_t)token_of(a, row) : (int32_t)r.len - 1; };
         // a row sees keys above its floor: its position less the window, -1 without one
         auto key_floor = [&](int32_t at) { return a.window ? (int32_t)max((int64_t)at - (int64_t)a.window, (int64_t)-1) : -1; };
-        const int32_t floor_last = key_floor(pos_last), floors[2] = {key_floor(pos[0]), key_floor(pos[1])};
 
-        // ---- key loop
-        float o[D / 8][4];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        // ---- the first copies: K and V of the first steps
         uint32_t valid = 0;   // bit s: the step in stage s has a block inside the cache
-        const int32_t *row = a.table + (size_t)seg.b * a.width;
+        const int32_t *table = a.table + (size_t)seg.b * a.width;
         auto entry = [&](uint32_t j) -> int32_t {
             const uint32_t key = key0 + j * kGran;
             uint32_t slot;
-            return j < take && key < hi ? __ldg(row + block_of(a, key, slot)) : -1;
+            return j < take && key < hi ? __ldg(table + block_of(a, key, slot)) : -1;
         };
         auto issue = [&](uint32_t j, uint32_t stage, int32_t blk) {
             const uint32_t key = key0 + j * kGran;
-            const bool wanted = j < take && key < hi;
-            const bool ok = wanted && (uint32_t)blk < a.n_blocks;
+            const bool wanted = j < take && key < hi, ok = wanted && (uint32_t)blk < a.n_blocks;
             if (wanted && !ok && lane == 0) flag(a.status, HXQ_SERVING_BAD_BLOCK);
             valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
             if (ok) {
-                const size_t bh = (size_t)(uint32_t)blk * a.H + h;
                 uint32_t slot;
                 block_of(a, key, slot);
-                const size_t base = bh * bh_bytes + (size_t)slot * D;
+                const size_t bh = (size_t)(uint32_t)blk * a.H + h, base = (bh * a.P + slot) * D;
+                const uint8_t *ks = a.k + base + k_lane, *vs = a.v + base + v_lane;
                 const uint32_t dst = ring + stage * G::kSlot + lane * 16;
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int c = 0; c < G::kKC; ++c)
-                        cp16(dst + (nt * G::kKC + c) * 512, a.k + base + (nt * 8 + g) * D + c * 64 + q * 16);
+                    for (int c = 0; c < G::kKC; ++c) cp16(dst + (half * G::kKC + c) * 512, ks + half * 8 * D + c * 64);
                 const uint32_t vdst = ring + stage * G::kSlot + 16 * D + lane * G::kVB;
 #pragma unroll
                 for (int ts = 0; ts < 4; ++ts)
 #pragma unroll
                     for (int c = 0; c < G::kVC; ++c) {
-                        const void *src = a.v + base + (2 * q + (ts & 1) + (ts >> 1) * 8) * D + c * 128 + g * G::kVB;
+                        const void *src = vs + ((ts & 1) + (ts >> 1) * 8) * D + c * 128;
                         if (G::kVB == 16) cp16(vdst + (ts * G::kVC + c) * 512, src);
                         else cp8(vdst + ts * 256, src);
                     }
@@ -219,6 +164,73 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
             for (int s = 0; s < G::kStages - 1; ++s) issue(s, s, blk[s]);
         }
         int32_t next = entry(G::kStages - 1);
+
+        // ---- Q: rows g + 8 n, in the order in which codes arrive
+        uint32_t qf[NT][D / 16][2];
+        float fac[NT][2];           // of rows 2 q and 2 q + 1, as the scores have them
+        int32_t pos[NT][2], floors[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t row = r0 + g + 8 * n;
+            const bool in = row < r1;
+            const uint32_t tok = in ? token_of(a, row) : 0, head = h * a.G + (in ? row - tok * a.G : 0);
+            const QT *p = static_cast<const QT *>(a.q) + (int64_t)(r.q0 + tok) * a.q_st + (int64_t)head * a.q_sh;
+            uint32_t top = 0;
+#pragma unroll
+            for (int c = 0; c < G::kKC; ++c)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint4 v = in ? __ldg(reinterpret_cast<const uint4 *>(p + c * 64 + q * 16) + w) : make_uint4(0, 0, 0, 0);
+                    qf[n][c * 4 + w * 2][0] = v.x;
+                    qf[n][c * 4 + w * 2][1] = v.y;
+                    qf[n][c * 4 + w * 2 + 1][0] = v.z;
+                    qf[n][c * 4 + w * 2 + 1][1] = v.w;
+                }
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const QT *e = reinterpret_cast<const QT *>(&qf[n][s][w]);
+                    top = max(top, __float_as_uint(fabsf(Elem<QT>::to(e[0]))));
+                    top = max(top, __float_as_uint(fabsf(Elem<QT>::to(e[1]))));
+                }
+            top = max(top, __shfl_xor_sync(~0u, top, 1));
+            top = max(top, __shfl_xor_sync(~0u, top, 2));
+            // 2^(14 - exponent of the largest): into [2^14, 2^15); 0 and non-finite rows as they are
+            const int32_t e = (int32_t)(top >> 23) - 127;
+            const int32_t shift = (top == 0 || e == 128) ? 0 : max(-100, min(100, 14 - e));
+            const float m = __uint_as_float((uint32_t)(127 + shift) << 23);
+            const float f = a.scale_log2 * __uint_as_float((uint32_t)(127 - shift) << 23);
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) qf[n][s][w] = to_f16x2<QT>(qf[n][s][w], m);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fac[n][i] = __shfl_sync(~0u, f, (2 * q + i) * 4);
+                const uint32_t rw = r0 + 8 * n + 2 * q + i;
+                pos[n][i] = rw < r1 ? position(rw) : -1;
+                floors[n][i] = key_floor(pos[n][i]);
+            }
+        }
+        const int32_t pos_first = position(r0), floor_last = key_floor(position(r1 - 1));
+
+        // ---- key loop
+        float o[D / 16][NT][4];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                m[n][i] = -INFINITY;
+                l[n][i] = 0.0f;
+            }
         uint32_t stage = 0;
         for (uint32_t j = 0; j < take; ++j) {
             cp_wait<G::kStages - 2>();
@@ -231,26 +243,22 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
             if (live) {
                 const uint32_t src = ring + stage * G::kSlot;
                 const uint2 sc = pipe::lds64(src + 32 * D + lane * 8);
-                float s[2][4];
+                float s[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+                for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
-                    for (int c = 0; c < G::kKC; ++c) {
-                        const uint4 kw = pipe::lds128(src + (nt * G::kKC + c) * 512 + lane * 16);
-                        const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+                for (int c = 0; c < G::kKC; ++c) {
+                    const uint4 ka = pipe::lds128(src + c * 512 + lane * 16);                // key g
+                    const uint4 kb = pipe::lds128(src + (G::kKC + c) * 512 + lane * 16);     // key g + 8
+                    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t b0, b1;
-                            codes_to_f16<FMT>(w[i], b0, b1);
-                            if (G::kQSmem) {
-                                const uint4 f = qs[(c * 4 + i) * 32 + lane];
-                                pipe::mma16816_f16(s[nt], f.x, f.y, f.z, f.w, b0, b1);
-                            } else {
-                                uint32_t *f = qf[(c * 4 + i) % (G::kQSmem ? 1 : D / 16)];
-                                pipe::mma16816_f16(s[nt], f[0], f[1], f[2], f[3], b0, b1);
-                            }
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_f16<FMT>(wa[i], a0, a2);
+                        codes_to_f16<FMT>(wb[i], a1, a3);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            pipe::mma16816_f16(s[n], a0, a1, a2, a3, qf[n][c * 4 + i][0], qf[n][c * 4 + i][1]);
                     }
                 }
                 const uint32_t key = key0 + j * kGran;
@@ -258,58 +266,66 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
                 bool zero;
                 value_scale(__uint_as_float(sc.y), lv, inv, zero);
                 const float ks = __uint_as_float(sc.x);
-                const bool all = (int32_t)(key + 15) <= pos_first && (int32_t)key > floor_last && r1 - r0 == kRows;
-                float top[2];
+                // scores: [0], [1] of key g and rows 2 q, 2 q + 1; [2], [3] of key g + 8
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float f = fac[i] * ks;
-                    top[i] = -INFINITY;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt)
+                    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], fac[n][e & 1] * ks, lv);
+                if (!((int32_t)(key + 15) <= pos_first && (int32_t)key > floor_last)) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float t = fmaf(s[nt][2 * i + e], f, lv);
-                            if (!all) {
-                                const int32_t kp = (int32_t)(key + nt * 8 + 2 * q + e);
-                                if (kp > pos[i] || kp <= floors[i]) t = -INFINITY;
-                            }
-                            s[nt][2 * i + e] = t;
-                            top[i] = fmaxf(top[i], t);
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int32_t kp = (int32_t)(key + g + (e >> 1) * 8);
+                            if (kp > pos[n][e & 1] || kp <= floors[n][e & 1]) s[n][e] = -INFINITY;
                         }
-                    top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 1));
-                    top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], 2));
                 }
-                if (__any_sync(~0u, top[0] > m[0] || top[1] > m[1])) {
-                    float al[2];
+                bool raise = false;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) raise |= fmaxf(s[n][i], s[n][i + 2]) > m[n][i] + kRaiseA;
+                if (__any_sync(~0u, raise)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float al[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float top = fmaxf(s[n][i], s[n][i + 2]);
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                            const float to = fmaxf(m[n][i], top);
+                            al[i] = to == -INFINITY ? 1.0f : ex2(m[n][i] - to);
+                            m[n][i] = to;
+                            l[n][i] *= al[i];
+                        }
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            o[i][n][0] *= al[0];
+                            o[i][n][1] *= al[1];
+                            o[i][n][2] *= al[0];
+                            o[i][n][3] *= al[1];
+                        }
+                    }
+                }
+                uint32_t p[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float ms = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
+                        w[e] = ex2(s[n][e] - ms);
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float to = fmaxf(m[i], top[i]);
-                        al[i] = to == -INFINITY ? 1.0f : ex2(m[i] - to);
-                        m[i] = to;
-                        l[i] *= al[i];
+                        // a row that sees none of the keys takes nothing from their block, whatever its scale
+                        const float sum = w[i] + w[i + 2];
+                        l[n][i] += sum == 0.0f ? 0.0f : sum * inv;
+                        const __half2 hh = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+                        const uint32_t v = turn8x8(*reinterpret_cast<const uint32_t *>(&hh));
+                        p[n][i] = zero ? 0u : v;
                     }
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        o[i][0] *= al[0];
-                        o[i][1] *= al[0];
-                        o[i][2] *= al[1];
-                        o[i][3] *= al[1];
-                    }
-                }
-                uint32_t p[4];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float ms = m[i] == -INFINITY ? 0.0f : m[i];
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) {
-                        const float w0 = ex2(s[nt][2 * i] - ms), w1 = ex2(s[nt][2 * i + 1] - ms);
-                        sum += w0 + w1;
-                        const __half2 hh = __floats2half2_rn(w0, w1);
-                        p[nt * 2 + i] = zero ? 0u : *reinterpret_cast<const uint32_t *>(&hh);
-                    }
-                    // a row that sees none of these keys takes nothing from the block, whatever its scale
-                    l[i] += (sum == 0.0f) ? 0.0f : sum * inv;
                 }
                 const bool tail = key + 16 > hi;
 #pragma unroll
@@ -329,22 +345,25 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
                             vw[ts][1] = v.y;
                             vw[ts][2] = vw[ts][3] = 0;
                         }
+                    }
+                    if (tail) {
                         // slots behind the last key may hold anything
-                        if (tail && key + 2 * q + (ts & 1) + (ts >> 1) * 8 >= hi)
-                            vw[ts][0] = vw[ts][1] = vw[ts][2] = vw[ts][3] = 0;
+#pragma unroll
+                        for (int ts = 0; ts < 4; ++ts)
+                            if (key + 2 * q + (ts & 1) + (ts >> 1) * 8 >= hi) vw[ts][0] = vw[ts][1] = vw[ts][2] = vw[ts][3] = 0;
                     }
 #pragma unroll
                     for (int i = 0; i < G::kVB / 4; ++i)
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            // bytes 2 half, 2 half + 1 of two keys: (a, b, a, b)
+                            // bytes 2 half, 2 half + 1 of two keys: (a, b, a, b); two dimensions of the tile's 16
                             const uint32_t sel = half ? 0x7362 : 0x5140;
-                            uint32_t b0, b1, b2, b3;
-                            codes_to_f16<FMT>(__byte_perm(vw[0][i], vw[1][i], sel), b0, b2);
-                            codes_to_f16<FMT>(__byte_perm(vw[2][i], vw[3][i], sel), b1, b3);
-                            const int t = c * G::kVB + i * 4 + half * 2;
-                            pipe::mma16816_f16(o[t], p[0], p[1], p[2], p[3], b0, b1);
-                            pipe::mma16816_f16(o[t + 1], p[0], p[1], p[2], p[3], b2, b3);
+                            uint32_t a0, a1, a2, a3;
+                            codes_to_f16<FMT>(__byte_perm(vw[0][i], vw[1][i], sel), a0, a1);
+                            codes_to_f16<FMT>(__byte_perm(vw[2][i], vw[3][i], sel), a2, a3);
+                            const int t = c * (G::kVB / 2) + i * 2 + half;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) pipe::mma16816_f16(o[t][n], a0, a1, a2, a3, p[n][0], p[n][1]);
                         }
                 }
             }
@@ -354,34 +373,39 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
 
         // ---- join the four warps
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(~0u, l[i], 1);
-            l[i] += __shfl_xor_sync(~0u, l[i], 2);
-            if (q == 0) {
-                sh_m[warp][g + 8 * i] = m[i];
-                sh_l[warp][g + 8 * i] = l[i];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[n][i] += __shfl_xor_sync(~0u, l[n][i], d);
+                if (g == 0) {
+                    sh_m[warp][8 * n + 2 * q + i] = m[n][i];
+                    sh_l[warp][8 * n + 2 * q + i] = l[n][i];
+                }
             }
-        }
         __syncthreads();
-        float wt[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarpsA; ++w) top = fmaxf(top, sh_m[w][g + 8 * i]);
-            wt[i] = top == -INFINITY ? 1.0f : ex2(m[i] - top);
-        }
         float *mine = merge + warp * kRows * (D + G::kPad);
 #pragma unroll
-        for (int t = 0; t < D / 8; ++t) {
-            const int d = (t / G::kVB) * 128 + (t % G::kVB);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                mine[(g + (e >> 1) * 8) * (D + G::kPad) + d + (2 * q + (e & 1)) * G::kVB] = o[t][e] * wt[e >> 1];
-        }
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t rr = 8 * n + 2 * q + i;
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarpsA; ++w) top = fmaxf(top, sh_m[w][rr]);
+                const float wt = top == -INFINITY ? 1.0f : ex2(m[n][i] - top);
+#pragma unroll
+                for (int c = 0; c < G::kVC; ++c)
+#pragma unroll
+                    for (int t = 0; t < G::kVB / 2; t += 2) {
+                        const float(&x)[4] = o[c * (G::kVB / 2) + t][n], (&y)[4] = o[c * (G::kVB / 2) + t + 1][n];
+                        *reinterpret_cast<float4 *>(mine + rr * (D + G::kPad) + c * 128 + g * G::kVB + 2 * t) =
+                            make_float4(x[i] * wt, x[i + 2] * wt, y[i] * wt, y[i + 2] * wt);
+                    }
+            }
         __syncthreads();
         const bool whole = seg.begins && take == seg.n;
-        float *part = a.part + (size_t)(2 * blockIdx.x + (seg.begins ? 1 : 0)) * part_floats<kRows, D>();
+        float *part = a.part + (size_t)(2 * blockIdx.x + (seg.begins ? 1 : 0)) * part_floats<kMostRows, D>();
         for (uint32_t i = tid; i < kRows * (D / 4); i += kThreadsA) {
             const uint32_t rr = i / (D / 4), d = (i % (D / 4)) * 4;
             if (r0 + rr >= r1) break;
@@ -411,8 +435,8 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
             } else {
                 *reinterpret_cast<float4 *>(part + rr * D + d) = v;
                 if (d == 0) {
-                    part[kRows * D + rr] = top;
-                    part[kRows * D + kRows + rr] = sum;
+                    part[kMostRows * D + rr] = top;
+                    part[kMostRows * D + kMostRows + rr] = sum;
                 }
             }
         }
@@ -421,41 +445,42 @@ __global__ void __launch_bounds__(kThreadsA, Geo<D>::kCtas) attn_mma_kernel(cons
     }
 }
 
-template <int D, typename QT> __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a)
+template <int D, typename QT, int NT> __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a)
 {
     wait_previous();
-    join_row<kRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
+    join_row<8 * NT, kMostRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
 }
 
-template <int D, int FMT, typename QT> cudaError_t launch_one(const AttnArgs &a, uint32_t grid, bool join, cudaStream_t s)
+template <int D, int FMT, typename QT, int NT> cudaError_t launch_one(const AttnArgs &a, uint32_t grid, cudaStream_t s)
 {
-    auto kernel = attn_mma_kernel<D, FMT, QT>;
+    auto kernel = attn_mma_kernel<D, FMT, QT, NT>;
     static std::atomic<uint64_t> ready{0};
     cudaError_t e = allow_smem(kernel, Geo<D>::kSmem, ready);
     if (e != cudaSuccess) return e;
     kernel<<<grid, kThreadsA, Geo<D>::kSmem, s>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess || !join) return e;
-    return launch_behind(attn_join_kernel<D, QT>, dim3(grid, kRows / 4), dim3(128), 0, s, a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    return launch_behind(attn_join_kernel<D, QT, NT>, dim3(grid, 2 * NT), dim3(128), 0, s, a);
 }
 
-template <int D> cudaError_t launch_dim(const AttnArgs &a, uint32_t fmt, int elem, uint32_t grid, bool join, cudaStream_t s)
+template <int D, int FMT, typename QT> cudaError_t launch_rows(const AttnArgs &a, bool few, uint32_t grid, cudaStream_t s)
+{
+    if constexpr (D == 256) return launch_one<D, FMT, QT, 1>(a, grid, s);   // 16 rows' accumulators would not fit
+    else return few ? launch_one<D, FMT, QT, 1>(a, grid, s) : launch_one<D, FMT, QT, 2>(a, grid, s);
+}
+
+template <int D> cudaError_t launch_dim(const AttnArgs &a, uint32_t fmt, int elem, bool few, uint32_t grid, cudaStream_t s)
 {
     if (elem == HXQ_ELEM_BF16)
-        return fmt == HXQ_KV_INT8 ? launch_one<D, HXQ_KV_INT8, __nv_bfloat16>(a, grid, join, s)
-                                  : launch_one<D, HXQ_KV_E4M3, __nv_bfloat16>(a, grid, join, s);
-    return fmt == HXQ_KV_INT8 ? launch_one<D, HXQ_KV_INT8, __half>(a, grid, join, s)
-                              : launch_one<D, HXQ_KV_E4M3, __half>(a, grid, join, s);
+        return fmt == HXQ_KV_INT8 ? launch_rows<D, HXQ_KV_INT8, __nv_bfloat16>(a, few, grid, s)
+                                  : launch_rows<D, HXQ_KV_E4M3, __nv_bfloat16>(a, few, grid, s);
+    return fmt == HXQ_KV_INT8 ? launch_rows<D, HXQ_KV_INT8, __half>(a, few, grid, s)
+                              : launch_rows<D, HXQ_KV_E4M3, __half>(a, few, grid, s);
 }
 
-cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, uint32_t grid, bool join, cudaStream_t s)
+cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, bool few, uint32_t grid, cudaStream_t s)
 {
-    return D == 64 ? launch_dim<64>(a, fmt, elem, grid, join, s)
-                   : D == 128 ? launch_dim<128>(a, fmt, elem, grid, join, s) : launch_dim<256>(a, fmt, elem, grid, join, s);
-}
-
-uint32_t attn_mma_ctas_per_sm(uint32_t D)
-{
-    return D == 256 ? Geo<256>::kCtas : Geo<128>::kCtas;
+    return D == 64 ? launch_dim<64>(a, fmt, elem, few, grid, s)
+                   : D == 128 ? launch_dim<128>(a, fmt, elem, few, grid, s) : launch_dim<256>(a, fmt, elem, few, grid, s);
 }
 
 hxq_error_t check_attention(const hxq_kv_cache_t *c, const hxq_kv_attention_t *p)
@@ -477,20 +502,22 @@ hxq_error_t check_attention(const hxq_kv_cache_t *c, const hxq_kv_attention_t *p
 // kernel and of the one for many rows.
 struct AttnLayout {
     uint32_t ctas, tc_ctas;
+    bool few;                     // tiles of 8 rows
     size_t part, tc_desc, tc_part, bytes;
 };
 
 // Requests with more rows than this go to the tcgen05 kernel.
 constexpr uint32_t kFewRows = 64;
 
-AttnLayout attn_layout(uint32_t D, uint64_t most_rows)
+AttnLayout attn_layout(uint32_t D, uint64_t most_rows)   // most_rows: of a request, as the caller says
 {
     AttnLayout l;
     const uint32_t sms = (uint32_t)sm_count();
-    l.ctas = sms * attn_mma_ctas_per_sm(D);
+    l.few = D == 256 || most_rows <= 8;
+    l.ctas = sms * ctas_per_sm(D, l.few);
     l.tc_ctas = D != 256 && most_rows > kFewRows ? sms : 0;
     l.part = l.ctas * sizeof(int4);
-    l.tc_desc = l.part + (size_t)l.ctas * 2 * (kRows * D + 2 * kRows) * sizeof(float);
+    l.tc_desc = l.part + (size_t)l.ctas * 2 * (kMostRows * D + 2 * kMostRows) * sizeof(float);
     l.tc_part = l.tc_desc + l.tc_ctas * sizeof(int4);
     l.bytes = l.tc_part + (size_t)l.tc_ctas * 2 * (kTcRows * D + 2 * kTcRows) * sizeof(float);
     return l;
@@ -557,12 +584,12 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     a.desc = reinterpret_cast<int4 *>(ws);
     a.part = reinterpret_cast<float *>(ws + lay.part);
     // Few rows of a request: this file's kernel. More: the tcgen05 kernel (64
-    // is where a tile of 16 rows reads the keys four times over; that kernel
+    // is where tiles of 16 rows read the keys four times over; that kernel
     // takes 128 rows at a time). Without rows of the other kind a launch ends
     // after its scan of the lengths.
     if (lay.tc_ctas) a.row_max = kFewRows;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_attn_mma(a, cache->head_dim, cache->format, args->elem, lay.ctas, true, s);
+    cudaError_t e = launch_attn_mma(a, cache->head_dim, cache->format, args->elem, lay.few, lay.ctas, s);
     if (e == cudaSuccess && lay.tc_ctas) {
         a.row_min = kFewRows;
         a.row_max = 0xffffffffu;

@@ -359,43 +359,67 @@ __device__ __forceinline__ void value_scale(float vs, float &lv, float &inv, boo
     zero = vs < 7.8886090522101181e-31f;   // 2^-100
     const float c = zero ? 7.8886090522101181e-31f : vs;
     lv = lg2(c);
-    inv = __frcp_rn(c);
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(c));   // within an ulp
 }
 
 // Partial results of a CTA: two slots of ROWS x D sums, then the rows' maxima
 // and sums; slot 0 a unit begun by the CTA in front, slot 1 one not finished.
 template <int ROWS, int D> __host__ __device__ constexpr size_t part_floats() { return (size_t)ROWS * D + 2 * ROWS; }
 
-// Joins the parts of the unit that CTA blockIdx.x began and did not finish:
-// its own second slot, then the first slots of the CTAs behind it, in order.
-// A warp takes a row.
-template <int ROWS, int D, typename QT>
+// Joins the parts of the unit that CTA `cta` began and did not finish: its own
+// second slot, then the first slots of the CTAs behind it, in order.  A warp
+// takes row rr of the unit's tile of ROWS (SLOT rows a slot); a lane looks
+// after the weight of a part.
+template <int ROWS, int SLOT, int D, typename QT>
 __device__ __forceinline__ void join_row(const AttnArgs &a, const int4 *desc, const float *parts, uint32_t cta, uint32_t rr)
 {
     const int4 d = desc[cta];
     if (d.x == 0) return;
-    const Req r = load_req(a, (uint32_t)d.y);
-    const uint32_t row = (uint32_t)d.w * ROWS + rr, lane = threadIdx.x & 31;
-    if (row >= r.rows) return;
-    constexpr size_t kPart = part_floats<ROWS, D>();
-    const float *first = parts + (2 * (size_t)cta + 1) * kPart, *rest = parts + 2 * ((size_t)cta + 1) * kPart;
-    auto part = [&](int i) { return i == 0 ? first : rest + (size_t)(i - 1) * 2 * kPart; };
-    float top = -INFINITY;
-    for (int i = lane; i < d.x; i += 32) top = fmaxf(top, part(i)[ROWS * D + rr]);
+    constexpr size_t kPart = part_floats<SLOT, D>();
+    const uint32_t lane = threadIdx.x & 31;
+    const float *first = parts + (2 * (size_t)cta + 1) * kPart, *rest = parts + 2 * (size_t)cta * kPart;
+    auto part = [&](int i) { return i == 0 ? first : rest + (size_t)i * 2 * kPart; };
+    // a first batch of sums while the weights are found
+    constexpr int N = D / 32, kAhead = 8;
+    float v[N], u[kAhead][N], sum = 0.0f, top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) u[i][j] = i < d.x ? part(i)[rr * D + j * 32 + lane] : 0.0f;
+    for (int i = lane; i < d.x; i += 32) top = fmaxf(top, part(i)[SLOT * D + rr]);
 #pragma unroll
     for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, m));
-    constexpr int N = D / 32;
-    float v[N], sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < d.x; ++i) {
-        const float *p = part(i);
-        const float m = p[ROWS * D + rr], w = top == -INFINITY ? 1.0f : ex2(m - top);
-        sum += p[ROWS * D + ROWS + rr] * w;
+    for (int i0 = 0; i0 < d.x; i0 += 32) {
+        float w = 0.0f, s = 0.0f;
+        if (i0 + (int)lane < d.x) {
+            const float *p = part(i0 + lane) + SLOT * D + rr;
+            w = top == -INFINITY ? 1.0f : ex2(p[0] - top);
+            s = p[SLOT];
+        }
+#pragma unroll 1
+        for (int k = 0; k < min(32, d.x - i0); k += kAhead) {
+            if (i0 + k > 0) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] += p[rr * D + j * 32 + lane] * w;
+                for (int i = 0; i < kAhead; ++i)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) u[i][j] = i0 + k + i < d.x ? part(i0 + k + i)[rr * D + j * 32 + lane] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const float wi = __shfl_sync(~0u, w, k + i), si = __shfl_sync(~0u, s, k + i);
+                if (i0 + k + i < d.x) {
+                    sum += si * wi;
+#pragma unroll
+                    for (int j = 0; j < N; ++j) v[j] += u[i][j] * wi;
+                }
+            }
+        }
     }
+    const Req r = load_req(a, (uint32_t)d.y);
+    const uint32_t row = (uint32_t)d.w * ROWS + rr;
+    if (row >= r.rows) return;
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
     const uint32_t tk = token_of(a, row), tok = r.q0 + tk, head = (uint32_t)d.z * a.G + (row - tk * a.G);
     QT *dst = static_cast<QT *>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
@@ -410,8 +434,7 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const int4 *desc, co
 constexpr int kTcRows = 256;
 cudaError_t launch_attn_tc(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, uint32_t grid, cudaStream_t s);
 
-cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, uint32_t grid, bool join, cudaStream_t s);
-uint32_t attn_mma_ctas_per_sm(uint32_t D);
+cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, bool few, uint32_t grid, cudaStream_t s);
 
 }  // namespace serving
 }  // namespace hxq

@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
 template <int D, typename QT> __global__ void __launch_bounds__(128) attn_tc_join_kernel(const __grid_constant__ AttnArgs a)
 {
     wait_previous();
-    for (uint32_t rr = threadIdx.x >> 5; rr < 32; rr += 4) join_row<kTcRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 32 + rr);
+    join_row<kTcRows, kTcRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
 }
 
 template <int D, int FMT, typename QT> cudaError_t launch_tc_one(const AttnArgs &a, uint32_t grid, cudaStream_t s)
@@ -756,7 +756,7 @@ template <int D, int FMT, typename QT> cudaError_t launch_tc_one(const AttnArgs 
     if (e != cudaSuccess) return e;
     kernel<<<grid, kThreadsT, TcGeo<D>::kSmem, s>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_behind(attn_tc_join_kernel<D, QT>, dim3(grid, kTcRows / 32), dim3(128), 0, s, a);
+    return launch_behind(attn_tc_join_kernel<D, QT>, dim3(grid, kTcRows / 4), dim3(128), 0, s, a);
 }
 
 template <int D> cudaError_t launch_tc_dim(const AttnArgs &a, uint32_t fmt, int elem, uint32_t grid, cudaStream_t s)
