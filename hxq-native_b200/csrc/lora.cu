@@ -140,7 +140,6 @@ struct LoraArgs {
     int64_t ldx, ldy, ldo;
     uint32_t T, n, R, I, O, parts, span;   // span: in_features of a part, a multiple of 128
     uint32_t pairs;                        // expand: 16-output pieces a warp takes
-    uint32_t wide;                         // y and out rows allow 16-byte accesses
 };
 
 // A tile's positions come from device memory that the caller could have
@@ -156,46 +155,97 @@ __device__ __forceinline__ bool load_tile(const LoraArgs &a, uint32_t i, int32_t
     return true;
 }
 
-// h[token, r] over [k0, k1): warps take 32 consecutive k in turn.  A lane holds
-// 8 consecutive k of a row (16 bytes), the same ones of A and x, which are the
-// operands of two m16n8k16 products.
-template <int NT> __device__ __forceinline__ void shrink_body(const LoraArgs &a, const uint16_t *A, uint32_t rows, const int64_t *xrow,
-                                                              uint32_t count, uint32_t k0, uint32_t k1, float (&acc)[2][8][4])
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool wanted)
 {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    const uint16_t *xp[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) xp[n] = a.x + xrow[n * 8 + g];
-#pragma unroll 2
-    for (uint32_t k = k0 + warp * 32 + q * 8; k - q * 8 < k1; k += 128) {
-        const bool in = k < k1;
-        uint4 av[4], xv[NT];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            av[i] = in && i * 8 + g < rows ? __ldg(reinterpret_cast<const uint4 *>(A + (size_t)(i * 8 + g) * a.I + k)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            xv[n] = in && n * 8 + g < count ? __ldg(reinterpret_cast<const uint4 *>(xp[n] + k)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                pipe::mma16816_bf16(acc[m][n], av[2 * m].x, av[2 * m + 1].x, av[2 * m].y, av[2 * m + 1].y, xv[n].x, xv[n].y);
-                pipe::mma16816_bf16(acc[m][n], av[2 * m].z, av[2 * m + 1].z, av[2 * m].w, av[2 * m + 1].w, xv[n].z, xv[n].w);
-            }
-    }
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(wanted ? 16 : 0) : "memory");
 }
 
-__global__ void __launch_bounds__(128) shrink_kernel(const __grid_constant__ LoraArgs a)
+constexpr int kShrinkRing = 24 * 1024;   // bytes of a warp's ring
+
+// h[token, r] over [k0, k1) for 8 NT tokens: warps take 32 consecutive k in
+// turn.  A lane holds 8 consecutive k of a row (16 bytes), the same ones of A
+// and x, which are the operands of two m16n8k16 products; the pieces come
+// through slots of shared memory that no other lane reads (cp.async, several
+// steps ahead, no barrier): 24 KB a warp under way, two CTAs an SM.
+template <int NT>
+__device__ __forceinline__ void shrink_body(const LoraArgs &a, const uint16_t *A, uint32_t rows, const int64_t *xrow, uint32_t count,
+                                            uint32_t k0, uint32_t k1, uint32_t ring, float (*red)[kShrinkRanks][kTile + 1])
 {
+    constexpr int kStep = (4 + NT) * 512, kStages = kShrinkRing / kStep < 8 ? kShrinkRing / kStep : 8;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
+    const uint16_t *ap = A + (size_t)g * a.I, *xp[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xp[n] = a.x + xrow[n * 8 + g];
+    const uint32_t dst0 = ring + lane * 16;
+    auto issue = [&](uint32_t k, uint32_t stage) {   // k: this lane's
+        const uint32_t dst = dst0 + stage * kStep;
+        const bool in = k < k1;
+        const uint32_t kk = in ? k : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool w = in && i * 8 + g < rows;
+            copy16(dst + i * 512, w ? ap + (size_t)i * 8 * a.I + kk : A, w);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) copy16(dst + (4 + n) * 512, xp[n] + kk, in && n * 8 + g < count);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float acc[2][NT][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.0f;
+    const uint32_t first = k0 + warp * 32 + q * 8, steps = k0 + warp * 32 < k1 ? (k1 - k0 - warp * 32 + 127) / 128 : 0;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(first + i * 128, i);
+    uint32_t stage = 0;
+    for (uint32_t i = 0; i < steps; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        issue(first + (i + kStages - 1) * 128, stage == 0 ? kStages - 1 : stage - 1);
+        const uint32_t src = dst0 + stage * kStep;
+        uint4 av[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) av[r] = pipe::lds128(src + r * 512);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint4 xv = pipe::lds128(src + (4 + n) * 512);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                pipe::mma16816_bf16(acc[m][n], av[2 * m].x, av[2 * m + 1].x, av[2 * m].y, av[2 * m + 1].y, xv.x, xv.y);
+                pipe::mma16816_bf16(acc[m][n], av[2 * m].z, av[2 * m + 1].z, av[2 * m].w, av[2 * m + 1].w, xv.z, xv.w);
+            }
+        }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    // the four warps' sums: (0 + 2) + (1 + 3), the latter added by the caller
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f(acc[m][n][e], m * 16 + g + (e >> 1) * 8, n * 8 + 2 * q + (e & 1));
+    };
+    if (warp >= 2) each([&](float v, int r, int t) { red[warp - 2][r][t] = v; });
+    __syncthreads();
+    if (warp < 2) each([&](float v, int r, int t) { red[warp][r][t] += v; });
+    __syncthreads();
+}
+
+__global__ void __launch_bounds__(128, 2) shrink_kernel(const __grid_constant__ LoraArgs a)
+{
+    extern __shared__ __align__(128) uint8_t rings[];
     __shared__ float red[2][kShrinkRanks][kTile + 1];
     __shared__ int64_t xrow[kTile];
-    let_next_start();
     wait_previous();
+    let_next_start();   // not before: the next kernel reads y ahead of its own wait
     int32_t id;
     uint32_t first, count;
     if (!load_tile(a, blockIdx.x, id, first, count) || id < 0) return;
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
+    const uint32_t tid = threadIdx.x;
     if (tid < kTile) {
         const int32_t t = tid < count ? a.order[first + tid] : 0;
         xrow[tid] = (int64_t)((uint32_t)t < a.T ? t : 0) * a.ldx;
@@ -204,32 +254,11 @@ __global__ void __launch_bounds__(128) shrink_kernel(const __grid_constant__ Lor
     const uint32_t r0 = blockIdx.z * kShrinkRanks, rows = min((uint32_t)kShrinkRanks, a.R - r0);
     const uint16_t *A = a.A + ((size_t)id * a.R + r0) * a.I;
     const uint32_t k0 = blockIdx.y * a.span, k1 = min(k0 + a.span, a.I);
-    float acc[2][8][4];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[m][n][e] = 0.0f;
-    if (count <= 8) shrink_body<1>(a, A, rows, xrow, count, k0, k1, acc);
-    else if (count <= 16) shrink_body<2>(a, A, rows, xrow, count, k0, k1, acc);
-    else if (count <= 32) shrink_body<4>(a, A, rows, xrow, count, k0, k1, acc);
-    else shrink_body<8>(a, A, rows, xrow, count, k0, k1, acc);
-    // the four warps' sums: (0 + 2) + (1 + 3)
-    const uint32_t tiles = (count + 7) / 8;
-    auto each = [&](auto f) {
-#pragma unroll
-        for (int n = 0; n < 8; ++n)
-            if (n < (int)tiles)
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) f(acc[m][n][e], m * 16 + g + (e >> 1) * 8, n * 8 + 2 * q + (e & 1));
-    };
-    if (warp >= 2) each([&](float v, int r, int t) { red[warp - 2][r][t] = v; });
-    __syncthreads();
-    if (warp < 2) each([&](float v, int r, int t) { red[warp][r][t] += v; });
-    __syncthreads();
+    const uint32_t ring = pipe::smem_u32(rings) + (tid >> 5) * kShrinkRing;
+    if (count <= 8) shrink_body<1>(a, A, rows, xrow, count, k0, k1, ring, red);
+    else if (count <= 16) shrink_body<2>(a, A, rows, xrow, count, k0, k1, ring, red);
+    else if (count <= 32) shrink_body<4>(a, A, rows, xrow, count, k0, k1, ring, red);
+    else shrink_body<8>(a, A, rows, xrow, count, k0, k1, ring, red);
     float *h = a.h + (size_t)blockIdx.y * a.T * a.R;
     for (uint32_t i = tid; i < count * rows; i += 128) {
         const uint32_t t = i / rows, r = i - t * rows;
@@ -237,48 +266,129 @@ __global__ void __launch_bounds__(128) shrink_kernel(const __grid_constant__ Lor
     }
 }
 
+__device__ __forceinline__ float4 load4(const float *p)
+{
+    float4 v;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float load1(const float *p)
+{
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load2(const uint16_t *p)
+{
+    uint2 v;
+    asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
 // out = y + (s h) B^T: 16 tokens x 16 outputs at a time.  The two 8-output
 // products of a piece take outputs {0,1,4,5,8,..} and {2,3,6,7,..}, so a lane
-// ends with four consecutive outputs of a token (16-byte accesses of y).
-template <int KS> __global__ void __launch_bounds__(128) expand_kernel(const __grid_constant__ LoraArgs a)
+// ends with four consecutive outputs of a token (16-byte accesses of y).  A
+// piece's B and y of the whole tile are loaded together, the first piece's
+// before the shrink kernel's results are waited for.
+template <int KS, bool WIDE> __global__ void __launch_bounds__(128) expand_kernel(const __grid_constant__ LoraArgs a)
 {
-    // s h of the tile as operand fragments: [token group][k step][hi, lo][lane]
+    // s h of the tile as operand fragments: [token group][k step][three parts][lane]
     extern __shared__ uint4 frag[];
     __shared__ int32_t rows[kTile];
-    wait_previous();
     int32_t id;
     uint32_t first, count;
-    if (!load_tile(a, blockIdx.x, id, first, count)) return;
+    if (!load_tile(a, blockIdx.x, id, first, count)) {
+        wait_previous();
+        return;
+    }
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
     if (tid < kTile) {
         const int32_t t = tid < count ? a.order[first + tid] : -1;
         rows[tid] = (uint32_t)t < a.T ? t : -1;
     }
-    const uint32_t o0 = (blockIdx.y * 4 + warp) * a.pairs * 16;
+    __syncthreads();
+    // the CTA's warps side by side, so that it reads and writes 256 bytes of a
+    // row of y at a time (64-byte pieces far apart: 2.5 times slower)
+    const uint32_t o0 = (blockIdx.y * a.pairs * 4 + warp) * 16;
     if (id < 0) {
         // no adapter: out is y
-        __syncthreads();
+        wait_previous();
         if (a.out == a.y && a.ldo == a.ldy) return;
-        const uint32_t n = min(a.pairs * 16, a.O > o0 ? a.O - o0 : 0);
-        for (uint32_t t = 0; t < count; ++t) {
-            if (rows[t] < 0) continue;
-            const float *src = a.y + (int64_t)rows[t] * a.ldy + o0;
-            float *dst = a.out + (int64_t)rows[t] * a.ldo + o0;
-            for (uint32_t i = lane; i < n; i += 32) dst[i] = src[i];
+        const uint32_t c0 = blockIdx.y * a.pairs * 64, n = min(a.pairs * 64, a.O > c0 ? a.O - c0 : 0);
+        if (WIDE) {
+            // 8 pieces of 16 bytes a thread under way
+            const uint32_t per = n / 4, all = count * per;
+            for (uint32_t i0 = tid; i0 < all; i0 += 128 * 8) {
+                float4 v[8];
+#pragma unroll
+                for (uint32_t u = 0; u < 8; ++u) {
+                    const uint32_t i = i0 + u * 128, t = min(i, all - 1) / per;
+                    v[u] = load4(a.y + (int64_t)max(rows[t], 0) * a.ldy + c0 + (min(i, all - 1) - t * per) * 4);
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < 8; ++u) {
+                    const uint32_t i = i0 + u * 128, t = min(i, all - 1) / per;
+                    if (i < all && rows[t] >= 0)
+                        *reinterpret_cast<float4 *>(a.out + (int64_t)rows[t] * a.ldo + c0 + (i - t * per) * 4) = v[u];
+                }
+            }
+        } else {
+            for (uint32_t t = warp; t < count; t += 4) {
+                if (rows[t] < 0) continue;
+                const float *src = a.y + (int64_t)rows[t] * a.ldy + c0;
+                float *dst = a.out + (int64_t)rows[t] * a.ldo + c0;
+                for (uint32_t i = lane; i < n; i += 32) dst[i] = load1(src + i);
+            }
         }
         return;
     }
     const uint32_t groups = (count + 15) / 16;
+    const uint16_t *Bm = a.Bm + (size_t)id * a.O * a.R;
+    uint2 b[2][KS];
+    float4 y[4][2];   // [token group][token g, g + 8]
+    // loads that stay where they are written, all before the first use; a row
+    // or column that does not exist reads one that does
+    auto load = [&](uint32_t o) {
+        const uint32_t at = o + q * 4;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            if (m >= (int)groups) break;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int32_t tok = rows[m * 16 + g + 8 * r];
+                const float *src = a.y + (int64_t)max(tok, 0) * a.ldy;
+                if (WIDE) y[m][r] = load4(src + (at < a.O ? at : 0));
+                else {
+                    y[m][r].x = load1(src + min(at, a.O - 1));
+                    y[m][r].y = load1(src + min(at + 1, a.O - 1));
+                    y[m][r].z = load1(src + min(at + 2, a.O - 1));
+                    y[m][r].w = load1(src + min(at + 3, a.O - 1));
+                }
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const uint32_t col = min(o + (g >> 1) * 4 + (g & 1) + 2 * w, a.O - 1);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                b[w][k] = make_uint2(0, 0);
+                if (k * 16 + q * 4 < a.R) b[w][k] = load2(Bm + (size_t)col * a.R + k * 16 + q * 4);
+            }
+        }
+    };
     const float scale = a.scales[id];
+    if (o0 < a.O) load(o0);
+    wait_previous();
     for (uint32_t i = warp; i < groups * KS; i += 4) {
         const uint32_t m = i / KS, k = i % KS;
-        uint32_t hi[4], lo[4];
+        uint32_t w3[3][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const uint32_t t = m * 16 + g + 8 * r, c = k * 16 + q * 4;
             float4 v = make_float4(0, 0, 0, 0);
             if (t < count && c < a.R) {
                 const float *h = a.h + (size_t)(first + t) * a.R + c;
+#pragma unroll 4
                 for (uint32_t p = 0; p < a.parts; ++p) {
                     const float4 u = *reinterpret_cast<const float4 *>(h + (size_t)p * a.T * a.R);
                     v.x += u.x;
@@ -287,72 +397,50 @@ template <int KS> __global__ void __launch_bounds__(128) expand_kernel(const __g
                     v.w += u.w;
                 }
             }
-            const float f[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+            float f[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const __nv_bfloat162 top = __floats2bfloat162_rn(f[2 * w], f[2 * w + 1]);
-                const float2 back = __bfloat1622float2(top);
-                const __nv_bfloat162 rest = __floats2bfloat162_rn(f[2 * w] - back.x, f[2 * w + 1] - back.y);
-                hi[w * 2 + r] = *reinterpret_cast<const uint32_t *>(&top);
-                lo[w * 2 + r] = *reinterpret_cast<const uint32_t *>(&rest);
-            }
-        }
-        frag[(i * 2) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        frag[(i * 2 + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    __syncthreads();
-    const uint16_t *Bm = a.Bm + (size_t)id * a.O * a.R;
-    for (uint32_t j = 0; j < a.pairs; ++j) {
-        const uint32_t o = o0 + j * 16;
-        if (o >= a.O) break;
-        uint2 b[2][KS];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            const uint32_t col = o + (g >> 1) * 4 + (g & 1) + 2 * w;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-                b[w][k] = col < a.O && k * 16 + q * 4 < a.R
-                              ? __ldg(reinterpret_cast<const uint2 *>(Bm + (size_t)col * a.R + k * 16 + q * 4)) : make_uint2(0, 0);
-        }
-        const uint32_t at = o + q * 4;
-        const bool wide = a.wide && at + 4 <= a.O;
-        for (uint32_t m = 0; m < groups; ++m) {
-            float v[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};   // [token g, g + 8]
-            int32_t tok[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                tok[r] = rows[m * 16 + g + 8 * r];
-                if (tok[r] < 0) continue;
-                const float *src = a.y + (int64_t)tok[r] * a.ldy + at;
-                if (wide) {
-                    const float4 u = *reinterpret_cast<const float4 *>(src);
-                    v[r][0] = u.x;
-                    v[r][1] = u.y;
-                    v[r][2] = u.z;
-                    v[r][3] = u.w;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (at + e < a.O) v[r][e] = src[e];
-                }
-            }
-            float d[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const uint4 hi = frag[((m * KS + k) * 2) * 32 + lane], lo = frag[((m * KS + k) * 2 + 1) * 32 + lane];
+            for (int part = 0; part < 3; ++part)
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    pipe::mma16816_bf16(d[w], hi.x, hi.y, hi.z, hi.w, b[w][k].x, b[w][k].y);
-                    pipe::mma16816_bf16(d[w], lo.x, lo.y, lo.z, lo.w, b[w][k].x, b[w][k].y);
+                    const __nv_bfloat162 top = __floats2bfloat162_rn(f[2 * w], f[2 * w + 1]);
+                    const float2 back = __bfloat1622float2(top);
+                    f[2 * w] -= back.x;
+                    f[2 * w + 1] -= back.y;
+                    w3[part][w * 2 + r] = *reinterpret_cast<const uint32_t *>(&top);
                 }
-            }
+        }
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+            frag[(i * 3 + part) * 32 + lane] = make_uint4(w3[part][0], w3[part][1], w3[part][2], w3[part][3]);
+    }
+    __syncthreads();
+    for (uint32_t j = 0; j < a.pairs; ++j) {
+        const uint32_t o = o0 + j * 64;
+        if (o >= a.O) break;
+        if (j) load(o);
+        const uint32_t at = o + q * 4;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            if (m >= (int)groups) break;
+            float d[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int part = 2; part >= 0; --part) {
+                    const uint4 h = frag[((m * KS + k) * 3 + part) * 32 + lane];
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) pipe::mma16816_bf16(d[w], h.x, h.y, h.z, h.w, b[w][k].x, b[w][k].y);
+                }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                if (tok[r] < 0) continue;
-                float *dst = a.out + (int64_t)tok[r] * a.ldo + at;
-                const float s[4] = {v[r][0] + d[0][2 * r], v[r][1] + d[0][2 * r + 1], v[r][2] + d[1][2 * r], v[r][3] + d[1][2 * r + 1]};
-                if (wide) *reinterpret_cast<float4 *>(dst) = make_float4(s[0], s[1], s[2], s[3]);
-                else {
+                const int32_t tok = rows[m * 16 + g + 8 * r];
+                if (tok < 0) continue;
+                float *dst = a.out + (int64_t)tok * a.ldo + at;
+                const float s[4] = {y[m][r].x + d[0][2 * r], y[m][r].y + d[0][2 * r + 1], y[m][r].z + d[1][2 * r],
+                                    y[m][r].w + d[1][2 * r + 1]};
+                if (WIDE) {
+                    if (at < a.O) *reinterpret_cast<float4 *>(dst) = make_float4(s[0], s[1], s[2], s[3]);
+                } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (at + e < a.O) dst[e] = s[e];
@@ -362,15 +450,22 @@ template <int KS> __global__ void __launch_bounds__(128) expand_kernel(const __g
     }
 }
 
-template <int KS> cudaError_t launch_expand(const LoraArgs &a, dim3 grid, cudaStream_t s)
+template <int KS, bool WIDE> cudaError_t launch_expand(const LoraArgs &a, dim3 grid, cudaStream_t s)
 {
-    const size_t smem = (size_t)(kTile / 16) * KS * 2 * 32 * sizeof(uint4);
+    const size_t smem = (size_t)(kTile / 16) * KS * 3 * 32 * sizeof(uint4);
     static std::atomic<uint64_t> ready{0};
-    if (smem > 48u * 1024u) {
-        const cudaError_t e = allow_smem(expand_kernel<KS>, smem, ready);
+    if (smem > 40u * 1024u) {   // 48 KB with the kernel's static part need no permission
+        const cudaError_t e = allow_smem(expand_kernel<KS, WIDE>, smem, ready);
         if (e != cudaSuccess) return e;
     }
-    return launch_behind(expand_kernel<KS>, grid, dim3(128), smem, s, a);
+    return launch_behind(expand_kernel<KS, WIDE>, grid, dim3(128), smem, s, a);
+}
+
+template <bool WIDE> cudaError_t launch_expand_rank(const LoraArgs &a, dim3 grid, cudaStream_t s)
+{
+    const uint32_t ks = (a.R + 15) / 16;
+    return ks == 1 ? launch_expand<1, WIDE>(a, grid, s) : ks == 2 ? launch_expand<2, WIDE>(a, grid, s)
+           : ks <= 4 ? launch_expand<4, WIDE>(a, grid, s) : launch_expand<8, WIDE>(a, grid, s);
 }
 
 // Parts that in_features is cut into, so that the shrink kernel has about
@@ -475,7 +570,8 @@ hxq_error_t hxq_cuda_lora(const hxq_lora_t *adapters, const uint16_t *d_x, int64
     a.I = adapters->in_features;
     a.O = adapters->out_features;
     a.parts = lora_parts(tiles, a.R, a.I, a.span);
-    a.wide = ((ldy | ldo) & 3) == 0 && (((uintptr_t)d_y | (uintptr_t)d_out) & 15u) == 0;
+    // 16-byte accesses of y and out where every row allows them
+    const bool wide = ((ldy | ldo | a.O) & 3) == 0 && (((uintptr_t)d_y | (uintptr_t)d_out) & 15u) == 0;
     // outputs of a warp: 32 while that gives no more than four CTAs an SM, up to 128
     const uint32_t pieces = (a.O + 63) / 64, full = 4u * (uint32_t)sm_count();
     a.pairs = 2;
@@ -483,11 +579,11 @@ hxq_error_t hxq_cuda_lora(const hxq_lora_t *adapters, const uint16_t *d_x, int64
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const dim3 grid1(tiles, a.parts, (a.R + kShrinkRanks - 1) / kShrinkRanks);
     const dim3 grid2(tiles, (pieces + a.pairs - 1) / a.pairs);
-    cudaError_t e = launch_behind(shrink_kernel, grid1, dim3(128), 0, s, a);
+    static std::atomic<uint64_t> ready{0};
+    cudaError_t e = allow_smem(shrink_kernel, 4 * kShrinkRing, ready);
+    if (e == cudaSuccess) e = launch_behind(shrink_kernel, grid1, dim3(128), 4 * kShrinkRing, s, a);
     if (e == cudaSuccess) {
-        const uint32_t ks = (a.R + 15) / 16;
-        e = ks == 1 ? launch_expand<1>(a, grid2, s) : ks == 2 ? launch_expand<2>(a, grid2, s)
-            : ks <= 4 ? launch_expand<4>(a, grid2, s) : launch_expand<8>(a, grid2, s);
+        e = wide ? launch_expand_rank<true>(a, grid2, s) : launch_expand_rank<false>(a, grid2, s);
     }
     if (e != cudaSuccess) {
         cudaGetLastError();

@@ -167,7 +167,7 @@ typedef struct {
 /* x: bf16 [n_tokens] rows of in_features, ldx elements apart (a multiple of
  * 8, 16-byte aligned); y, out: fp32 rows of out_features, ldy and ldo apart;
  * out may be y.  n_requests is the B of the plan.  x A^T is summed in fp32 and
- * enters the second product as two bf16 parts (2^-17 of each value).
+ * enters the second product as three bf16 parts (together its 24 bits).
  * workspace: hxq_cuda_lora_workspace bytes, 16-byte aligned, contents don't
  * matter; calls that may overlap in time need one each. */
 size_t hxq_cuda_lora_workspace(const hxq_lora_t *adapters, uint32_t n_requests, uint32_t n_tokens);
