@@ -290,7 +290,7 @@ __device__ __forceinline__ uint2 load2(const uint16_t *p)
 // ends with four consecutive outputs of a token (16-byte accesses of y).  A
 // piece's B and y of the whole tile are loaded together, the first piece's
 // before the shrink kernel's results are waited for.
-template <int KS, bool WIDE> __global__ void __launch_bounds__(128) expand_kernel(const __grid_constant__ LoraArgs a)
+template <int KS, bool WIDE> __global__ void __launch_bounds__(128, KS == 8 ? 2 : 4) expand_kernel(const __grid_constant__ LoraArgs a)
 {
     // s h of the tile as operand fragments: [token group][k step][three parts][lane]
     extern __shared__ uint4 frag[];
@@ -344,11 +344,11 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128) expand_kerne
     }
     const uint32_t groups = (count + 15) / 16;
     const uint16_t *Bm = a.Bm + (size_t)id * a.O * a.R;
-    uint2 b[2][KS];
-    float4 y[4][2];   // [token group][token g, g + 8]
+    uint2 b[2][2][KS];
+    float4 y[2][4][2];   // two pieces: [token group][token g, g + 8]
     // loads that stay where they are written, all before the first use; a row
     // or column that does not exist reads one that does
-    auto load = [&](uint32_t o) {
+    auto load = [&](uint32_t o, uint2 (&b)[2][KS], float4 (&y)[4][2]) {
         const uint32_t at = o + q * 4;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -377,26 +377,37 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128) expand_kerne
         }
     };
     const float scale = a.scales[id];
-    if (o0 < a.O) load(o0);
+    if (o0 < a.O) load(o0, b[0], y[0]);
     wait_previous();
     for (uint32_t i = warp; i < groups * KS; i += 4) {
         const uint32_t m = i / KS, k = i % KS;
         uint32_t w3[3][4];
+        float4 sums[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+        const uint32_t c = k * 16 + q * 4, t0 = min(m * 16 + g, count - 1), t1 = min(m * 16 + g + 8, count - 1);
+        const float *h0 = a.h + (size_t)(first + t0) * a.R + min(c, a.R - 4), *h1 = a.h + (size_t)(first + t1) * a.R + min(c, a.R - 4);
+        for (uint32_t p0 = 0; p0 < a.parts; p0 += 4) {
+            float4 u[4][2];
+#pragma unroll
+            for (uint32_t p = 0; p < 4; ++p) {
+                const size_t off = (size_t)min(p0 + p, a.parts - 1) * a.T * a.R;
+                u[p][0] = load4(h0 + off);
+                u[p][1] = load4(h1 + off);
+            }
+#pragma unroll
+            for (uint32_t p = 0; p < 4; ++p)
+                if (p0 + p < a.parts)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        sums[r].x += u[p][r].x;
+                        sums[r].y += u[p][r].y;
+                        sums[r].z += u[p][r].z;
+                        sums[r].w += u[p][r].w;
+                    }
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const uint32_t t = m * 16 + g + 8 * r, c = k * 16 + q * 4;
-            float4 v = make_float4(0, 0, 0, 0);
-            if (t < count && c < a.R) {
-                const float *h = a.h + (size_t)(first + t) * a.R + c;
-#pragma unroll 4
-                for (uint32_t p = 0; p < a.parts; ++p) {
-                    const float4 u = *reinterpret_cast<const float4 *>(h + (size_t)p * a.T * a.R);
-                    v.x += u.x;
-                    v.y += u.y;
-                    v.z += u.z;
-                    v.w += u.w;
-                }
-            }
+            float4 v = sums[r];
+            if (m * 16 + g + 8 * r >= count || c >= a.R) v = make_float4(0, 0, 0, 0);
             float f[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
 #pragma unroll
             for (int part = 0; part < 3; ++part)
@@ -414,10 +425,7 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128) expand_kerne
             frag[(i * 3 + part) * 32 + lane] = make_uint4(w3[part][0], w3[part][1], w3[part][2], w3[part][3]);
     }
     __syncthreads();
-    for (uint32_t j = 0; j < a.pairs; ++j) {
-        const uint32_t o = o0 + j * 64;
-        if (o >= a.O) break;
-        if (j) load(o);
+    auto piece = [&](uint32_t o, const uint2 (&b)[2][KS], const float4 (&y)[4][2]) {
         const uint32_t at = o + q * 4;
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -447,6 +455,17 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128) expand_kerne
                 }
             }
         }
+    };
+    // the next piece is on its way while this one is multiplied
+    for (uint32_t j = 0; j < a.pairs; j += 2) {
+        const uint32_t o = o0 + j * 64;
+        if (o >= a.O) break;
+        const bool more = j + 1 < a.pairs && o + 64 < a.O;
+        if (more) load(o + 64, b[1], y[1]);
+        piece(o, b[0], y[0]);
+        if (!more) break;
+        if (j + 2 < a.pairs && o + 128 < a.O) load(o + 128, b[0], y[0]);
+        piece(o + 64, b[1], y[1]);
     }
 }
 

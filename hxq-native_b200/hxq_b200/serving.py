@@ -19,7 +19,6 @@ There is no CPU implementation.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import NamedTuple
 
@@ -67,19 +66,14 @@ def _cuda(t: torch.Tensor, name: str) -> torch.device:
     return t.device
 
 
-@contextlib.contextmanager
-def _switched(dev: torch.device):
-    with torch.cuda.device(dev):
-        yield
-
-
-def _on(dev: torch.device):
-    """The tensors' device made current, when it is not."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else _switched(dev)
-
-
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+# The current device and a device's current stream as plain numbers: the
+# wrapper objects of torch.cuda cost more than a launch.
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _stream = torch._C._cuda_getCurrentRawStream
+else:
+    def _stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
 
 
 class KvPlan(NamedTuple):
@@ -104,13 +98,18 @@ def kv_plan(new: torch.Tensor, cached: torch.Tensor, table: torch.Tensor, free: 
     B = new.numel()
     _need(cached.numel() == B and table.shape[0] == B, "new, cached and table must have one entry per request")
     _need(0 < block_tokens <= 65536 and 0 <= n_slots < 2 ** 31, "block_tokens or n_slots out of range")
-    with _on(dev):
-        buf = torch.empty(2 * B + 2 + 2 * n_slots, dtype=torch.int32, device=dev)
-        starts, lens, taken, slots, positions = buf.split((B + 1, B, 1, n_slots, n_slots))
-        check(lib().hxq_cuda_kv_plan(new.data_ptr(), cached.data_ptr(), B, table.data_ptr(), table.shape[1], block_tokens,
-                                     free.data_ptr(), free.numel(), starts.data_ptr(), lens.data_ptr(), slots.data_ptr(),
-                                     positions.data_ptr(), n_slots, taken.data_ptr(), _status(status, dev), _stream(dev)),
-              "hxq_cuda_kv_plan")
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return kv_plan(new, cached, table, free, block_tokens, n_slots, status)
+    buf = torch.empty(2 * B + 2 + 2 * n_slots, dtype=torch.int32, device=dev)
+    at = buf.data_ptr()
+    err = lib().hxq_cuda_kv_plan(new.data_ptr(), cached.data_ptr(), B, table.data_ptr(), table.shape[1], block_tokens,
+                                 free.data_ptr(), free.numel(), at, at + 4 * (B + 1), at + 4 * (2 * B + 2),
+                                 at + 4 * (2 * B + 2 + n_slots), n_slots, at + 4 * (2 * B + 1), _status(status, dev),
+                                 _stream(dev.index))
+    if err:
+        check(err, "hxq_cuda_kv_plan")
+    starts, lens, taken, slots, positions = torch.split_with_sizes(buf, (B + 1, B, 1, n_slots, n_slots))
     return KvPlan(starts, lens, slots, positions, taken)
 
 
@@ -161,10 +160,15 @@ class KvCache:
         k, v = self._rows(k, "k"), self._rows(v, "v")
         _ints(slots, "slots", self.device)
         _need(k.dtype == v.dtype and k.shape[0] == v.shape[0] == slots.numel(), "k, v and slots must go together")
-        with _on(self.device):
-            check(lib().hxq_cuda_kv_append(self._ref, k.data_ptr(), v.data_ptr(), _ELEM[k.dtype], k.stride(0), k.stride(1),
-                                           v.stride(0), v.stride(1), slots.data_ptr(), slots.numel(),
-                                           _status(status, self.device), _stream(self.device)), "hxq_cuda_kv_append")
+        dev = self.device
+        if dev.index != _current_device():
+            with torch.cuda.device(dev):
+                return self.append(k, v, slots, status)
+        err = lib().hxq_cuda_kv_append(self._ref, k.data_ptr(), v.data_ptr(), _ELEM[k.dtype], k.stride(0), k.stride(1),
+                                       v.stride(0), v.stride(1), slots.data_ptr(), slots.numel(), _status(status, dev),
+                                       _stream(dev.index))
+        if err:
+            check(err, "hxq_cuda_kv_append")
 
     def read(self, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
              status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -172,10 +176,15 @@ class KvCache:
         zeros at negative slots."""
         _ints(slots, "slots", self.device)
         _need(dtype in _ELEM, "dtype must be fp32, bf16 or f16")
-        with _on(self.device):
-            k, v = (torch.empty((slots.numel(), self.n_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
-            check(lib().hxq_cuda_kv_read(self._ref, slots.data_ptr(), slots.numel(), k.data_ptr(), v.data_ptr(), _ELEM[dtype],
-                                         _status(status, self.device), _stream(self.device)), "hxq_cuda_kv_read")
+        dev = self.device
+        if dev.index != _current_device():
+            with torch.cuda.device(dev):
+                return self.read(slots, dtype, status)
+        k, v = torch.empty((2, slots.numel(), self.n_heads, self.head_dim), dtype=dtype, device=dev).unbind()
+        err = lib().hxq_cuda_kv_read(self._ref, slots.data_ptr(), slots.numel(), k.data_ptr(), v.data_ptr(), _ELEM[dtype],
+                                     _status(status, dev), _stream(dev.index))
+        if err:
+            check(err, "hxq_cuda_kv_read")
         return k, v
 
     def attention(self, q: torch.Tensor, starts: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, max_new: int,
@@ -202,29 +211,43 @@ class KvCache:
         _need(window >= 0 and (causal or not window), "a window needs causal attention")
         _need(lse is None or (lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == tuple(q.shape[:2])
                               and lse.device == dev), "lse must be fp32 [rows, heads]")
-        with _on(dev):
-            if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-            else:
-                _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.stride(2) == 1,
-                      "out must be like q")
-            p = KvAttention(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), q.stride(0), q.stride(1),
-                            out.stride(0), out.stride(1), starts.data_ptr(), lens.data_ptr(), table.data_ptr(), B, T,
-                            q.shape[1], table.shape[1], max_new, window, self.head_dim ** -0.5 if scale is None else scale,
-                            _ELEM[q.dtype], 1 if causal else 0)
-            L, ref = lib(), C.byref(p)
-            size = L.hxq_cuda_kv_attention_workspace(self._ref, ref)
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            check(L.hxq_cuda_kv_attention(self._ref, ref, ws.data_ptr(), size, _status(status, dev), _stream(dev)),
-                  "hxq_cuda_kv_attention")
+        if dev.index != _current_device():
+            with torch.cuda.device(dev):
+                return self.attention(q, starts, lens, table, max_new, scale, window, causal, out, lse, status)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        else:
+            _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.stride(2) == 1,
+                  "out must be like q")
+        p = KvAttention(q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), q.stride(0), q.stride(1),
+                        out.stride(0), out.stride(1), starts.data_ptr(), lens.data_ptr(), table.data_ptr(), B, T,
+                        q.shape[1], table.shape[1], max_new, window, self.head_dim ** -0.5 if scale is None else scale,
+                        _ELEM[q.dtype], 1 if causal else 0)
+        L, ref = lib(), C.byref(p)
+        size = L.hxq_cuda_kv_attention_workspace(self._ref, ref)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        err = L.hxq_cuda_kv_attention(self._ref, ref, ws.data_ptr(), size, _status(status, dev), _stream(dev.index))
+        if err:
+            check(err, "hxq_cuda_kv_attention")
         return out
 
 
 class LoraPlan(NamedTuple):
-    order: torch.Tensor    # [n_tokens] token rows sorted by adapter
-    tiles: torch.Tensor    # [tiles, 4] adapter, first, count, 0
+    buf: torch.Tensor      # tiles, then the order
+    n_tiles: int
+    n_tokens: int
     n_requests: int
     n_adapters: int
+
+    @property
+    def tiles(self) -> torch.Tensor:
+        """[n_tiles, 4]: adapter (-1: none), first place in order, tokens, 0."""
+        return self.buf[:4 * self.n_tiles].view(-1, 4)
+
+    @property
+    def order(self) -> torch.Tensor:
+        """[n_tokens] token rows sorted by adapter."""
+        return self.buf[4 * self.n_tiles:]
 
 
 def lora_plan(starts: torch.Tensor, adapters: torch.Tensor, n_adapters: int, n_tokens: int,
@@ -237,13 +260,18 @@ def lora_plan(starts: torch.Tensor, adapters: torch.Tensor, n_adapters: int, n_t
     B = adapters.numel()
     _need(starts.numel() == B + 1, "starts must have one entry more than adapters")
     _need(0 < n_adapters <= 4096 and 0 <= n_tokens < 2 ** 31, "n_adapters or n_tokens out of range")
+    if dev.index != _current_device():
+        with torch.cuda.device(dev):
+            return lora_plan(starts, adapters, n_adapters, n_tokens, status)
     L = lib()
-    with _on(dev):
-        tiles = torch.empty((L.hxq_lora_tiles(B, n_adapters, n_tokens), 4), dtype=torch.int32, device=dev)
-        order = torch.empty(n_tokens, dtype=torch.int32, device=dev)
-        check(L.hxq_cuda_lora_plan(starts.data_ptr(), adapters.data_ptr(), B, n_adapters, n_tokens, order.data_ptr(),
-                                   tiles.data_ptr(), _status(status, dev), _stream(dev)), "hxq_cuda_lora_plan")
-    return LoraPlan(order, tiles, B, n_adapters)
+    n_tiles = L.hxq_lora_tiles(B, n_adapters, n_tokens)
+    buf = torch.empty(4 * n_tiles + n_tokens, dtype=torch.int32, device=dev)
+    at = buf.data_ptr()
+    err = L.hxq_cuda_lora_plan(starts.data_ptr(), adapters.data_ptr(), B, n_adapters, n_tokens, at + 16 * n_tiles, at,
+                               _status(status, dev), _stream(dev.index))
+    if err:
+        check(err, "hxq_cuda_lora_plan")
+    return LoraPlan(buf, n_tiles, n_tokens, B, n_adapters)
 
 
 class LoraAdapters:
@@ -280,23 +308,26 @@ class LoraAdapters:
         T = x.shape[0]
         _need(y.device == dev and y.dtype == torch.float32 and tuple(y.shape) == (T, self.out_features),
               f"y must be fp32 [tokens, {self.out_features}] on {dev}")
-        _need(plan.n_adapters == self.n_adapters and plan.order.numel() == T and plan.order.device == dev,
+        _need(plan.n_adapters == self.n_adapters and plan.n_tokens == T and plan.buf.device == dev,
               "the plan was made for other adapters or tokens")
         if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
             x = x.clone(memory_format=torch.contiguous_format)
         if y.stride(1) != 1:
             _need(out is not y, "y must have consecutive elements to be written in place")
             y = y.contiguous()
+        if dev.index != _current_device():
+            with torch.cuda.device(dev):
+                return self.add(y, x, plan, out)
+        if out is None:
+            out = torch.empty((T, self.out_features), dtype=torch.float32, device=dev)
+        else:
+            _need(out.device == dev and out.dtype == torch.float32 and out.shape == y.shape and out.stride(1) == 1,
+                  "out must be like y")
         L = lib()
-        with _on(dev):
-            if out is None:
-                out = torch.empty((T, self.out_features), dtype=torch.float32, device=dev)
-            else:
-                _need(out.device == dev and out.dtype == torch.float32 and out.shape == y.shape and out.stride(1) == 1,
-                      "out must be like y")
-            size = L.hxq_cuda_lora_workspace(self._ref, plan.n_requests, T)
-            ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            check(L.hxq_cuda_lora(self._ref, x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(),
-                                  out.stride(0), plan.n_requests, T, plan.order.data_ptr(), plan.tiles.data_ptr(),
-                                  ws.data_ptr(), size, _stream(dev)), "hxq_cuda_lora")
+        size = L.hxq_cuda_lora_workspace(self._ref, plan.n_requests, T)
+        ws, at = torch.empty(size, dtype=torch.uint8, device=dev), plan.buf.data_ptr()
+        err = L.hxq_cuda_lora(self._ref, x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0),
+                              plan.n_requests, T, at + 16 * plan.n_tiles, at, ws.data_ptr(), size, _stream(dev.index))
+        if err:
+            check(err, "hxq_cuda_lora")
         return out
