@@ -139,7 +139,7 @@ struct LoraArgs {
     const hxq_lora_tile_t *tiles;
     int64_t ldx, ldy, ldo;
     uint32_t T, n, R, I, O, parts, span;   // span: in_features of a part, a multiple of 128
-    uint32_t pairs;                        // expand: 16-output pieces a warp takes
+    uint32_t pairs;                        // expand: pieces of 64 outputs a CTA takes
 };
 
 // A tile's positions come from device memory that the caller could have
@@ -285,6 +285,13 @@ __device__ __forceinline__ uint2 load2(const uint16_t *p)
     return v;
 }
 
+__device__ __forceinline__ uint4 load_b(const uint16_t *p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // out = y + (s h) B^T: 16 tokens x 16 outputs at a time.  The two 8-output
 // products of a piece take outputs {0,1,4,5,8,..} and {2,3,6,7,..}, so a lane
 // ends with four consecutive outputs of a token (16-byte accesses of y).  A
@@ -369,10 +376,18 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128, KS == 8 ? 2 
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const uint32_t col = min(o + (g >> 1) * 4 + (g & 1) + 2 * w, a.O - 1);
+            if (KS == 1) {
+                b[w][0] = make_uint2(0, 0);
+                if (q * 4 < a.R) b[w][0] = load2(Bm + (size_t)col * a.R + q * 4);
+            } else {
+                // 8 ranks a lane: two steps' operands
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                b[w][k] = make_uint2(0, 0);
-                if (k * 16 + q * 4 < a.R) b[w][k] = load2(Bm + (size_t)col * a.R + k * 16 + q * 4);
+                for (int k = 0; k < KS; k += 2) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (k * 16 + q * 8 < a.R) v = load_b(Bm + (size_t)col * a.R + k * 16 + q * 8);
+                    b[w][k] = make_uint2(v.x, v.y);
+                    b[w][(k + 1) % KS] = make_uint2(v.z, v.w);
+                }
             }
         }
     };
@@ -383,7 +398,7 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128, KS == 8 ? 2 
         const uint32_t m = i / KS, k = i % KS;
         uint32_t w3[3][4];
         float4 sums[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
-        const uint32_t c = k * 16 + q * 4, t0 = min(m * 16 + g, count - 1), t1 = min(m * 16 + g + 8, count - 1);
+        const uint32_t c = KS == 1 ? q * 4 : (k >> 1) * 32 + q * 8 + (k & 1) * 4, t0 = min(m * 16 + g, count - 1), t1 = min(m * 16 + g + 8, count - 1);
         const float *h0 = a.h + (size_t)(first + t0) * a.R + min(c, a.R - 4), *h1 = a.h + (size_t)(first + t1) * a.R + min(c, a.R - 4);
         for (uint32_t p0 = 0; p0 < a.parts; p0 += 4) {
             float4 u[4][2];
@@ -487,7 +502,7 @@ template <bool WIDE> cudaError_t launch_expand_rank(const LoraArgs &a, dim3 grid
            : ks <= 4 ? launch_expand<4, WIDE>(a, grid, s) : launch_expand<8, WIDE>(a, grid, s);
 }
 
-// Parts that in_features is cut into, so that the shrink kernel has about
+// Parts that in_features is cut into, so that the shrink kernel has at least
 // two CTAs for every SM; a part has at least 256 features.
 uint32_t lora_parts(uint32_t tiles, uint32_t R, uint32_t I, uint32_t &span)
 {
@@ -591,7 +606,9 @@ hxq_error_t hxq_cuda_lora(const hxq_lora_t *adapters, const uint16_t *d_x, int64
     a.parts = lora_parts(tiles, a.R, a.I, a.span);
     // 16-byte accesses of y and out where every row allows them
     const bool wide = ((ldy | ldo | a.O) & 3) == 0 && (((uintptr_t)d_y | (uintptr_t)d_out) & 15u) == 0;
-    // outputs of a warp: 32 while that gives no more than four CTAs an SM, up to 128
+    // pieces of 64 outputs a CTA takes: 2 while that gives no more than four
+    // CTAs an SM, up to 8 (tiles differ in length: some more CTAs than fit at
+    // once even that out; one full wave of longer CTAs took a fifth more)
     const uint32_t pieces = (a.O + 63) / 64, full = 4u * (uint32_t)sm_count();
     a.pairs = 2;
     while (a.pairs < 8 && (uint64_t)tiles * ((pieces + a.pairs - 1) / a.pairs) > full) a.pairs *= 2;
