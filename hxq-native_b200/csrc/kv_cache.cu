@@ -133,10 +133,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
 
 // ---------------------------------------------------------------------------
 // Append.  The unit of work is one (run, head, k or v): a run is the rows of
-// one block that follow each other in the call.  A warp finds the largest
-// magnitude of the run, merges it with the block's scale, writes the run's
-// codes and, when the scale grew, rounds the block's other codes to the new
-// one.  Bound by the bytes of the rows (the second look at a run hits L1/L2).
+// one block that follow each other in the call.  G warps find the largest
+// magnitude of the run, merge it with the block's scale, write the run's codes
+// and, when the scale grew, round the block's other codes to the new one.  A
+// lane keeps up to 8 pieces of 8 values between the two looks at a run, G
+// chosen so that a whole block's rows fit (blocks beyond 8 warps' worth are
+// read again, out of L2).  Bound by the bytes of the rows.
 //
 // Magnitudes are compared as the integers of their bits (non-negative floats
 // order like integers, NaN above all), so infinities and NaN reach the scale.
@@ -156,21 +158,60 @@ struct AppendArgs {
     uint32_t n_tokens, n_heads, P, D, n_blocks, window;
 };
 
-template <typename T, int VEC> struct Pack { T v[VEC]; };
+template <typename T> struct Piece {   // 8 values as they are in memory
+    static constexpr int kWords = sizeof(T) * 8 / 16;
+    uint4 raw[kWords];
+};
 
-template <typename T, int VEC> __device__ __forceinline__ void load_row(float (&f)[8], const T *p)
+// 16-byte loads where VEC, else one by one.
+template <typename T, bool VEC> __device__ __forceinline__ Piece<T> load_piece(const T *p)
 {
-    if (VEC == 8) {
-        constexpr int W = sizeof(T) * 8 / 16;
-        uint4 raw[W];
+    Piece<T> v;
+    if (VEC) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) raw[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-        const T *e = reinterpret_cast<const T *>(raw);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to(e[i]);
+        for (int i = 0; i < Piece<T>::kWords; ++i) v.raw[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to(p[i]);
+        for (int i = 0; i < Piece<T>::kWords; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (sizeof(T) == 4) w[u] = reinterpret_cast<const uint32_t *>(p)[i * 4 + u];
+                else {
+                    const uint16_t *e = reinterpret_cast<const uint16_t *>(p) + 2 * u;
+                    w[u] = e[0] | (uint32_t)e[1] << 16;
+                }
+            }
+            v.raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    return v;
+}
+
+__device__ __forceinline__ float2 pair_of(uint32_t w, const float *) { return make_float2(__uint_as_float(w), 0.0f); }
+__device__ __forceinline__ float2 pair_of(uint32_t w, const __nv_bfloat16 *)
+{
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 pair_of(uint32_t w, const __half *)
+{
+    return __half22float2(__halves2half2(__ushort_as_half((uint16_t)w), __ushort_as_half((uint16_t)(w >> 16))));
+}
+
+template <typename T> __device__ __forceinline__ void values(const Piece<T> &v, float (&f)[8])
+{
+#pragma unroll
+    for (int i = 0; i < Piece<T>::kWords; ++i) {
+        const uint32_t w[4] = {v.raw[i].x, v.raw[i].y, v.raw[i].z, v.raw[i].w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float2 p = pair_of(w[u], static_cast<const T *>(nullptr));
+            if (sizeof(T) == 4) f[(i * 4 + u) & 7] = p.x;
+            else {
+                f[(2 * u) & 7] = p.x;
+                f[(2 * u + 1) & 7] = p.y;
+            }
+        }
     }
 }
 
@@ -199,18 +240,25 @@ template <int FMT> __device__ __forceinline__ uint2 pack_codes(const float (&f)[
     return r;
 }
 
-template <typename T, int FMT, int VEC>
-__global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendArgs a)
+constexpr int kHeld = 8;   // pieces a lane keeps
+
+template <typename T, int FMT, bool VEC, int G>
+__global__ void __launch_bounds__(kAppendWarps * 32, sizeof(T) == 4 ? 2 : 3) append_kernel(const AppendArgs a)
 {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t item = blockIdx.y * kAppendWarps + warp;   // (head, k or v)
-    if (item >= a.n_heads * 2) return;
-    const uint32_t kv = item & 1, h = item >> 1;
-    const T *x = static_cast<const T *>(a.x[kv]) + (int64_t)h * a.sh[kv];
-    const int64_t st = a.st[kv];
+    __shared__ uint32_t tops[2][kAppendWarps];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wg = warp % G;
+    // CTAs of the same rows follow each other, so that whole rows of the call
+    // are under way at once
+    const uint32_t groups = (a.n_heads * 2 + kAppendWarps / G - 1) / (kAppendWarps / G), window = blockIdx.x / groups;
+    const uint32_t item = (blockIdx.x - window * groups) * (kAppendWarps / G) + warp / G;   // (head, k or v)
+    const bool mine_too = item < a.n_heads * 2;                         // the CTA's warps stay together
+    const uint32_t kv = item & 1, h = mine_too ? item >> 1 : 0;
+    const T *x = static_cast<const T *>(kv ? a.x[1] : a.x[0]) + (int64_t)h * (kv ? a.sh[1] : a.sh[0]);
+    const int64_t st = kv ? a.st[1] : a.st[0];
     const uint32_t n_slots = a.n_blocks * a.P, lg = a.D == 64 ? 3 : a.D == 128 ? 4 : 5;   // 8-value pieces a row
     const float qmax = FMT == HXQ_KV_INT8 ? 127.0f : 448.0f;
-    const uint32_t t_begin = blockIdx.x * a.window, t_end = min(t_begin + a.window, a.n_tokens);
+    const uint32_t t_begin = window * a.window, t_end = min(t_begin + a.window, a.n_tokens);
+    uint32_t turn = 0;
     for (uint32_t t0 = t_begin; t0 < t_end; t0 += 32) {
         // which rows of the window begin a run
         const uint32_t tl = t0 + lane;
@@ -219,11 +267,11 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendA
             const int32_t s = a.slots[tl], before = tl ? a.slots[tl - 1] : -1;
             if (s >= 0) {
                 if ((uint32_t)s >= n_slots) {
-                    if (item == 0) flag(a.status, HXQ_SERVING_BAD_BLOCK);
+                    if (item == 0 && wg == 0) flag(a.status, HXQ_SERVING_BAD_BLOCK);
                 } else {
                     const bool same = before >= 0 && (uint32_t)before / a.P == (uint32_t)s / a.P;
                     lead = !same || before >= s;
-                    if (same && before >= s && item == 0) flag(a.status, HXQ_SERVING_ORDER);
+                    if (same && before >= s && item == 0 && wg == 0) flag(a.status, HXQ_SERVING_ORDER);
                 }
             }
         }
@@ -231,7 +279,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendA
         while (leads) {
             const uint32_t t = t0 + __ffs(leads) - 1;
             leads &= leads - 1;
-            const uint32_t s0 = (uint32_t)a.slots[t], block = s0 / a.P, pos0 = s0 % a.P;
+            const uint32_t s0 = (uint32_t)a.slots[t], block = s0 / a.P, pos0 = s0 - block * a.P;
+            float *scale_at = (kv ? a.scales[1] : a.scales[0]) + (size_t)block * a.n_heads + h;
+            const float old = pos0 == 0 ? 0.0f : *scale_at;
             // length of the run (at most P rows) and the block's positions it writes
             uint32_t len = 0, mine[8] = {0, 0, 0, 0, 0, 0, 0, 0};
             for (bool more = true; more;) {
@@ -245,44 +295,64 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendA
                 }
                 const uint32_t yes = __ballot_sync(~0u, in), n = yes == ~0u ? 32u : (uint32_t)__ffs(~yes) - 1;
                 if (lane >= n) in = false;
+                if (pos0 != 0) {   // needed where codes are rounded again
 #pragma unroll
-                for (int w = 0; w < 8; ++w)
-                    mine[w] |= __reduce_or_sync(~0u, in && (p >> 5) == (uint32_t)w ? 1u << (p & 31) : 0u);
+                    for (int w = 0; w < 8; ++w)
+                        mine[w] |= __reduce_or_sync(~0u, in && (p >> 5) == (uint32_t)w ? 1u << (p & 31) : 0u);
+                }
                 len += n;
                 more = n == 32;
             }
             // largest magnitude of the run
-            const uint32_t pieces = len << lg;
+            const uint32_t pieces = len << lg, e0 = wg * 32 + lane;
+            auto row_at = [&](uint32_t e) { return x + (int64_t)(t + (e >> lg)) * st + (e & ((1u << lg) - 1)) * 8; };
+            Piece<T> held[kHeld];
             uint32_t top = 0;
-#pragma unroll 4
-            for (uint32_t e = lane; e < pieces; e += 32) {
+            auto look = [&](const Piece<T> &v) {
                 float f[8];
-                load_row<T, VEC>(f, x + (int64_t)(t + (e >> lg)) * st + (e & ((1u << lg) - 1)) * 8);
+                values(v, f);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-            }
+            };
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (e0 + i * (32 * G) < pieces) held[i] = load_piece<T, VEC>(row_at(e0 + i * (32 * G)));
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (e0 + i * (32 * G) < pieces) look(held[i]);
+            for (uint32_t e = e0 + kHeld * (32 * G); e < pieces; e += 32 * G) look(load_piece<T, VEC>(row_at(e)));
             top = __reduce_max_sync(~0u, top);
-            float *scale_at = a.scales[kv] + (size_t)block * a.n_heads + h;
-            const float old = pos0 == 0 ? 0.0f : *scale_at;
+            if (G > 1) {
+                if (lane == 0) tops[turn][warp] = top;
+                __syncthreads();   // a lead is every warp's of the CTA: the slots are the same
+#pragma unroll
+                for (int w = 0; w < G; ++w) top = max(top, tops[turn][warp - wg + w]);
+                turn ^= 1u;
+            }
             float scale = __uint_as_float(max(__float_as_uint(old) & 0x7fffffffu, __float_as_uint(__uint_as_float(top) / qmax)));
             if (scale < 1.17549435e-38f) scale = 0.0f;
             const float inv = scale > 0.0f ? 1.0f / scale : 0.0f;
             const bool lost = !(scale <= 3.402823466e38f);   // infinite or NaN: the codes are 0, so that no code is NaN
-            uint8_t *codes = a.codes[kv] + ((size_t)block * a.n_heads + h) * a.P * a.D;
+            uint8_t *codes = (kv ? a.codes[1] : a.codes[0]) + ((size_t)block * a.n_heads + h) * a.P * a.D;
             const bool grew = pos0 != 0 && !(scale <= old);
-            __syncwarp();
-            if (lane == 0) *scale_at = scale;
-#pragma unroll 4
-            for (uint32_t e = lane; e < pieces; e += 32) {
-                const uint32_t u = t + (e >> lg), col = (e & ((1u << lg) - 1)) * 8;
+            if (!mine_too) continue;
+            const bool dense = (uint32_t)a.slots[t + len - 1] - s0 == len - 1;   // ascending: no gaps
+            auto put = [&](uint32_t e, const Piece<T> &v) {
                 float f[8];
-                load_row<T, VEC>(f, x + (int64_t)u * st + col);
-                *reinterpret_cast<uint2 *>(codes + (size_t)((uint32_t)a.slots[u] % a.P) * a.D + col) =
+                values(v, f);
+                const uint32_t at = dense ? pos0 + (e >> lg) : (uint32_t)a.slots[t + (e >> lg)] - block * a.P;
+                *reinterpret_cast<uint2 *>(codes + (size_t)at * a.D + (e & ((1u << lg) - 1)) * 8) =
                     lost ? make_uint2(0u, 0u) : pack_codes<FMT>(f, inv);
-            }
+            };
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i)
+                if (e0 + i * (32 * G) < pieces) put(e0 + i * (32 * G), held[i]);
+            for (uint32_t e = e0 + kHeld * (32 * G); e < pieces; e += 32 * G) put(e, load_piece<T, VEC>(row_at(e)));
+            __syncwarp();   // (G > 1: the barrier above) the old scale is read
+            if (lane == 0 && wg == 0) *scale_at = scale;
             if (grew) {
                 const float ratio = scale > 0.0f ? old / scale : 0.0f;
-                for (uint32_t e = lane; e < a.P << lg; e += 32) {
+                for (uint32_t e = e0; e < a.P << lg; e += 32 * G) {
                     const uint32_t p = e >> lg;
                     uint32_t word = 0;
 #pragma unroll
@@ -300,51 +370,73 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(const AppendA
     }
 }
 
-// Read-back: one thread per 8 values of k and of v.
+// Read-back: a thread takes 16 consecutive codes of k or v, a CTA whole
+// tokens, four of a thread's pieces under way.
 template <typename T, int FMT>
-__global__ void read_kernel(const hxq_kv_cache_t c, const int32_t *slots, uint32_t n_tokens, T *k, T *v, uint32_t *status)
+__global__ void __launch_bounds__(256) read_kernel(const hxq_kv_cache_t c, const int32_t *slots, uint32_t n_tokens, T *k, T *v, uint32_t *status)
 {
-    const uint32_t lg = c.head_dim == 64 ? 3 : c.head_dim == 128 ? 4 : 5, per = c.n_heads << lg;
-    const uint64_t n = (uint64_t)n_tokens * per, step = (uint64_t)gridDim.x * blockDim.x;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        const uint32_t t = (uint32_t)(i / per), r = (uint32_t)(i - (uint64_t)t * per), h = r >> lg, col = (r & ((1u << lg) - 1)) * 8;
-        const int32_t s = slots[t];
-        const bool ok = s >= 0 && (uint32_t)s < c.n_blocks * c.block_tokens;
-        if (s >= 0 && !ok && r == 0) flag(status, HXQ_SERVING_BAD_BLOCK);
-        const uint32_t block = ok ? (uint32_t)s / c.block_tokens : 0, pos = ok ? (uint32_t)s % c.block_tokens : 0;
-        const size_t bh = (size_t)block * c.n_heads + h, at = (bh * c.block_tokens + pos) * c.head_dim + col;
+    const uint32_t lg = c.head_dim == 64 ? 2 : c.head_dim == 128 ? 3 : 4, per = c.n_heads << lg;   // pieces of a token
+    const uint32_t side = per < 256 ? 256 / per : 1, mine = threadIdx.x / per;                      // tokens side by side
+    T *out = blockIdx.y ? v : k;
+    if (!out || (per < 256 && mine >= side)) return;
+    const uint8_t *codes = static_cast<const uint8_t *>(blockIdx.y ? c.v : c.k);
+    const float *scales = blockIdx.y ? c.v_scales : c.k_scales;
+    const uint32_t n_slots = c.n_blocks * c.block_tokens, step = gridDim.x * side;
+    const bool wide = ((uintptr_t)out & 15u) == 0;
+    for (uint32_t r = per < 256 ? threadIdx.x - mine * per : threadIdx.x; r < per; r += 256) {
+        const uint32_t h = r >> lg, col = (r & ((1u << lg) - 1)) * 16;
+        for (uint64_t t0 = (uint64_t)blockIdx.x * side + (per < 256 ? mine : 0); t0 < n_tokens; t0 += 4ull * step) {
+            uint4 raw[4];
+            float scale[4];
+            bool ok[4];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-            T *out = w ? v : k;
-            if (!out) continue;
-            T o[8];
-            if (ok) {
-                const uint2 raw = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(w ? c.v : c.k) + at));
-                const float scale = (w ? c.v_scales : c.k_scales)[bh];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    o[j] = Elem<T>::from(code_value<FMT>((uint8_t)((j < 4 ? raw.x : raw.y) >> (8 * (j & 3)))) * scale);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = Elem<T>::from(0.0f);
+            for (int u = 0; u < 4; ++u) {
+                const uint64_t t = t0 + (uint64_t)u * step;
+                const int32_t s = t < n_tokens ? __ldg(slots + t) : -1;
+                ok[u] = s >= 0 && (uint32_t)s < n_slots;
+                if (s >= 0 && !ok[u] && r == 0) flag(status, HXQ_SERVING_BAD_BLOCK);
+                const uint32_t block = ok[u] ? (uint32_t)s / c.block_tokens : 0, pos = ok[u] ? (uint32_t)s - block * c.block_tokens : 0;
+                const size_t bh = (size_t)block * c.n_heads + h;
+                raw[u] = make_uint4(0, 0, 0, 0);
+                scale[u] = 0.0f;
+                if (ok[u]) {
+                    raw[u] = __ldg(reinterpret_cast<const uint4 *>(codes + (bh * c.block_tokens + pos) * c.head_dim + col));
+                    scale[u] = __ldg(scales + bh);
+                }
             }
-            T *dst = out + ((size_t)t * c.n_heads + h) * c.head_dim + col;
-            if ((((uintptr_t)out) & 15u) == 0) {
 #pragma unroll
-                for (int j = 0; j < (int)sizeof(T) / 2; ++j)
-                    reinterpret_cast<uint4 *>(dst)[j] = reinterpret_cast<const uint4 *>(o)[j];
-            } else {
+            for (int u = 0; u < 4; ++u) {
+                const uint64_t t = t0 + (uint64_t)u * step;
+                if (t >= n_tokens) break;
+                const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+                __align__(16) T o[16];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) dst[j] = o[j];
+                for (int j = 0; j < 16; ++j)
+                    o[j] = Elem<T>::from(ok[u] ? code_value<FMT>((uint8_t)(w[j >> 2] >> (8 * (j & 3)))) * scale[u] : 0.0f);
+                T *dst = out + (t * c.n_heads + h) * c.head_dim + col;
+                if (wide) {
+#pragma unroll
+                    for (int j = 0; j < (int)sizeof(T); ++j) reinterpret_cast<uint4 *>(dst)[j] = reinterpret_cast<const uint4 *>(o)[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) dst[j] = o[j];
+                }
             }
         }
     }
 }
 
-template <typename T, int FMT> void launch_append(const AppendArgs &a, bool vec, dim3 grid, cudaStream_t s)
+// Warps of a run: a block's rows in kHeld pieces a lane.
+template <typename T, int FMT> void launch_append(const AppendArgs &a, bool vec, uint32_t windows, cudaStream_t s)
 {
-    if (vec) append_kernel<T, FMT, 8><<<grid, kAppendWarps * 32, 0, s>>>(a);
-    else append_kernel<T, FMT, 1><<<grid, kAppendWarps * 32, 0, s>>>(a);
+    const uint32_t need = a.P * a.D / (8 * 32 * kHeld), g = !vec || need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
+    const uint32_t grid = windows * ((a.n_heads * 2 + kAppendWarps / g - 1) / (kAppendWarps / g));
+    constexpr int N = kAppendWarps * 32;
+    if (!vec) append_kernel<T, FMT, false, 1><<<grid, N, 0, s>>>(a);
+    else if (g == 1) append_kernel<T, FMT, true, 1><<<grid, N, 0, s>>>(a);
+    else if (g == 2) append_kernel<T, FMT, true, 2><<<grid, N, 0, s>>>(a);
+    else if (g == 4) append_kernel<T, FMT, true, 4><<<grid, N, 0, s>>>(a);
+    else append_kernel<T, FMT, true, 8><<<grid, N, 0, s>>>(a);
 }
 
 }  // namespace serving
@@ -414,16 +506,17 @@ hxq_error_t hxq_cuda_kv_append(const hxq_kv_cache_t *cache, const void *d_k, con
     // its own), up to 64 when there are enough to fill the GPU all the same
     const uint64_t fill = (uint64_t)n_tokens * cache->n_heads * 2 / ((uint64_t)sm_count() * 32);
     a.window = (uint32_t)(fill < 1 ? 1 : fill > 64 ? 64 : fill);
-    const dim3 grid((n_tokens + a.window - 1) / a.window, (cache->n_heads * 2 + kAppendWarps - 1) / kAppendWarps);
+    const uint32_t windows = (n_tokens + a.window - 1) / a.window;
+    if ((uint64_t)windows * cache->n_heads * 2 > 0x7fffffffu) return HXQ_ERR_INVALID_ARG;
     // 16-byte loads where every row begins on a 16-byte boundary
     const uint64_t s = (uint64_t)(k_stride_t | k_stride_h | v_stride_t | v_stride_h) * size;
     const bool vec = ((s | (uintptr_t)d_k | (uintptr_t)d_v) & 15u) == 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool i8 = cache->format == HXQ_KV_INT8;
-    if (elem == HXQ_ELEM_F32) i8 ? launch_append<float, HXQ_KV_INT8>(a, vec, grid, st) : launch_append<float, HXQ_KV_E4M3>(a, vec, grid, st);
+    if (elem == HXQ_ELEM_F32) i8 ? launch_append<float, HXQ_KV_INT8>(a, vec, windows, st) : launch_append<float, HXQ_KV_E4M3>(a, vec, windows, st);
     else if (elem == HXQ_ELEM_BF16)
-        i8 ? launch_append<__nv_bfloat16, HXQ_KV_INT8>(a, vec, grid, st) : launch_append<__nv_bfloat16, HXQ_KV_E4M3>(a, vec, grid, st);
-    else i8 ? launch_append<__half, HXQ_KV_INT8>(a, vec, grid, st) : launch_append<__half, HXQ_KV_E4M3>(a, vec, grid, st);
+        i8 ? launch_append<__nv_bfloat16, HXQ_KV_INT8>(a, vec, windows, st) : launch_append<__nv_bfloat16, HXQ_KV_E4M3>(a, vec, windows, st);
+    else i8 ? launch_append<__half, HXQ_KV_INT8>(a, vec, windows, st) : launch_append<__half, HXQ_KV_E4M3>(a, vec, windows, st);
     return launched();
 }
 
@@ -438,9 +531,9 @@ hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots
     if (!d_slots || (!d_k && !d_v)) return HXQ_ERR_NULL_PTR;
     const uintptr_t size = elem == HXQ_ELEM_F32 ? 4 : 2;
     if (((uintptr_t)d_k | (uintptr_t)d_v) & (size - 1)) return HXQ_ERR_INVALID_ARG;
-    const uint64_t n = (uint64_t)n_tokens * cache->n_heads * (cache->head_dim / 8), want = (n + 255) / 256;
-    const uint64_t most = (uint64_t)sm_count() * 16;
-    const unsigned grid = (unsigned)(want < most ? want : most);
+    const uint32_t per = cache->n_heads * (cache->head_dim / 16), side = per < 256 ? 256 / per : 1;
+    const uint32_t want = (n_tokens + side - 1) / side, most = (uint32_t)sm_count() * 4;
+    const dim3 grid(want < most ? want : most, 2);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool i8 = cache->format == HXQ_KV_INT8;
 #define HXQ_READ(T)                                                                                                  \
