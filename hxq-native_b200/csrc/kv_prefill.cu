@@ -42,7 +42,7 @@ constexpr int kSoftWarps = 16, kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps, kLoadWarp = kMmaWarp + 1, kPlanWarp = kMmaWarp + 2;
 constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups; the last warp has nothing to do
 // Registers: launched with 80 a thread, 61,440 in all; the rows' threads hold
-// 32 scores at a time. 512 x 88 + 128 x 64 + 128 x 64 = 61,440.
+// 16 scores and the next 16. 512 x 88 + 128 x 64 + 128 x 64 = 61,440.
 constexpr int kRegsSoft = 88, kRegsConv = 64, kRegsRest = 64;
 constexpr int kThreadsT = kWarpsT * 32;
 constexpr int kScaleSlots = 4, kSegSlots = 2;
@@ -68,23 +68,34 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr)
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+// The products' warp runs as one, so that descriptors stay in uniform
+// registers; `one` is true in the lane that issues.
+__device__ __forceinline__ void tc_mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
                  : "memory");
 }
 
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+__device__ __forceinline__ void tc_mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
                  : "memory");
 }
 
-__device__ __forceinline__ void tc_commit(uint64_t *bar)
+__device__ __forceinline__ void tc_commit(uint32_t one, uint64_t *bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(pipe::smem_u32(bar)) : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(pipe::smem_u32(bar)), "r"(one)
+                 : "memory");
+}
+
+__device__ __forceinline__ uint32_t elect_one()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r));
+    return r;
 }
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -676,7 +687,8 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 pipe::mbar_arrive(&bars->seg_full[si % kSegSlots]);
                 if (!more) break;
             }
-        } else if (warp == kMmaWarp && lane == 0) {
+        } else if (warp == kMmaWarp) {
+        const uint32_t one = elect_one();
         // ------------------------------------------------------- products
         uint32_t it = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
         // descriptors address 16-byte units
@@ -685,48 +697,49 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             const uint64_t qa = q_desc + t * (G::kQ >> 4), kb = k_desc + st * (G::kK >> 4);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
-                tc_mma_ss(tmem + t * 128u, qa + ((kk >> 2) * (kTile * 8) + (kk & 3) * 2), kb + ((kk >> 2) * (kKeys * 8) + (kk & 3) * 2),
+                tc_mma_ss(one, tmem + t * 128u, qa + ((kk >> 2) * (kTile * 8) + (kk & 3) * 2), kb + ((kk >> 2) * (kKeys * 8) + (kk & 3) * 2),
                           G::kIdescQK, kk != 0);
-            tc_commit(&bars->s_full[t]);
+            tc_commit(one, &bars->s_full[t]);
         };
         for (uint32_t si = 0; ok; ++si) {
-            ok = wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u);
+            ok = __all_sync(~0u, wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u));
             if (!ok) break;
             const uint32_t take = segs[si % kSegSlots].take, take0 = segs[si % kSegSlots].take0;
             const uint32_t tiles = segs[si % kSegSlots].r1 - segs[si % kSegSlots].r0 > (uint32_t)kTile ? 2u : 1u;
-            pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
+            __syncwarp();
+            if (one) pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
             if (take == 0) break;
-            ok = wait(&bars->k_full[it & 1u], (it >> 1) & 1u);
+            ok = __all_sync(~0u, wait(&bars->k_full[it & 1u], (it >> 1) & 1u));
             for (uint32_t t = 0; ok && t < tiles; ++t) {
-                ok = wait(&bars->q_full[t], n_q[t]++ & 1u);
+                ok = __all_sync(~0u, wait(&bars->q_full[t], n_q[t]++ & 1u));
                 if (!ok) break;
                 fence_after();
                 qk(t, it & 1u);
             }
             if (!ok) break;
-            tc_commit(&bars->k_empty[it & 1u]);
+            tc_commit(one, &bars->k_empty[it & 1u]);
             for (uint32_t j = 0; ok && j < take; ++j, ++it) {
                 const uint32_t st = it & 1u, sn = (it + 1) & 1u;
-                ok = wait(&bars->v_full[st], (it >> 1) & 1u) && (j + 1 >= take || wait(&bars->k_full[sn], ((it + 1) >> 1) & 1u));
+                ok = __all_sync(~0u, wait(&bars->v_full[st], (it >> 1) & 1u) && (j + 1 >= take || wait(&bars->k_full[sn], ((it + 1) >> 1) & 1u)));
                 for (uint32_t t = j < take0 ? 0 : 1; ok && t < tiles; ++t) {
-                    ok = wait(&bars->p_full[t], n_p[t]++ & 1u);
+                    ok = __all_sync(~0u, wait(&bars->p_full[t], n_p[t]++ & 1u));
                     if (!ok) break;
                     fence_after();
                     const uint64_t vb = v_desc + st * (G::kK >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        tc_mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + (kk >> 2) * 64u + (kk & 3) * 8u, vb + ((kk >> 2) * (D * 8) + (kk & 3) * 2),
+                        tc_mma_ts(one, tmem + 256u + t * 128u, tmem + t * 128u + (kk >> 2) * 64u + (kk & 3) * 8u, vb + ((kk >> 2) * (D * 8) + (kk & 3) * 2),
                                   G::kIdescPV, (j | kk) != 0);
-                    tc_commit(&bars->o_done[t]);
+                    tc_commit(one, &bars->o_done[t]);
                     if (j + 1 < (t == 0 ? take0 : take)) qk(t, sn);
                 }
-                if (ok) tc_commit(&bars->v_empty[st]);
-                if (ok && j + 1 < take) tc_commit(&bars->k_empty[sn]);
+                if (ok) tc_commit(one, &bars->v_empty[st]);
+                if (ok && j + 1 < take) tc_commit(one, &bars->k_empty[sn]);
             }
         }
         if (!ok) {
             // unwinding: the products in flight end before their memory is given back
-            tc_commit(&bars->drained);
+            tc_commit(one, &bars->drained);
             const uint64_t t0 = clock64();
             while (!pipe::mbar_try(&bars->drained, 0) && clock64() - t0 < pipe::kWaitCycles) {}
         }
