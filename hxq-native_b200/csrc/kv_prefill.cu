@@ -103,16 +103,10 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ void tm_ld32(uint32_t taddr, uint32_t *v)
+__device__ __forceinline__ void tm_st8(uint32_t taddr, const uint32_t *v)
 {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-                 "%14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                 "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
-                 "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
-                 "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
-                 "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-                 : "r"(taddr)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                 "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
 
@@ -210,6 +204,62 @@ __device__ __forceinline__ float weigh16(const uint32_t *s, float f, float off, 
     }
     const float2 sum = unpack2(sum2);
     return sum.x + sum.y;
+}
+
+// The largest s + log2 vs of a row's 64 scores (of those it may see), 16 at a
+// time with the next 16 on their way.  Scales are not negative; NaN is passed
+// over here.
+template <bool MASK>
+__device__ __forceinline__ float largest64(uint32_t tS, const float4 *sc, float fac, uint32_t key0, int32_t pos, int32_t floor)
+{
+    uint32_t s[2][16];
+    float top = -INFINITY;
+    tm_ld16(tS, s[0]);
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int g = 2 * c + u;
+            wait_ld();
+            tm_ld16(tS + (min(g + 1, 3)) * 16, s[u ^ 1]);
+            if (MASK) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int32_t key = (int32_t)key0 + g * 16 + i;
+                    if (key > pos || key <= floor) s[u][i] = 0xff800000u;   // -infinity
+                }
+            }
+            top = fmaxf(top, fmaf(largest16(s[u]), fac * sc[g].x, sc[g].y));
+        }
+    }
+    wait_ld();
+    return top;
+}
+
+// Their weights as f16 over the first half of their columns (16 scores are
+// read, then 8 columns written); returns the sum of weight / vs.
+template <bool MASK>
+__device__ __forceinline__ float weigh64(uint32_t tS, const float4 *sc, float fac, float ms, uint32_t key0, int32_t pos, int32_t floor)
+{
+    uint32_t s[2][16];
+    float l = 0.0f;
+    tm_ld16(tS, s[0]);
+#pragma unroll 1
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int g = 2 * c + u;
+            uint32_t p[8];
+            wait_ld();
+            tm_ld16(tS + (min(g + 1, 3)) * 16, s[u ^ 1]);
+            const float sum = weigh16<MASK>(s[u], fac * sc[g].x, sc[g].y - ms, p, (int32_t)key0 + g * 16, pos, floor);
+            // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
+            l += MASK && sum == 0.0f ? 0.0f : sum * sc[g].z;
+            tm_st8(tS + g * 8, p);
+        }
+    }
+    wait_ld();
+    return l;
 }
 
 template <int D, int FMT, typename QT>
@@ -340,25 +390,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 fence_after();
                 const float4 *sc = scales + ((step0 + j) & (kScaleSlots - 1)) * 8 + hf * 4;
                 const bool all = (int32_t)(key0 + 63) <= pos_first && (int32_t)key0 > floor_last;
-                float top = -INFINITY;
-                // scales are not negative; NaN is passed over here
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t s[32];
-                    tm_ld32(tS + c * 32, s);
-                    wait_ld();
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        if (!all) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const int32_t key = (int32_t)key0 + c * 32 + g * 16 + i;
-                                if (key > pos || key <= floor) s[g * 16 + i] = 0xff800000u;   // -infinity
-                            }
-                        }
-                        top = fmaxf(top, fmaf(largest16(s + g * 16), fac * sc[c * 2 + g].x, sc[c * 2 + g].y));
-                    }
-                }
+                float top = all ? largest64<false>(tS, sc, fac, key0, pos, floor) : largest64<true>(tS, sc, fac, key0, pos, floor);
                 // and of the other half's
                 tops[hf * kTile + rr] = top;
                 named_sync(pair, 64);
@@ -385,27 +417,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     }
                 }
                 const float ms = M == -INFINITY ? 0.0f : M;
-                // weights as f16 over the first half of this half's columns: 32 scores are read, then 16 columns written
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t s[32], p[16];
-                    tm_ld32(tS + c * 32, s);
-                    wait_ld();
-                    if (all) {
-#pragma unroll
-                        for (int g = 0; g < 2; ++g)
-                            l += weigh16<false>(s + g * 16, fac * sc[c * 2 + g].x, sc[c * 2 + g].y - ms, p + g * 8, 0, 0, 0) * sc[c * 2 + g].z;
-                    } else {
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const float sum = weigh16<true>(s + g * 16, fac * sc[c * 2 + g].x, sc[c * 2 + g].y - ms, p + g * 8,
-                                                            (int32_t)key0 + c * 32 + g * 16, pos, floor);
-                            // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
-                            l += sum == 0.0f ? 0.0f : sum * sc[c * 2 + g].z;
-                        }
-                    }
-                    tm_st16(tS + c * 16, p);
-                }
+                l += all ? weigh64<false>(tS, sc, fac, ms, key0, pos, floor) : weigh64<true>(tS, sc, fac, ms, key0, pos, floor);
                 wait_st();
                 fence_before();
                 pipe::mbar_arrive(&bars->p_full[t]);
