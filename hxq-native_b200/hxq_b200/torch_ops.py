@@ -22,9 +22,6 @@ import ctypes as C
 import torch
 
 from . import (HXQ_IMAGE_MATMUL, HXQ_OUT_BF16, HXQ_OUT_F32, AffineTensor, Tensor, check, lib)
-from .serving import KvCache, LoraAdapters, LoraPlan
-from .serving import kv_plan as _kv_plan
-from .serving import lora_plan as _lora_plan
 
 _DT = {torch.float32: HXQ_OUT_F32, torch.bfloat16: HXQ_OUT_BF16}
 
@@ -102,8 +99,9 @@ def _(x, codes, scales, offsets, bias, group_size):
 def kv_plan(new: torch.Tensor, cached: torch.Tensor, table: torch.Tensor, free: torch.Tensor, block_tokens: int,
             n_slots: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """starts, lens, slots, positions, taken; enters new blocks in table."""
+    from .serving import kv_plan as plan
     # an operator's results may not share memory
-    return tuple(t.clone() for t in _kv_plan(new, cached, table, free, block_tokens, n_slots))
+    return tuple(t.clone() for t in plan(new, cached, table, free, block_tokens, n_slots))
 
 
 @kv_plan.register_fake
@@ -116,6 +114,7 @@ def _(new, cached, table, free, block_tokens, n_slots):
 def kv_append(k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor, k: torch.Tensor,
               v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantise rows of k and v into their slots of an 8-bit cache."""
+    from .serving import KvCache
     KvCache(k_codes, v_codes, k_scales, v_scales).append(k, v, slots)
 
 
@@ -129,6 +128,7 @@ def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, 
                  starts: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, max_new: int, scale: float, window: int,
                  causal: bool) -> torch.Tensor:
     """Attention of q [rows, heads, head_dim] over an 8-bit cache."""
+    from .serving import KvCache
     return KvCache(k_codes, v_codes, k_scales, v_scales).attention(q, starts, lens, table, max_new, scale, window, causal)
 
 
@@ -141,7 +141,8 @@ def _(q, k_codes, v_codes, k_scales, v_scales, starts, lens, table, max_new, sca
 def lora(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, starts: torch.Tensor,
          adapters: torch.Tensor) -> torch.Tensor:
     """y + scale (x A^T) B^T of each request's adapter."""
-    return LoraAdapters(a, b, scales).add(y, x, _lora_plan(starts, adapters, a.shape[0], x.shape[0]))
+    from .serving import LoraAdapters, lora_plan
+    return LoraAdapters(a, b, scales).add(y, x, lora_plan(starts, adapters, a.shape[0], x.shape[0]))
 
 
 @lora.register_fake
@@ -182,9 +183,10 @@ class HxqLinear(torch.nn.Module):
     def weight(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return dequant(self.image, self.out_features, self.in_features, dtype)
 
-    def forward(self, x: torch.Tensor, adapters: LoraAdapters | None = None, plan: LoraPlan | None = None) -> torch.Tensor:
-        """x @ W.T in fp32; with `adapters` (of this projection's rows) and the
-        step's plan (hxq_b200.serving.lora_plan), plus each token's adapter."""
+    def forward(self, x: torch.Tensor, adapters=None, plan=None) -> torch.Tensor:
+        """x @ W.T in fp32; with `adapters` (a hxq_b200.serving.LoraAdapters of
+        this projection's rows) and the step's plan (lora_plan), plus each
+        token's adapter."""
         if self.fused:
             y = vq_matmul(x.to(torch.bfloat16), self.image, self.out_features)
         else:

@@ -83,3 +83,45 @@ def test_affine_op_matches_the_c_abi(H, L, cuda):
         assert L.hxq_affine_group_matmul_bf16(x.data_ptr(), C.byref(t), ref.data_ptr(), N, None) == 0
         torch.cuda.synchronize()
         assert torch.equal(y.view(torch.int32), ref.view(torch.int32))
+
+
+def test_serving_ops_fake_shapes():
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import hxq_b200.torch_ops  # noqa: F401
+    with FakeTensorMode():
+        i = lambda *s: torch.empty(s, dtype=torch.int32, device="cuda")  # noqa: E731
+        q = torch.empty((7, 8, 128), dtype=torch.bfloat16, device="cuda")
+        c, s = torch.empty((4, 2, 16, 128), dtype=torch.int8, device="cuda"), torch.empty((4, 2), device="cuda")
+        o = torch.ops.hxq.kv_attention(q, c, c, s, s, i(4), i(3), i(3, 5), 4, 0.1, 0, True)
+        assert o.shape == q.shape and o.dtype == q.dtype
+        starts, lens, slots, pos, taken = torch.ops.hxq.kv_plan(i(3), i(3), i(3, 5), i(9), 16, 20)
+        assert (starts.shape[0], lens.shape[0], slots.shape[0], pos.shape[0], taken.shape[0]) == (4, 3, 20, 20, 1)
+        y, x = torch.empty((7, 32), device="cuda"), torch.empty((7, 64), dtype=torch.bfloat16, device="cuda")
+        a, b = (torch.empty(n, dtype=torch.bfloat16, device="cuda") for n in ((2, 8, 64), (2, 32, 8)))
+        assert torch.ops.hxq.lora(y, x, a, b, torch.empty(2, device="cuda"), i(4), i(3)).shape == y.shape
+
+
+@pytest.mark.gpu
+def test_serving_ops_match_the_calls(H, L, cuda):
+    torch = cuda
+    import hxq_b200.torch_ops  # noqa: F401
+    from hxq_b200 import serving as S
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.full((2, 3), -1, dtype=torch.int32, device="cuda")
+    starts, lens, slots, _, _ = torch.ops.hxq.kv_plan(i(20, 3), i(0, 0), table, i(4, 2, 5, 0), 16, 23)
+    one, two = S.KvCache.allocate(6, 2, 64), S.KvCache.allocate(6, 2, 64)
+    k, v = torch.randn((2, 23, 2, 64), device="cuda")
+    torch.ops.hxq.kv_append(one.k, one.v, one.k_scales, one.v_scales, k, v, slots)
+    two.append(k, v, slots)
+    assert torch.equal(one.k, two.k) and torch.equal(one.v_scales, two.v_scales)
+    q = torch.randn((23, 4, 64), device="cuda").to(torch.bfloat16)
+    o = torch.ops.hxq.kv_attention(q, one.k, one.v, one.k_scales, one.v_scales, starts, lens, table, 20, 0.125, 0, True)
+    assert torch.equal(o, two.attention(q, starts, lens, table, 20))
+    y, x = torch.randn((23, 32), device="cuda"), torch.randn((23, 64), device="cuda").to(torch.bfloat16)
+    a, b = torch.randn((1, 8, 64), device="cuda").to(torch.bfloat16), torch.randn((1, 32, 8), device="cuda").to(torch.bfloat16)
+    s = torch.ones(1, device="cuda")
+    got = torch.ops.hxq.lora(y, x, a, b, s, starts, i(0, -1))
+    assert torch.equal(got, S.LoraAdapters(a, b, s).add(y, x, S.lora_plan(starts, i(0, -1), 1, 23)))
+    assert torch.equal(got[20:], y[20:]) and not torch.equal(got[:20], y[:20])
