@@ -17,10 +17,11 @@
 // products are m16n8k16 with keys, then dimensions, on the side of 16 and rows
 // on that of 8 (S^T = K Q^T, O^T = V^T P^T): one request's group of heads
 // fills the small side, so a decode step of up to 8 heads a group wastes
-// nothing of it.  A lane's share of a key row is 16 consecutive bytes: the
-// order of the head's dimensions inside a product is free as long as Q has
-// the same, so codes go from a lane's own 16-byte copies (cp.async into slots
-// that no other lane reads: no barrier in the loop) through a byte permute
+// nothing of it.  TMA brings 16 keys' codes at a time (two boxes of 16 rows,
+// swizzled so that the fragments' loads meet no bank twice) into a ring of each
+// warp's own, two steps ahead; the order of the head's dimensions inside a
+// product is free as long as Q has the same, so a lane reads 16 consecutive
+// bytes of a key and brings them through a byte permute
 // into the fragments; the weights turn round with movmatrix.  The maximum is
 // raised only where a weight would pass 2^8 (f16 holds 2^16): a vote a step
 // instead of a reduction.
@@ -45,26 +46,23 @@ constexpr int kThreadsA = kWarpsA * 32;
 constexpr float kRaiseA = 8.0f;  // log2 of the largest weight before the maximum is raised
 
 template <int D> struct Geo {
-    static constexpr int kVB = D >= 128 ? 16 : 8;      // bytes of a lane's copy of a value row
-    static constexpr int kVC = D / (8 * kVB);          // copies of a value row per lane
-    static constexpr int kKC = D / 64;                 // copies of a key row per lane
-    static constexpr int kSlot = 32 * D + 32 * 8;      // K and V of 16 keys, and the two scales per lane
+    static constexpr int kVB = D >= 128 ? 16 : 8;      // bytes of a lane's load of a value row
+    static constexpr int kVC = D / (8 * kVB);          // loads of a value row per lane
+    static constexpr int kKC = D / 64;                 // loads of a key row per lane
+    static constexpr int kLine = D >= 128 ? 128 : 64;  // bytes of a box's rows (swizzled over that span)
+    static constexpr int kBoxes = D / kLine;
+    static constexpr int kSlot = 32 * D;               // K and V of 16 keys
     static constexpr int kStages = D == 64 ? 4 : 3;
     static constexpr int kRing = kWarpsA * kStages * kSlot;
     static constexpr int kPad = 4;
     static constexpr int kMerge = kWarpsA * kMostRows * (D + kPad) * 4;
-    static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
-    static_assert(kSmem >= 4 * (HXQ_ATTENTION_MAX_REQUESTS + 1), "room for the scan");
+    static constexpr int kBig = kRing > kMerge ? kRing : kMerge;
+    static constexpr int kOffScale = kBig > 33024 ? kBig : 33024;             // two scales a lane and stage
+    static constexpr int kOffBar = kOffScale + kWarpsA * kStages * 256;
+    static constexpr int kSmem = kOffBar + kWarpsA * kStages * 8 + 1024;      // and room to begin on 1024
+    static_assert(kOffScale >= 4 * (HXQ_ATTENTION_MAX_REQUESTS + 1), "room for the scan");
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void *src)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp4(uint32_t dst, const void *src)
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -79,6 +77,21 @@ template <typename QT> __device__ __forceinline__ uint32_t to_f16x2(uint32_t w, 
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Bounded wait for a copy (2^21 tries of up to a microsecond).
+__device__ __forceinline__ bool arrived(uint64_t *bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
+        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t@p bra DONE_%=;\n\t"
+        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 2097152;\n\t@q bra AGAIN_%=;\n"
+        "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(pipe::smem_u32(bar)), "r"(parity), "r"(1000u)
+        : "memory");
+    return ok != 0;
+}
+
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v)
 {
     uint32_t d;
@@ -90,11 +103,12 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t v)
 __host__ __device__ constexpr uint32_t ctas_per_sm(uint32_t D, bool few) { return D == 256 ? 2u : D == 128 && !few ? 3u : 4u; }
 
 template <int D, int FMT, typename QT, int NT>
-__global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_kernel(const __grid_constant__ AttnArgs a)
+__global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap)
 {
     using G = Geo<D>;
     constexpr int kRows = 8 * NT;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (pipe::smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ RangeShared<kWarpsA> sh;
     __shared__ float sh_m[kWarpsA][kRows], sh_l[kWarpsA][kRows];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
@@ -105,8 +119,31 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
     __syncthreads();   // the sums in front of the requests are read: the ring may be filled
 
     const uint32_t ring = pipe::smem_u32(smem) + warp * (G::kStages * G::kSlot);
+    const uint32_t scales = pipe::smem_u32(smem) + G::kOffScale + warp * (G::kStages * 256) + lane * 8;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + G::kOffBar) + warp * G::kStages;
     float *merge = reinterpret_cast<float *>(smem);
-    const uint32_t k_lane = g * D + q * 16, v_lane = 2 * q * D + g * G::kVB;   // of a 16-key piece
+    if (lane == 0) {
+        for (int s = 0; s < G::kStages; ++s) pipe::mbar_init(full + s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    uint32_t phase = 0;   // bit s: parity of stage s's next arrival
+    // This lane's 16 bytes of key g (key g + 8: 8 rows on), and of dimensions
+    // 16 g .. of keys 2 q and 2 q + 1; a row's 16-byte pieces are swapped by
+    // the row's number (128-byte rows: row & 7, 64-byte rows: row / 2 & 3)
+    uint32_t k_at[2], v_at[2];
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t row = 2 * q + i;
+        if (D == 64) {
+            k_at[i] = g * 64 + ((q ^ (g >> 1 & 3u)) << 4);
+            v_at[i] = row * 64 + (((g >> 1) ^ (row >> 1 & 3u)) << 4) + (g & 1u) * 8;
+        } else {
+            k_at[i] = g * 128 + (((2 * q + i) ^ g) << 4);
+            v_at[i] = row * 128 + ((g ^ (row & 7u)) << 4);
+        }
+    }
+    bool in_time = true;
 
     Segment seg;
     while (next_segment<kRows, kGran, kFixed>(a, range, seg)) {
@@ -134,25 +171,22 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
             if (ok) {
                 uint32_t slot;
                 block_of(a, key, slot);
-                const size_t bh = (size_t)(uint32_t)blk * a.H + h, base = (bh * a.P + slot) * D;
-                const uint8_t *ks = a.k + base + k_lane, *vs = a.v + base + v_lane;
-                const uint32_t dst = ring + stage * G::kSlot + lane * 16;
+                const uint32_t bh = (uint32_t)blk * a.H + h;
+                cp4(scales + stage * 256, a.ks + bh);
+                cp4(scales + stage * 256 + 4, a.vs + bh);
+                // the stage's last reads come before the copy
+                pipe::async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    const int32_t row = (int32_t)(bh * a.P + slot);
+                    uint8_t *dst = smem + (size_t)(warp * G::kStages + stage) * G::kSlot;
+                    pipe::mbar_expect_tx(full + stage, G::kSlot);
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int c = 0; c < G::kKC; ++c) cp16(dst + (half * G::kKC + c) * 512, ks + half * 8 * D + c * 64);
-                const uint32_t vdst = ring + stage * G::kSlot + 16 * D + lane * G::kVB;
-#pragma unroll
-                for (int ts = 0; ts < 4; ++ts)
-#pragma unroll
-                    for (int c = 0; c < G::kVC; ++c) {
-                        const void *src = vs + ((ts & 1) + (ts >> 1) * 8) * D + c * 128;
-                        if (G::kVB == 16) cp16(vdst + (ts * G::kVC + c) * 512, src);
-                        else cp8(vdst + ts * 256, src);
+                    for (int b = 0; b < G::kBoxes; ++b) {
+                        pipe::tma_load_2d(dst + b * 2048, &kmap, full + stage, b * 128, row);
+                        pipe::tma_load_2d(dst + 16 * D + b * 2048, &vmap, full + stage, b * 128, row);
                     }
-                const uint32_t sdst = ring + stage * G::kSlot + 32 * D + lane * 8;
-                cp4(sdst, a.ks + bh);
-                cp4(sdst + 4, a.vs + bh);
+                }
             }
             cp_commit();
         };
@@ -180,7 +214,8 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
             for (int c = 0; c < G::kKC; ++c)
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const uint4 v = in ? __ldg(reinterpret_cast<const uint4 *>(p + c * 64 + q * 16) + w) : make_uint4(0, 0, 0, 0);
+                    const uint32_t d0 = D == 64 ? q * 16 : (c >> 1) * 128 + (2 * q + (c & 1)) * 16;
+                    const uint4 v = in ? __ldg(reinterpret_cast<const uint4 *>(p + d0) + w) : make_uint4(0, 0, 0, 0);
                     qf[n][c * 4 + w * 2][0] = v.x;
                     qf[n][c * 4 + w * 2][1] = v.y;
                     qf[n][c * 4 + w * 2 + 1][0] = v.z;
@@ -235,6 +270,10 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
         for (uint32_t j = 0; j < take; ++j) {
             cp_wait<G::kStages - 2>();
             const bool live = valid >> stage & 1u;
+            if (live) {
+                in_time = in_time && arrived(full + stage, phase >> stage & 1u);
+                phase ^= 1u << stage;
+            }
             {
                 const uint32_t into = stage == 0 ? G::kStages - 1 : stage - 1;
                 issue(j + G::kStages - 1, into, next);
@@ -242,14 +281,16 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
             }
             if (live) {
                 const uint32_t src = ring + stage * G::kSlot;
-                const uint2 sc = pipe::lds64(src + 32 * D + lane * 8);
-                float s[NT][4];
+                const uint2 sc = pipe::lds64(scales + stage * 256);
+                float s[NT][4], s2[NT][4];   // two chains of products
 #pragma unroll
-                for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < G::kKC; ++c) {
-                    const uint4 ka = pipe::lds128(src + c * 512 + lane * 16);                // key g
-                    const uint4 kb = pipe::lds128(src + (G::kKC + c) * 512 + lane * 16);     // key g + 8
+                    const uint32_t at = src + (c >> 1) * 2048 + k_at[c & 1];
+                    const uint4 ka = pipe::lds128(at), kb = pipe::lds128(at + 8 * G::kLine);   // keys g, g + 8
                     const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -258,7 +299,7 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
                         codes_to_f16<FMT>(wb[i], a1, a3);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
-                            pipe::mma16816_f16(s[n], a0, a1, a2, a3, qf[n][c * 4 + i][0], qf[n][c * 4 + i][1]);
+                            pipe::mma16816_f16(i & 1 ? s2[n] : s[n], a0, a1, a2, a3, qf[n][c * 4 + i][0], qf[n][c * 4 + i][1]);
                     }
                 }
                 const uint32_t key = key0 + j * kGran;
@@ -270,7 +311,7 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e], fac[n][e & 1] * ks, lv);
+                    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(s[n][e] + s2[n][e], fac[n][e & 1] * ks, lv);
                 if (!((int32_t)(key + 15) <= pos_first && (int32_t)key > floor_last)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -334,13 +375,13 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
 #pragma unroll
                     for (int ts = 0; ts < 4; ++ts) {
                         if (G::kVB == 16) {
-                            const uint4 v = pipe::lds128(src + 16 * D + (ts * G::kVC + c) * 512 + lane * 16);
+                            const uint4 v = pipe::lds128(src + 16 * D + c * 2048 + (ts >> 1) * 8 * G::kLine + v_at[ts & 1]);
                             vw[ts][0] = v.x;
                             vw[ts][1] = v.y;
                             vw[ts][2] = v.z;
                             vw[ts][3] = v.w;
                         } else {
-                            const uint2 v = pipe::lds64(src + 16 * D + ts * 256 + lane * 8);
+                            const uint2 v = pipe::lds64(src + 16 * D + (ts >> 1) * 8 * G::kLine + v_at[ts & 1]);
                             vw[ts][0] = v.x;
                             vw[ts][1] = v.y;
                             vw[ts][2] = vw[ts][3] = 0;
@@ -441,8 +482,10 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
             }
         }
         if (seg.begins && take < seg.n && tid == 0) a.desc[blockIdx.x] = cut_unit(range, seg);
+        pipe::async_proxy_fence();
         __syncthreads();   // the ring is free again
     }
+    if (!in_time && lane == 0) flag(a.status, HXQ_SERVING_TIMEOUT);
 }
 
 template <int D, typename QT, int NT> __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a)
@@ -451,13 +494,27 @@ template <int D, typename QT, int NT> __global__ void __launch_bounds__(128) att
     join_row<8 * NT, kMostRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
 }
 
+// The codes as rows of D bytes, in boxes of 16 rows of 128 (64) bytes.
+bool encode_codes(CUtensorMap *map, const uint8_t *codes, const AttnArgs &a, uint32_t D)
+{
+    const pipe::EncodeTiledFn enc = pipe::encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {D, (cuuint64_t)a.n_blocks * a.H * a.P}, strides[1] = {D};
+    const cuuint32_t box[2] = {D >= 128 ? 128u : 64u, 16u}, step[2] = {1u, 1u};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dims, strides, box, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, D >= 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, int FMT, typename QT, int NT> cudaError_t launch_one(const AttnArgs &a, uint32_t grid, cudaStream_t s)
 {
     auto kernel = attn_mma_kernel<D, FMT, QT, NT>;
     static std::atomic<uint64_t> ready{0};
     cudaError_t e = allow_smem(kernel, Geo<D>::kSmem, ready);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, kThreadsA, Geo<D>::kSmem, s>>>(a);
+    CUtensorMap kmap, vmap;
+    if (!encode_codes(&kmap, a.k, a, D) || !encode_codes(&vmap, a.v, a, D)) return cudaErrorInvalidValue;
+    kernel<<<grid, kThreadsA, Geo<D>::kSmem, s>>>(a, kmap, vmap);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     return launch_behind(attn_join_kernel<D, QT, NT>, dim3(grid, 2 * NT), dim3(128), 0, s, a);
 }
@@ -493,6 +550,7 @@ hxq_error_t check_attention(const hxq_kv_cache_t *c, const hxq_kv_attention_t *p
     if (p->n_requests > HXQ_ATTENTION_MAX_REQUESTS || (uint64_t)p->n_rows * (p->n_heads / c->n_heads) >= (1ull << 30))
         return HXQ_ERR_INVALID_ARG;
     if ((uint64_t)p->table_width * c->block_tokens >= (1ull << 31)) return HXQ_ERR_INVALID_ARG;
+    if ((uint64_t)c->n_blocks * c->block_tokens * c->n_heads >= (1ull << 31)) return HXQ_ERR_INVALID_ARG;   // rows of a copy's map
     if (p->window && !p->causal) return HXQ_ERR_INVALID_ARG;
     if (!(p->scale >= 0.0f) || p->scale > 3.402823466e38f) return HXQ_ERR_INVALID_ARG;
     return HXQ_OK;

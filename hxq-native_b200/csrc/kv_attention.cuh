@@ -196,8 +196,13 @@ __device__ __forceinline__ bool find_range(const AttnArgs &a, RangeShared<WARPS>
     uint64_t n = (out.total + least - 1) / least;
     n = n < gridDim.x ? n : gridDim.x;
     if (blockIdx.x >= n) return false;
-    out.x = out.total * blockIdx.x / n;
-    out.x1 = out.total * (blockIdx.x + 1) / n;
+    if (out.total <= 0xffffffffu / 4096u && gridDim.x < 4096u) {   // products of 32 bits
+        out.x = (uint32_t)out.total * blockIdx.x / (uint32_t)n;
+        out.x1 = (uint32_t)out.total * (blockIdx.x + 1) / (uint32_t)n;
+    } else {
+        out.x = out.total * blockIdx.x / n;
+        out.x1 = out.total * (blockIdx.x + 1) / n;
+    }
     out.ctas = n;
     if (at <= out.x && out.x < at + mine) {
         Req r = load_req(a, lo);
@@ -222,7 +227,7 @@ __device__ __forceinline__ bool find_range(const AttnArgs &a, RangeShared<WARPS>
     out.tile = sh.tile;
     out.r = load_req(a, out.b);
     out.n = FIXED + tile_grans<ROWS, KEYS>(a, out.r, out.tile, out.first);
-    out.h = (uint32_t)(sh.off / out.n);
+    out.h = sh.off <= 0xffffffffu ? (uint32_t)sh.off / out.n : (uint32_t)(sh.off / out.n);
     out.rem = (uint32_t)(sh.off - (uint64_t)out.h * out.n);
     return true;
 }
@@ -294,7 +299,7 @@ __device__ __forceinline__ float ex2(float x)
 __device__ __forceinline__ float lg2(float x)
 {
     float y;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -359,7 +364,7 @@ __device__ __forceinline__ void value_scale(float vs, float &lv, float &inv, boo
     zero = vs < 7.8886090522101181e-31f;   // 2^-100
     const float c = zero ? 7.8886090522101181e-31f : vs;
     lv = lg2(c);
-    asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(c));   // within an ulp
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(c));   // within an ulp
 }
 
 // Partial results of a CTA: two slots of ROWS x D sums, then the rows' maxima

@@ -120,7 +120,8 @@ hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots
  * max_new: the most rows of any request; it only chooses the kernel, results
  * hold for any value.  workspace: hxq_cuda_kv_attention_workspace bytes,
  * 16-byte aligned, contents don't matter before or after; calls that may
- * overlap in time need one each.  At most HXQ_ATTENTION_MAX_REQUESTS. */
+ * overlap in time need one each.  At most HXQ_ATTENTION_MAX_REQUESTS requests;
+ * n_blocks * n_heads * block_tokens < 2^31. */
 #define HXQ_ATTENTION_MAX_REQUESTS 8192
 typedef struct {
     const void    *d_q;
