@@ -77,17 +77,17 @@ template <typename QT> __device__ __forceinline__ uint32_t to_f16x2(uint32_t w, 
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Bounded wait for a copy (2^21 tries of up to a microsecond).
+// Bounded wait for a copy (2^24 tries).
 __device__ __forceinline__ bool arrived(uint64_t *bar, uint32_t parity)
 {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
-        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t@p bra DONE_%=;\n\t"
-        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 2097152;\n\t@q bra AGAIN_%=;\n"
+        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\t"
+        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 16777216;\n\t@q bra AGAIN_%=;\n"
         "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(pipe::smem_u32(bar)), "r"(parity), "r"(1000u)
+        : "r"(pipe::smem_u32(bar)), "r"(parity)
         : "memory");
     return ok != 0;
 }

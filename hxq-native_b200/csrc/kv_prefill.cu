@@ -15,8 +15,9 @@
 //               [dim][key], both K-major with 128-byte swizzle;
 //   warp 20     one thread issues S = Q K^T (both operands in shared memory)
 //               and O += P V (P in tensor memory);
-//   warp 21     a lane for every 16 keys looks up their block, copies its
-//               codes to shared memory (cp.async.bulk) and its scales;
+//   warps 21,23 a lane for every 16 keys looks up their block, copies its
+//               codes to shared memory (cp.async.bulk) and its scales, one
+//               warp for keys and one for values;
 //   warp 22     one thread cuts the CTA's range into segments for the others.
 // The two tiles take turns: while one is at its exponentials, the tensor
 // cores work for the other.  Tensor memory: S/P of tile t at column 128 t,
@@ -40,7 +41,7 @@ constexpr int kTile = 128;                 // rows of a tile
 constexpr int kFixedT = 2;                 // steps that a unit costs by itself
 constexpr int kSoftWarps = 16, kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps, kLoadWarp = kMmaWarp + 1, kPlanWarp = kMmaWarp + 2;
-constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups; the last warp has nothing to do
+constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups
 // Registers: launched with 80 a thread, 61,440 in all; the rows' threads hold
 // 16 scores and the next 16. 512 x 88 + 128 x 64 + 128 x 64 = 61,440.
 constexpr int kRegsSoft = 88, kRegsConv = 64, kRegsRest = 64;
@@ -152,18 +153,18 @@ struct SegInfo {
 };
 static_assert(sizeof(SegInfo) == 64, "a slot");
 
-// Bounded wait (2^21 tries of up to a microsecond, in which the thread is
-// suspended); false if it ran out.
+// Bounded wait (2^24 tries, each of which the hardware suspends for a while);
+// false if it ran out.
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity)
 {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
-        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t@p bra DONE_%=;\n\t"
-        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 2097152;\n\t@q bra AGAIN_%=;\n"
+        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\t"
+        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 16777216;\n\t@q bra AGAIN_%=;\n"
         "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(pipe::smem_u32(bar)), "r"(parity), "r"(1000u)
+        : "r"(pipe::smem_u32(bar)), "r"(parity)
         : "memory");
     return ok != 0;
 }
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         pipe::mbar_init(&bars->rawv_empty, kConvWarps);
         for (int i = 0; i < kSegSlots; ++i) {
             pipe::mbar_init(&bars->seg_full[i], 1);
-            pipe::mbar_init(&bars->seg_empty[i], kSoftWarps + 2);   // the rows' warps, loads, products
+            pipe::mbar_init(&bars->seg_empty[i], kSoftWarps + 3);   // the rows' warps, both loads, products
         }
         pipe::mbar_init(&bars->drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -598,8 +599,12 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
-        if (warp == kLoadWarp && lane < 8) {
-            // --------------------------------------------------- loads
+        if ((warp == kLoadWarp || warp == kLoadWarp + 2) && lane < 8) {
+            // --------------------------------------------------- loads: a warp for the keys, one for the values
+            const bool keys = warp == kLoadWarp;
+            uint64_t *raw_full = keys ? &bars->rawk_full : &bars->rawv_full, *raw_empty = keys ? &bars->rawk_empty : &bars->rawv_empty;
+            const uint8_t *codes = keys ? a.k : a.v;
+            uint8_t *dst = smem + G::kOffRaw + (keys ? 0 : G::kRaw) + lane * 16 * D;
             uint32_t it = 0;
             for (uint32_t si = 0; ok; ++si) {
                 ok = wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u);
@@ -609,61 +614,68 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 if (lane == 0) pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
                 if (seg.take == 0) break;
                 const int32_t *row = a.table + (size_t)seg.b * a.width;
-                uint32_t slot;
-                // the block of the next step is looked up while this one's copies are under way
+                // blocks are looked up two steps ahead, their scales one
                 auto entry = [&](uint32_t j) -> int32_t {
                     const uint32_t key = seg.key0 + j * kKeys + lane * 16;
+                    uint32_t slot;
                     return j < seg.take && key < seg.hi ? __ldg(row + block_of(a, key, slot)) : -1;
                 };
-                auto zeros = [&](uint8_t *dst) {   // in place of a block outside the cache
-                    for (int i = 0; i < D; ++i) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0, 0, 0, 0);
-                    pipe::async_proxy_fence();
+                auto scales_of = [&](int32_t blk, float &ks, float &vs) {
+                    ks = vs = 0.0f;
+                    if ((uint32_t)blk < a.n_blocks) {
+                        const size_t bh = (size_t)(uint32_t)blk * a.H + seg.h;
+                        if (keys) ks = __ldg(a.ks + bh);
+                        vs = __ldg(a.vs + bh);
+                    }
                 };
-                int32_t next = entry(0);
+                int32_t blk = entry(0), blk1 = entry(1);
+                float ks, vs;
+                scales_of(blk, ks, vs);
                 for (uint32_t j = 0; j < seg.take; ++j, ++it) {
-                    const int32_t blk = next;
                     const uint32_t key0 = seg.key0 + j * kKeys, key = key0 + lane * 16;
+                    const int32_t blk2 = entry(j + 2);
+                    float ks1, vs1;
+                    scales_of(blk1, ks1, vs1);
                     const bool in = key < seg.hi && (uint32_t)blk < a.n_blocks;
-                    if (key < seg.hi && !in) flag(a.status, HXQ_SERVING_BAD_BLOCK);
+                    if (keys && key < seg.hi && !in) flag(a.status, HXQ_SERVING_BAD_BLOCK);
+                    uint32_t slot;
+                    block_of(a, key, slot);
+                    const size_t src = (((size_t)(in ? (uint32_t)blk : 0u) * a.H + seg.h) * a.P + slot) * D;
                     float4 b = make_float4(0.0f, -INFINITY, 0.0f, 0.0f);   // keys outside: no weight
                     bool zero = true;
-                    const size_t bh = (size_t)(in ? (uint32_t)blk : 0u) * a.H + seg.h;
-                    block_of(a, key, slot);
-                    const size_t src = (bh * a.P + slot) * D;
                     if (in) {
-                        b.x = __ldg(a.ks + bh);
-                        value_scale(__ldg(a.vs + bh), b.y, b.z, zero);
+                        b.x = ks;
+                        value_scale(vs, b.y, b.z, zero);
                     }
-                    next = entry(j + 1);
-                    if (it >= 1) ok = wait(&bars->rawk_empty, (it - 1) & 1u);
+                    if (it >= 1) ok = wait(raw_empty, (it - 1) & 1u);
                     if (!ok) break;
-                    scales[(it & (kScaleSlots - 1)) * 8 + lane] = b;
-                    bars->zero[it & 1u][lane] = zero;
-                    if (lane == 0) bars->live[it & 1u] = min((uint32_t)kKeys, seg.hi > key0 ? seg.hi - key0 : 1u);
-                    uint8_t *dst = smem + G::kOffRaw + lane * 16 * D;
+                    if (keys) {
+                        scales[(it & (kScaleSlots - 1)) * 8 + lane] = b;
+                        if (lane == 0) bars->live[it & 1u] = min((uint32_t)kKeys, seg.hi > key0 ? seg.hi - key0 : 1u);
+                    } else bars->zero[it & 1u][lane] = zero;
                     if (in) {
-                        pipe::mbar_expect_tx(&bars->rawk_full, 16 * D);
-                        pipe::bulk_g2s(dst, a.k + src, 16 * D, &bars->rawk_full);
+                        pipe::mbar_expect_tx(raw_full, 16 * D);
+                        pipe::bulk_g2s(dst, codes + src, 16 * D, raw_full);
                     } else {
-                        if (key < seg.hi) zeros(dst);
-                        pipe::mbar_arrive(&bars->rawk_full);
+                        if (key < seg.hi) {   // in place of a block outside the cache
+                            for (int i = 0; i < D; ++i) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0, 0, 0, 0);
+                            pipe::async_proxy_fence();
+                        }
+                        pipe::mbar_arrive(raw_full);
                     }
-                    if (it >= 1) ok = wait(&bars->rawv_empty, (it - 1) & 1u);
-                    if (!ok) break;
-                    if (in) {
-                        pipe::mbar_expect_tx(&bars->rawv_full, 16 * D);
-                        pipe::bulk_g2s(dst + G::kRaw, a.v + src, 16 * D, &bars->rawv_full);
-                    } else {
-                        if (key < seg.hi) zeros(dst + G::kRaw);
-                        pipe::mbar_arrive(&bars->rawv_full);
-                    }
+                    blk = blk1;
+                    blk1 = blk2;
+                    ks = ks1;
+                    vs = vs1;
                 }
             }
             // the end of the work
-            if (ok && it >= 1) ok = wait(&bars->rawk_empty, (it - 1) & 1u);
-            if (ok) {
-                if (lane == 0) bars->live[it & 1u] = 0;
-                pipe::mbar_arrive(&bars->rawk_full);
+            if (keys) {
+                if (ok && it >= 1) ok = wait(raw_empty, (it - 1) & 1u);
+                if (ok) {
+                    if (lane == 0) bars->live[it & 1u] = 0;
+                    pipe::mbar_arrive(raw_full);
+                }
             }
             // copies under way end before the CTA does
             if (!ok) {
