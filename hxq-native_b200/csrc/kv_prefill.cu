@@ -280,13 +280,13 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
     if (!find_range<kWarpsT, kTcRows, kKeys, kFixedT>(a, sh, reinterpret_cast<uint32_t *>(smem), false, range)) return;
     if (tid == 0) {
         for (int t = 0; t < 2; ++t) {
-            pipe::mbar_init(&bars->q_full[t], 2 * kTile);
+            pipe::mbar_init(&bars->q_full[t], kSoftWarps / 2);   // one arrival a warp
             pipe::mbar_init(&bars->s_full[t], 1);
-            pipe::mbar_init(&bars->p_full[t], 2 * kTile);
+            pipe::mbar_init(&bars->p_full[t], kSoftWarps / 2);
             pipe::mbar_init(&bars->o_done[t], 1);
-            pipe::mbar_init(&bars->k_full[t], kConvWarps * 32);
+            pipe::mbar_init(&bars->k_full[t], kConvWarps);
             pipe::mbar_init(&bars->k_empty[t], 1);
-            pipe::mbar_init(&bars->v_full[t], kConvWarps * 32);
+            pipe::mbar_init(&bars->v_full[t], kConvWarps);
             pipe::mbar_init(&bars->v_empty[t], 1);
         }
         pipe::mbar_init(&bars->rawk_full, 8);
@@ -378,7 +378,8 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     if (c == 0) tops[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - shift) << 23);
                 }
                 pipe::async_proxy_fence();
-                pipe::mbar_arrive(&bars->q_full[t]);
+                __syncwarp();
+                if (lane == 0) pipe::mbar_arrive(&bars->q_full[t]);
             }
             named_sync(whole_tile, 2 * kTile);
             const float fac = tops[rr];
@@ -421,7 +422,8 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 l += all ? weigh64<false>(tS, sc, fac, ms, key0, pos, floor) : weigh64<true>(tS, sc, fac, ms, key0, pos, floor);
                 wait_st();
                 fence_before();
-                pipe::mbar_arrive(&bars->p_full[t]);
+                __syncwarp();
+                if (lane == 0) pipe::mbar_arrive(&bars->p_full[t]);
                 ++n_s;
             }
             if (!ok) break;
@@ -560,9 +562,11 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 sts128(kb + i * (4 * kRowsK * 128u), h[0], h[1], h[2], h[3]);
             }
             pipe::async_proxy_fence();
-            pipe::mbar_arrive(&bars->k_full[st]);
             __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bars->rawk_empty);
+            if (lane == 0) {
+                pipe::mbar_arrive(&bars->k_full[st]);
+                pipe::mbar_arrive(&bars->rawk_empty);
+            }
             ok = __all_sync(~0u, wait(&bars->rawv_full, it & 1u));
             if (!ok) break;
             if (it >= 2) ok = __all_sync(~0u, wait(&bars->v_empty[st], par ^ 1u));
@@ -593,9 +597,11 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 for (int u = 0; u < 4; ++u) sts128(dst + (v_dst[u] ^ flip), o[u][0], o[u][1], o[u][2], o[u][3]);
             }
             pipe::async_proxy_fence();
-            pipe::mbar_arrive(&bars->v_full[st]);
             __syncwarp();
-            if (lane == 0) pipe::mbar_arrive(&bars->rawv_empty);
+            if (lane == 0) {
+                pipe::mbar_arrive(&bars->v_full[st]);
+                pipe::mbar_arrive(&bars->rawv_empty);
+            }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
