@@ -207,33 +207,26 @@ __device__ __forceinline__ float weigh16(const uint32_t *s, float f, float off, 
     return sum.x + sum.y;
 }
 
-// The largest s + log2 vs of a row's 64 scores (of those it may see), 16 at a
-// time with the next 16 on their way.  Scales are not negative; NaN is passed
-// over here.
+// The largest s + log2 vs of a row's 64 scores (of those it may see).  Scales
+// are not negative; NaN is passed over here.
 template <bool MASK>
 __device__ __forceinline__ float largest64(uint32_t tS, const float4 *sc, float fac, uint32_t key0, int32_t pos, int32_t floor)
 {
-    uint32_t s[2][16];
     float top = -INFINITY;
-    tm_ld16(tS, s[0]);
 #pragma unroll 1
-    for (int c = 0; c < 2; ++c) {
+    for (int g = 0; g < 4; ++g) {
+        uint32_t s[16];
+        tm_ld16(tS + g * 16, s);
+        wait_ld();
+        if (MASK) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int g = 2 * c + u;
-            wait_ld();
-            tm_ld16(tS + (min(g + 1, 3)) * 16, s[u ^ 1]);
-            if (MASK) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int32_t key = (int32_t)key0 + g * 16 + i;
-                    if (key > pos || key <= floor) s[u][i] = 0xff800000u;   // -infinity
-                }
+            for (int i = 0; i < 16; ++i) {
+                const int32_t key = (int32_t)key0 + g * 16 + i;
+                if (key > pos || key <= floor) s[i] = 0xff800000u;   // -infinity
             }
-            top = fmaxf(top, fmaf(largest16(s[u]), fac * sc[g].x, sc[g].y));
         }
+        top = fmaxf(top, fmaf(largest16(s), fac * sc[g].x, sc[g].y));
     }
-    wait_ld();
     return top;
 }
 
@@ -242,24 +235,17 @@ __device__ __forceinline__ float largest64(uint32_t tS, const float4 *sc, float 
 template <bool MASK>
 __device__ __forceinline__ float weigh64(uint32_t tS, const float4 *sc, float fac, float ms, uint32_t key0, int32_t pos, int32_t floor)
 {
-    uint32_t s[2][16];
     float l = 0.0f;
-    tm_ld16(tS, s[0]);
 #pragma unroll 1
-    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int g = 2 * c + u;
-            uint32_t p[8];
-            wait_ld();
-            tm_ld16(tS + (min(g + 1, 3)) * 16, s[u ^ 1]);
-            const float sum = weigh16<MASK>(s[u], fac * sc[g].x, sc[g].y - ms, p, (int32_t)key0 + g * 16, pos, floor);
-            // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
-            l += MASK && sum == 0.0f ? 0.0f : sum * sc[g].z;
-            tm_st8(tS + g * 8, p);
-        }
+    for (int g = 0; g < 4; ++g) {
+        uint32_t s[16], p[8];
+        tm_ld16(tS + g * 16, s);
+        wait_ld();
+        const float sum = weigh16<MASK>(s, fac * sc[g].x, sc[g].y - ms, p, (int32_t)key0 + g * 16, pos, floor);
+        // a row that sees none of the 16 keys takes nothing from their block, whatever its scale
+        l += MASK && sum == 0.0f ? 0.0f : sum * sc[g].z;
+        tm_st8(tS + g * 8, p);
     }
-    wait_ld();
     return l;
 }
 
