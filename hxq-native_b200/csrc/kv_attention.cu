@@ -35,6 +35,8 @@
 
 #include "tc_pipe.cuh"
 
+#include <type_traits>
+
 namespace hxq {
 namespace serving {
 
@@ -506,7 +508,20 @@ bool encode_codes(CUtensorMap *map, const uint8_t *codes, const AttnArgs &a, uin
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int FMT, typename QT, int NT> cudaError_t launch_one(const AttnArgs &a, uint32_t grid, cudaStream_t s)
+// The same for both kernels' cut units: first those of this file's kernel.
+template <int D, typename QT>
+__global__ void __launch_bounds__(128) attn_join_both_kernel(const __grid_constant__ AttnArgs a, const int4 *tc_desc, const float *tc_part, uint32_t few)
+{
+    wait_previous();
+    const uint32_t warp = threadIdx.x >> 5;
+    if (blockIdx.x < few) join_row<16, kMostRows, D, QT>(a, a.desc, a.part, blockIdx.x >> 2, (blockIdx.x & 3u) * 4 + warp);
+    else {
+        const uint32_t i = blockIdx.x - few;
+        join_row<kTcRows, kTcRows, D, QT>(a, tc_desc, tc_part, i / (kTcRows / 4), i % (kTcRows / 4) * 4 + warp);
+    }
+}
+
+template <int D, int FMT, typename QT, int NT> cudaError_t launch_one(const AttnArgs &a, const AttnArgs *tc, uint32_t grid, uint32_t tc_grid, cudaStream_t s)
 {
     auto kernel = attn_mma_kernel<D, FMT, QT, NT>;
     static std::atomic<uint64_t> ready{0};
@@ -516,28 +531,40 @@ template <int D, int FMT, typename QT, int NT> cudaError_t launch_one(const Attn
     if (!encode_codes(&kmap, a.k, a, D) || !encode_codes(&vmap, a.v, a, D)) return cudaErrorInvalidValue;
     kernel<<<grid, kThreadsA, Geo<D>::kSmem, s>>>(a, kmap, vmap);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if constexpr (D != 256 && NT == 2) {
+        if (tc) {
+            // beside each other: the kernel for many rows starts with this one
+            if ((e = launch_attn_tc(*tc, D, FMT, std::is_same<QT, __half>::value ? HXQ_ELEM_F16 : HXQ_ELEM_BF16, tc_grid, s)) != cudaSuccess) return e;
+            AttnArgs both = a;
+            both.row_min = 0;
+            both.row_max = 0xffffffffu;
+            return launch_behind(attn_join_both_kernel<D, QT>, dim3(grid * 4 + tc_grid * (kTcRows / 4)), dim3(128), 0, s, both,
+                                 (const int4 *)tc->desc, (const float *)tc->part, grid * 4);
+        }
+    }
     return launch_behind(attn_join_kernel<D, QT, NT>, dim3(grid, 2 * NT), dim3(128), 0, s, a);
 }
 
-template <int D, int FMT, typename QT> cudaError_t launch_rows(const AttnArgs &a, bool few, uint32_t grid, cudaStream_t s)
+template <int D, int FMT, typename QT> cudaError_t launch_rows(const AttnArgs &a, const AttnArgs *tc, bool few, uint32_t grid, uint32_t tc_grid, cudaStream_t s)
 {
-    if constexpr (D == 256) return launch_one<D, FMT, QT, 1>(a, grid, s);   // 16 rows' accumulators would not fit
-    else return few ? launch_one<D, FMT, QT, 1>(a, grid, s) : launch_one<D, FMT, QT, 2>(a, grid, s);
+    if constexpr (D == 256) return launch_one<D, FMT, QT, 1>(a, nullptr, grid, 0, s);   // 16 rows' accumulators would not fit
+    else return few ? launch_one<D, FMT, QT, 1>(a, nullptr, grid, 0, s) : launch_one<D, FMT, QT, 2>(a, tc, grid, tc_grid, s);
 }
 
-template <int D> cudaError_t launch_dim(const AttnArgs &a, uint32_t fmt, int elem, bool few, uint32_t grid, cudaStream_t s)
+template <int D> cudaError_t launch_dim(const AttnArgs &a, const AttnArgs *tc, uint32_t fmt, int elem, bool few, uint32_t grid, uint32_t tc_grid, cudaStream_t s)
 {
     if (elem == HXQ_ELEM_BF16)
-        return fmt == HXQ_KV_INT8 ? launch_rows<D, HXQ_KV_INT8, __nv_bfloat16>(a, few, grid, s)
-                                  : launch_rows<D, HXQ_KV_E4M3, __nv_bfloat16>(a, few, grid, s);
-    return fmt == HXQ_KV_INT8 ? launch_rows<D, HXQ_KV_INT8, __half>(a, few, grid, s)
-                              : launch_rows<D, HXQ_KV_E4M3, __half>(a, few, grid, s);
+        return fmt == HXQ_KV_INT8 ? launch_rows<D, HXQ_KV_INT8, __nv_bfloat16>(a, tc, few, grid, tc_grid, s)
+                                  : launch_rows<D, HXQ_KV_E4M3, __nv_bfloat16>(a, tc, few, grid, tc_grid, s);
+    return fmt == HXQ_KV_INT8 ? launch_rows<D, HXQ_KV_INT8, __half>(a, tc, few, grid, tc_grid, s)
+                              : launch_rows<D, HXQ_KV_E4M3, __half>(a, tc, few, grid, tc_grid, s);
 }
 
-cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, bool few, uint32_t grid, cudaStream_t s)
+cudaError_t launch_attn_mma(const AttnArgs &a, const AttnArgs *tc, uint32_t D, uint32_t fmt, int elem, bool few, uint32_t grid, uint32_t tc_grid,
+                            cudaStream_t s)
 {
-    return D == 64 ? launch_dim<64>(a, fmt, elem, few, grid, s)
-                   : D == 128 ? launch_dim<128>(a, fmt, elem, few, grid, s) : launch_dim<256>(a, fmt, elem, few, grid, s);
+    return D == 64 ? launch_dim<64>(a, tc, fmt, elem, few, grid, tc_grid, s)
+                   : D == 128 ? launch_dim<128>(a, tc, fmt, elem, few, grid, tc_grid, s) : launch_dim<256>(a, tc, fmt, elem, few, grid, tc_grid, s);
 }
 
 hxq_error_t check_attention(const hxq_kv_cache_t *c, const hxq_kv_attention_t *p)
@@ -645,21 +672,20 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     // is where tiles of 16 rows read the keys four times over; that kernel
     // takes 128 rows at a time). Without rows of the other kind a launch ends
     // after its scan of the lengths.
-    if (lay.tc_ctas) a.row_max = kFewRows;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    cudaError_t e = launch_attn_mma(a, cache->head_dim, cache->format, args->elem, lay.few, lay.ctas, s);
-    if (e == cudaSuccess && lay.tc_ctas) {
-        a.row_min = kFewRows;
-        a.row_max = 0xffffffffu;
-        a.desc = reinterpret_cast<int4 *>(ws + lay.tc_desc);
-        a.part = reinterpret_cast<float *>(ws + lay.tc_part);
-        e = launch_attn_tc(a, cache->head_dim, cache->format, args->elem, lay.tc_ctas, s);
+    AttnArgs tc = a;
+    if (lay.tc_ctas) {
+        a.row_max = kFewRows;
+        tc.row_min = kFewRows;
+        tc.desc = reinterpret_cast<int4 *>(ws + lay.tc_desc);
+        tc.part = reinterpret_cast<float *>(ws + lay.tc_part);
     }
+    const cudaError_t e = launch_attn_mma(a, lay.tc_ctas ? &tc : nullptr, cache->head_dim, cache->format, args->elem, lay.few, lay.ctas,
+                                          lay.tc_ctas, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) {
         cudaGetLastError();
         return HXQ_ERR_CUDA;
     }
-    return launched(lay.tc_ctas ? 4 : 2);
+    return launched(lay.tc_ctas ? 3 : 2);
 }
 
 }  // extern "C"

@@ -439,7 +439,9 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const int4 *desc, co
 constexpr int kTcRows = 256;
 cudaError_t launch_attn_tc(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, uint32_t grid, cudaStream_t s);
 
-cudaError_t launch_attn_mma(const AttnArgs &a, uint32_t D, uint32_t fmt, int elem, bool few, uint32_t grid, cudaStream_t s);
+// tc: the arguments of the kernel for many rows, where it runs too.
+cudaError_t launch_attn_mma(const AttnArgs &a, const AttnArgs *tc, uint32_t D, uint32_t fmt, int elem, bool few, uint32_t grid, uint32_t tc_grid,
+                            cudaStream_t s);
 
 }  // namespace serving
 }  // namespace hxq

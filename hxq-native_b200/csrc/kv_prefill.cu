@@ -38,7 +38,7 @@ namespace serving {
 
 constexpr int kKeys = 128;                 // keys of a step
 constexpr int kTile = 128;                 // rows of a tile
-constexpr int kFixedT = 2;                 // steps that a unit costs by itself
+constexpr int kFixedT = 3;                 // steps that a unit costs by itself (2: prompts 390 us, 3: 355, 4: 361)
 constexpr int kSoftWarps = 16, kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps, kLoadWarp = kMmaWarp + 1, kPlanWarp = kMmaWarp + 2;
 constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups
@@ -261,9 +261,13 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t base = pipe::smem_u32(smem);
 
+    let_next_start();
     if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     Range range;
-    if (!find_range<kWarpsT, kTcRows, kKeys, kFixedT>(a, sh, reinterpret_cast<uint32_t *>(smem), false, range)) return;
+    if (!find_range<kWarpsT, kTcRows, kKeys, kFixedT>(a, sh, reinterpret_cast<uint32_t *>(smem), false, range)) {
+        wait_previous();
+        return;
+    }
     if (tid == 0) {
         for (int t = 0; t < 2; ++t) {
             pipe::mbar_init(&bars->q_full[t], kSoftWarps / 2);   // one arrival a warp
@@ -769,12 +773,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
-}
-
-template <int D, typename QT> __global__ void __launch_bounds__(128) attn_tc_join_kernel(const __grid_constant__ AttnArgs a)
-{
-    wait_previous();
-    join_row<kTcRows, kTcRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
+    wait_previous();   // the kernel for few rows, beside which this one ran: the joining kernel waits for this one alone
 }
 
 template <int D, int FMT, typename QT> cudaError_t launch_tc_one(const AttnArgs &a, uint32_t grid, cudaStream_t s)
@@ -783,9 +782,7 @@ template <int D, int FMT, typename QT> cudaError_t launch_tc_one(const AttnArgs 
     static std::atomic<uint64_t> ready{0};
     cudaError_t e = allow_smem(kernel, TcGeo<D>::kSmem, ready);
     if (e != cudaSuccess) return e;
-    kernel<<<grid, kThreadsT, TcGeo<D>::kSmem, s>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_behind(attn_tc_join_kernel<D, QT>, dim3(grid, kTcRows / 4), dim3(128), 0, s, a);
+    return launch_behind(kernel, dim3(grid), dim3(kThreadsT), TcGeo<D>::kSmem, s, a);
 }
 
 template <int D> cudaError_t launch_tc_dim(const AttnArgs &a, uint32_t fmt, int elem, uint32_t grid, cudaStream_t s)
