@@ -63,7 +63,7 @@ hxq_error_t hxq_cuda_kv_plan(const int32_t *d_new, const int32_t *d_cached, uint
 
 /* -- KV cache in 8 bits ------------------------------------------------------
  * Codes [n_blocks][n_heads][block_tokens][head_dim], 16-byte aligned, with
- * one fp32 scale per (block, head); a value is code * scale.  Filled by
+ * one fp32 scale >= 0 per (block, head); a value is code * scale.  Filled by
  * hxq_cuda_kv_append; the caller owns the memory. */
 #define HXQ_KV_INT8 0   /* -127..127, scale = max |x| / 127 */
 #define HXQ_KV_E4M3 1   /* fp8 e4m3 (finite), scale = max |x| / 448 */

@@ -747,3 +747,95 @@ def test_serving_step(H, L, cuda):
         taken = int(state["plan"].taken)
         fl.copy_(torch.cat([fl[taken:], fl[:taken]]))
         cached += 1
+
+
+# -- calls that programs make in other ways ----------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new_most", [1, 70])
+def test_attention_many_requests(cuda, new_most):
+    """Thousands of short requests, some empty: more than threads, several to a CTA."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    g = torch.Generator().manual_seed(new_most)
+    B = 2500 if new_most == 1 else 300
+    new = [new_most if i % 50 == 7 else 1 for i in range(B)]
+    lens = [int(v) if i % 11 else 0 for i, v in enumerate(torch.randint(1, 60, (B,), generator=g))]
+    lens = [max(n, m) if n else 0 for n, m in zip(lens, new)]
+    c, q, starts, sd, ld, table = _attention_case(torch, S, new, lens, 1, 2, 64, 16, "int8", "bf16", seed=new_most)
+    _check_attention(torch, S, c, q, starts, sd, ld, table, new_most)
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(cuda):
+    torch = cuda
+    from hxq_b200 import serving as S
+    cases = [_attention_case(torch, S, new, lens, 2, 4, 128, 16, fmt, "bf16", seed=s)
+             for s, (new, lens, fmt) in enumerate((([1, 1], [3000, 900], "int8"), ([300, 20], [700, 2000], "e4m3")))]
+    want = [c.attention(q, sd, ld, t, 300) for c, q, _, sd, ld, t in cases]
+    g = torch.Generator().manual_seed(1)
+    a = torch.randn((3, 16, 512), generator=g).to(torch.bfloat16).cuda()
+    b = torch.randn((3, 640, 16), generator=g).to(torch.bfloat16).cuda()
+    h = S.LoraAdapters(a, b, torch.ones(3, device="cuda"))
+    x, y = torch.randn((90, 512), generator=g).to(torch.bfloat16).cuda(), torch.randn((90, 640), generator=g).cuda()
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    starts, ids = i([0, 40, 41, 90]), i([2, -1, 0])
+    added = h.add(y, x, S.lora_plan(starts, ids, 3, 90))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], [[], [], []]
+    for _ in range(5):
+        for k, (c, q, _, sd, ld, t) in enumerate(cases):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(c.attention(q, sd, ld, t, 300))
+        with torch.cuda.stream(streams[2]):
+            got[2].append(h.add(y, x, S.lora_plan(starts, ids, 3, 90)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[k]) for k in range(2) for o in got[k]) and all(torch.equal(o, added) for o in got[2])
+
+
+@pytest.mark.gpu
+def test_lora_replayed_with_other_requests(cuda):
+    torch = cuda
+    from hxq_b200 import serving as S
+    g = torch.Generator().manual_seed(4)
+    n, R, I, O, T = 4, 24, 256, 96, 50
+    a = (torch.randn((n, R, I), generator=g) / 16).to(torch.bfloat16).cuda()
+    b, sc = torch.randn((n, O, R), generator=g).to(torch.bfloat16).cuda(), torch.ones(n, device="cuda")
+    x, y = torch.randn((T, I), generator=g).to(torch.bfloat16).cuda(), torch.randn((T, O), generator=g).cuda()
+    h = S.LoraAdapters(a, b, sc)
+    starts, ids = torch.tensor([0, 50, 50, 50], dtype=torch.int32, device="cuda"), torch.tensor([0, 0, 0], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        h.add(y, x, S.lora_plan(starts, ids, n, T))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = h.add(y, x, S.lora_plan(starts, ids, n, T))
+    for st, ad in (([0, 50, 50, 50], [0, 1, 2]), ([0, 7, 30, 50], [3, -1, 3]), ([0, 1, 2, 3], [1, 2, 0])):
+        starts.copy_(torch.tensor(st, dtype=torch.int32))
+        ids.copy_(torch.tensor(ad, dtype=torch.int32))
+        out.fill_(8.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, tol = _lora_ref(torch, y, x, a, b, sc, st, ad, I, R)
+        assert bool(((out.double() - want).abs() <= tol)[:st[-1]].all()) and bool((out[st[-1]:] == 8).all())
+
+
+@pytest.mark.gpu
+def test_empty_calls(cuda):
+    torch = cuda
+    from hxq_b200 import serving as S
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    c = S.KvCache.allocate(4, 2, 64)
+    none = torch.zeros((0, 2, 64), device="cuda")
+    c.append(none, none, i())
+    assert c.read(i())[0].shape == (0, 2, 64)
+    q = torch.zeros((0, 2, 64), dtype=torch.bfloat16, device="cuda")
+    assert c.attention(q, i(0), i(), torch.zeros((0, 1), dtype=torch.int32, device="cuda"), 1).shape == q.shape
+    q = torch.full((3, 2, 64), 2.0, dtype=torch.bfloat16, device="cuda")
+    out = q.clone()
+    c.attention(q, i(0, 0, 0), i(5, 0), torch.zeros((2, 1), dtype=torch.int32, device="cuda"), 1, out=out)   # no rows of any request
+    assert bool((out == 2).all())
+    h = S.LoraAdapters(torch.zeros((1, 8, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((1, 32, 8), dtype=torch.bfloat16, device="cuda"),
+                       torch.ones(1, device="cuda"))
+    assert h.add(torch.zeros((0, 32), device="cuda"), torch.zeros((0, 64), dtype=torch.bfloat16, device="cuda"), S.lora_plan(i(0), i(), 1, 0)).shape == (0, 32)
