@@ -430,8 +430,9 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128, KS == 8 ? 2 
                 for (int w = 0; w < 2; ++w) {
                     const __nv_bfloat162 top = __floats2bfloat162_rn(f[2 * w], f[2 * w + 1]);
                     const float2 back = __bfloat1622float2(top);
-                    f[2 * w] -= back.x;
-                    f[2 * w + 1] -= back.y;
+                    // (nothing is left of an infinity)
+                    f[2 * w] = fabsf(back.x) <= 3.402823466e38f ? f[2 * w] - back.x : 0.0f;
+                    f[2 * w + 1] = fabsf(back.y) <= 3.402823466e38f ? f[2 * w + 1] - back.y : 0.0f;
                     w3[part][w * 2 + r] = *reinterpret_cast<const uint32_t *>(&top);
                 }
         }

@@ -839,3 +839,28 @@ def test_empty_calls(cuda):
     h = S.LoraAdapters(torch.zeros((1, 8, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((1, 32, 8), dtype=torch.bfloat16, device="cuda"),
                        torch.ones(1, device="cuda"))
     assert h.add(torch.zeros((0, 32), device="cuda"), torch.zeros((0, 64), dtype=torch.bfloat16, device="cuda"), S.lora_plan(i(0), i(), 1, 0)).shape == (0, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [8, 32])
+def test_lora_infinity(cuda, R):
+    # an infinity in a row of x gives that row infinities (NaN where B is
+    # zero), as the formula does, and nothing in another row
+    torch = cuda
+    from hxq_b200 import serving as S
+    T, I, O = 5, 64, 24
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.randn(T, I, device="cuda", generator=g).bfloat16()
+    x[2, 5] = float("inf")
+    a = torch.rand(1, R, I, device="cuda", generator=g).bfloat16() + 1
+    b = torch.rand(1, O, R, device="cuda", generator=g).bfloat16() + 1
+    b[0, 3] = 0
+    b[0, 7] = -b[0, 7]
+    y = torch.zeros(T, O, device="cuda")
+    starts = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    ids = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = S.LoraAdapters(a, b, torch.ones(1, device="cuda")).add(y, x, S.lora_plan(starts, ids, 1, T))
+    want = (x.double() @ a[0].double().T) @ b[0].double().T
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and bool(torch.isnan(out[2, 3]))
+    assert bool((out[2][torch.isinf(want[2])] == want[2][torch.isinf(want[2])].float()).all())
+    assert bool(torch.isfinite(out[[0, 1, 3, 4]]).all())
