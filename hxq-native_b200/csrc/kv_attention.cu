@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
 template <int D, typename QT, int NT> __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a)
 {
     wait_previous();
-    join_row<8 * NT, kMostRows, D, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
+    join_row<8 * NT, kMostRows, D, D == 256 ? 4 : 8, QT>(a, a.desc, a.part, blockIdx.x, blockIdx.y * 4 + (threadIdx.x >> 5));
 }
 
 // The codes as rows of D bytes, in boxes of 16 rows of 128 (64) bytes.
@@ -514,10 +514,10 @@ __global__ void __launch_bounds__(128) attn_join_both_kernel(const __grid_consta
 {
     wait_previous();
     const uint32_t warp = threadIdx.x >> 5;
-    if (blockIdx.x < few) join_row<16, kMostRows, D, QT>(a, a.desc, a.part, blockIdx.x >> 2, (blockIdx.x & 3u) * 4 + warp);
+    if (blockIdx.x < few) join_row<16, kMostRows, D, 4, QT>(a, a.desc, a.part, blockIdx.x >> 2, (blockIdx.x & 3u) * 4 + warp);
     else {
         const uint32_t i = blockIdx.x - few;
-        join_row<kTcRows, kTcRows, D, QT>(a, tc_desc, tc_part, i / (kTcRows / 4), i % (kTcRows / 4) * 4 + warp);
+        join_row<kTcRows, kTcRows, D, 4, QT>(a, tc_desc, tc_part, i / (kTcRows / 4), i % (kTcRows / 4) * 4 + warp);
     }
 }
 

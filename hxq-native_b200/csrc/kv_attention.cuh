@@ -375,45 +375,70 @@ template <int ROWS, int D> __host__ __device__ constexpr size_t part_floats() { 
 // second slot, then the first slots of the CTAs behind it, in order.  A warp
 // takes row rr of the unit's tile of ROWS (SLOT rows a slot); a lane looks
 // after the weight of a part.
-template <int ROWS, int SLOT, int D, typename QT>
+template <int ROWS, int SLOT, int D, int AHEAD, typename QT>
 __device__ __forceinline__ void join_row(const AttnArgs &a, const int4 *desc, const float *parts, uint32_t cta, uint32_t rr)
 {
     const int4 d = desc[cta];
     if (d.x == 0) return;
     constexpr size_t kPart = part_floats<SLOT, D>();
+    constexpr int N = D / 32;
     const uint32_t lane = threadIdx.x & 31;
     const float *first = parts + (2 * (size_t)cta + 1) * kPart, *rest = parts + 2 * (size_t)cta * kPart;
     auto part = [&](int i) { return i == 0 ? first : rest + (size_t)i * 2 * kPart; };
-    // a first batch of sums while the weights are found
-    constexpr int N = D / 32, kAhead = 8;
-    float v[N], u[kAhead][N], sum = 0.0f, top = -INFINITY;
+    float v[N], u[AHEAD][N], sum = 0.0f;
+    auto fetch = [&](int i0) {   // sums of AHEAD parts, N consecutive dimensions a lane
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
+        for (int i = 0; i < AHEAD; ++i) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) u[i][j] = i < d.x ? part(i)[rr * D + j * 32 + lane] : 0.0f;
-    for (int i = lane; i < d.x; i += 32) top = fmaxf(top, part(i)[SLOT * D + rr]);
+            for (int j = 0; j < N; ++j) u[i][j] = 0.0f;
+            if (i0 + i < d.x) {
+                const float *p = part(i0 + i) + rr * D + lane * N;
+                if constexpr (N == 2) {
+                    const float2 f = *reinterpret_cast<const float2 *>(p);
+                    u[i][0] = f.x;
+                    u[i][1] = f.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < N; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4 *>(p + j);
+                        u[i][j] = f.x;
+                        u[i][j + 1] = f.y;
+                        u[i][j + 2] = f.z;
+                        u[i][j + 3] = f.w;
+                    }
+                }
+            }
+        }
+    };
+    // one latency for all of it: the first parts, their maxima and sums, the
+    // request
+    fetch(0);
+    float t0 = -INFINITY, s0 = 0.0f;
+    if ((int)lane < d.x) {
+        const float *p = part(lane) + SLOT * D + rr;
+        t0 = p[0];
+        s0 = p[SLOT];
+    }
+    const Req r = load_req(a, (uint32_t)d.y);
+    float top = t0;
+    for (int i = lane + 32; i < d.x; i += 32) top = fmaxf(top, part(i)[SLOT * D + rr]);
 #pragma unroll
     for (int m = 16; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, m));
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = 0.0f;
     for (int i0 = 0; i0 < d.x; i0 += 32) {
-        float w = 0.0f, s = 0.0f;
-        if (i0 + (int)lane < d.x) {
+        if (i0 > 0 && i0 + (int)lane < d.x) {
             const float *p = part(i0 + lane) + SLOT * D + rr;
-            w = top == -INFINITY ? 1.0f : ex2(p[0] - top);
-            s = p[SLOT];
+            t0 = p[0];
+            s0 = p[SLOT];
         }
+        const float w = top == -INFINITY ? 1.0f : ex2(t0 - top);
 #pragma unroll 1
-        for (int k = 0; k < min(32, d.x - i0); k += kAhead) {
-            if (i0 + k > 0) {
+        for (int k = 0; k < min(32, d.x - i0); k += AHEAD) {
+            if (i0 + k > 0) fetch(i0 + k);
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-                    for (int j = 0; j < N; ++j) u[i][j] = i0 + k + i < d.x ? part(i0 + k + i)[rr * D + j * 32 + lane] : 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                const float wi = __shfl_sync(~0u, w, k + i), si = __shfl_sync(~0u, s, k + i);
+            for (int i = 0; i < AHEAD; ++i) {
+                const float wi = __shfl_sync(~0u, w, k + i), si = __shfl_sync(~0u, s0, k + i);
                 if (i0 + k + i < d.x) {
                     sum += si * wi;
 #pragma unroll
@@ -422,14 +447,22 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const int4 *desc, co
             }
         }
     }
-    const Req r = load_req(a, (uint32_t)d.y);
     const uint32_t row = (uint32_t)d.w * ROWS + rr;
     if (row >= r.rows) return;
     const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
     const uint32_t tk = token_of(a, row), tok = r.q0 + tk, head = (uint32_t)d.z * a.G + (row - tk * a.G);
-    QT *dst = static_cast<QT *>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh;
+    QT *dst = static_cast<QT *>(a.out) + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + lane * N;
+    __align__(16) QT o[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) dst[j * 32 + lane] = Elem<QT>::from(v[j] * f);
+    for (int j = 0; j < N; ++j) o[j] = Elem<QT>::from(v[j] * f);
+    if (((uintptr_t)dst & (N * 2 - 1)) == 0) {
+        if constexpr (N == 2) *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(o);
+        else if constexpr (N == 4) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(o);
+        else *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) dst[j] = o[j];
+    }
     if (a.lse && lane == 0)
         a.lse[(size_t)tok * a.Hq + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
