@@ -14,7 +14,8 @@ namespace serving {
 // itself, so no CTA reads what another one writes and one launch does it all:
 // every CTA sums the lengths (8 bytes a request out of L2, a block scan) and
 // then fills its own part of the slot map and of the table.  Bound by the
-// launch and two dependent loads, not by bytes.
+// launch and two dependent loads, not by bytes: 8.5 us a call for 64 decoding
+// requests and 8.3 for 500 prompts of up to 1024 tokens.
 
 constexpr int kPlanThreads = 512;
 
@@ -138,7 +139,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
 // and, when the scale grew, round the block's other codes to the new one.  A
 // lane keeps up to 8 pieces of 8 values between the two looks at a run, G
 // chosen so that a whole block's rows fit (blocks beyond 8 warps' worth are
-// read again, out of L2).  Bound by the bytes of the rows.
+// read again, out of L2).  Bound by the latency of a run (slots, then rows,
+// then codes, with no more warps an SM than the held pieces' registers allow;
+// fewer registers spill and cost more): 79 us for 9 prompts of up to 2048 rows,
+// 32 heads of 128, bf16 to e4m3, where the bytes take 36.  Rows read
+// twice instead of held: 149 us with the read-back against 130.
 //
 // Magnitudes are compared as the integers of their bits (non-negative floats
 // order like integers, NaN above all), so infinities and NaN reach the scale.
@@ -371,7 +376,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, sizeof(T) == 4 ? 2 : 3) app
 }
 
 // Read-back: a thread takes 16 consecutive codes of k or v, a CTA whole
-// tokens, four of a thread's pieces under way.
+// tokens, four of a thread's pieces under way.  Bound by memory: 48 us for the
+// rows of the append above (e4m3 to bf16), where the bytes take 36.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) read_kernel(const hxq_kv_cache_t c, const int32_t *slots, uint32_t n_tokens, T *k, T *v, uint32_t *status)
 {
