@@ -141,9 +141,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a)
 // chosen so that a whole block's rows fit (blocks beyond 8 warps' worth are
 // read again, out of L2).  Bound by the latency of a run (slots, then rows,
 // then codes, with no more warps an SM than the held pieces' registers allow;
-// fewer registers spill and cost more): 79 us for 9 prompts of up to 2048 rows,
+// fewer registers spill and cost more; half the pieces with twice the
+// warps a run: 140 us for both kernels): 77 us for 9 prompts of up to 2048 rows,
 // 32 heads of 128, bf16 to e4m3, where the bytes take 36.  Rows read
-// twice instead of held: 149 us with the read-back against 130.
+// twice instead of held: 149 us with the read-back against 130, 128 with the next
+// run's rows brought to L2 while this one's are looked at.
 //
 // Magnitudes are compared as the integers of their bits (non-negative floats
 // order like integers, NaN above all), so infinities and NaN reach the scale.
@@ -322,6 +324,15 @@ __global__ void __launch_bounds__(kAppendWarps * 32, sizeof(T) == 4 ? 2 : 3) app
 #pragma unroll
             for (int i = 0; i < kHeld; ++i)
                 if (e0 + i * (32 * G) < pieces) held[i] = load_piece<T, VEC>(row_at(e0 + i * (32 * G)));
+            // the rows behind them on their way to L2 meanwhile
+            {
+                constexpr uint32_t kLine = 128 / sizeof(T);
+                const uint32_t per = a.D / kLine, lgl = per == 1 ? 0 : per == 2 ? 1 : per == 4 ? 2 : 3;
+                for (uint32_t e = e0; e < a.P << lgl; e += 32 * G) {
+                    const uint32_t u = t + len + (e >> lgl);
+                    if (u < t_end) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + (int64_t)u * st + (e & (per - 1)) * kLine));
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kHeld; ++i)
                 if (e0 + i * (32 * G) < pieces) look(held[i]);
