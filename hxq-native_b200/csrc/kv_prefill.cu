@@ -20,8 +20,10 @@
 //               warp for keys and one for values;
 //   warp 22     one thread cuts the CTA's range into segments for the others.
 // The two tiles take turns: while one is at its exponentials, the tensor
-// cores work for the other.  Tensor memory: S/P of tile t at column 128 t,
-// O of tile t at 256 + 128 t, all 512 columns, one CTA an SM.
+// cores work for the other.  Tensor memory, all 512 columns, one CTA an SM:
+// heads of 128 have a buffer of 128 scores for each tile and two accumulators,
+// heads of 64 a third buffer, so that the next scores of a tile are computed
+// while it is at these (chunks below 115 -> 106 us).
 //
 // The running maximum is lazy: it is raised, and O rescaled, only where a
 // weight would pass 2^8 (f16 holds 2^16), which after the first keys is rare,
@@ -31,10 +33,10 @@
 // weights back, the next scores behind the weights' product (about 4,900 cycles
 // a step of two tiles, where the tensor pipe needs 2,060, the exponentials
 // 2,050 and the conversion's shared memory traffic about 2,500).  Three prompts
-// of up to 4096 rows, 32 heads of 128, int8: 368 us a call, 656 TFLOP/s (38% of
+// of up to 4096 rows, 32 heads of 128, int8: 358 us a call, 673 TFLOP/s (39% of
 // the measured matrix rate; tensor pipe active 34% of the time, instructions
 // issued in 61% of the cycles); two chunks of 512 rows x 40 heads of 64 over a
-// window of 4096 keys, e4m3: 115 us.  A second issuing warp, one a
+// window of 4096 keys, e4m3: 106 us.  A second issuing warp, one a
 // tile, cost (462 -> 490 us at the time).
 //
 // Work is cut and joined as in kv_attention.cu, with granules of 128 keys.
@@ -56,7 +58,7 @@ constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups
 // 16 scores and the next 16. 512 x 88 + 128 x 64 + 128 x 64 = 61,440.
 constexpr int kRegsSoft = 88, kRegsConv = 64, kRegsRest = 64;
 constexpr int kThreadsT = kWarpsT * 32;
-constexpr int kScaleSlots = 4, kSegSlots = 2;
+constexpr int kSegSlots = 2;
 constexpr float kRaise = 8.0f;             // log2 of the largest weight before the maximum is raised
 
 template <int D> struct TcGeo {
@@ -64,6 +66,10 @@ template <int D> struct TcGeo {
     static constexpr int kK = kKeys * D * 2;           // of a step's keys, and of its values
     static constexpr int kRaw = kKeys * D;             // bytes of their codes
     static constexpr int kOffK = 2 * kQ, kOffV = kOffK + 2 * kK, kOffRaw = kOffV + 2 * kK, kOffS = kOffRaw + 2 * kRaw;
+    // Buffers of scores: one a tile, and one more where heads of 64 leave the
+    // columns for it: then the scores of a tile's next step are there when it
+    // is done with this one's. Their steps' scales are kept that much longer.
+    static constexpr int kBufs = D == 64 ? 3 : 2, kScaleSlots = D == 64 ? 8 : 4, kColO = 128 * kBufs;
     static constexpr int kOffSeg = kOffS + kScaleSlots * 8 * 16, kOffBar = kOffSeg + kSegSlots * 64;
     static constexpr int kOffTop = kOffBar + 320;      // a float for every row of both tiles and halves
     static constexpr int kSmem = kOffTop + 2 * 2 * kTile * 4;
@@ -146,7 +152,7 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 }
 
 struct Bars {
-    uint64_t q_full[2], s_full[2], p_full[2], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_full[2], s_full[3], p_full[3], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t rawk_full, rawk_empty, rawv_full, rawv_empty, seg_full[kSegSlots], seg_empty[kSegSlots], drained;
     uint32_t tmem;
     uint32_t live[2], zero[2][8];   // of a raw step (by its parity): keys within the range (0: no more steps), value groups that count as 0
@@ -281,13 +287,15 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
     if (tid == 0) {
         for (int t = 0; t < 2; ++t) {
             pipe::mbar_init(&bars->q_full[t], kSoftWarps / 2);   // one arrival a warp
-            pipe::mbar_init(&bars->s_full[t], 1);
-            pipe::mbar_init(&bars->p_full[t], kSoftWarps / 2);
             pipe::mbar_init(&bars->o_done[t], 1);
             pipe::mbar_init(&bars->k_full[t], kConvWarps);
             pipe::mbar_init(&bars->k_empty[t], 1);
             pipe::mbar_init(&bars->v_full[t], kConvWarps);
             pipe::mbar_init(&bars->v_empty[t], 1);
+        }
+        for (int b = 0; b < 3; ++b) {
+            pipe::mbar_init(&bars->s_full[b], 1);
+            pipe::mbar_init(&bars->p_full[b], kSoftWarps / 2);
         }
         pipe::mbar_init(&bars->rawk_full, 8);
         pipe::mbar_init(&bars->rawk_empty, kConvWarps);
@@ -315,21 +323,24 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoft));
         const uint32_t t = warp >> 3, hf = warp >> 2 & 1u, rr = tid & (kTile - 1);   // tile, half of the keys, row of the tile
         const uint32_t lanes = (warp & 3u) << 21;                      // this warp's 32 lanes of tensor memory
-        const uint32_t tS = tmem + lanes + t * 128u + hf * 64u;
-        const uint32_t tO = tmem + lanes + 256u + t * 128u + hf * (D / 2);
+        const uint32_t tS0 = tmem + lanes + hf * 64u;
+        const uint32_t tO = tmem + lanes + G::kColO + t * D + hf * (D / 2);
         const uint32_t pair = 1 + t * 4 + (warp & 3u), whole_tile = 9 + t;           // named barriers: 64 and 256 threads
         float *tops = reinterpret_cast<float *>(smem + G::kOffTop) + t * 2 * kTile;
         const uint32_t qt = base + t * G::kQ;
         uint32_t n_s = 0;                                              // steps of this tile so far
-        uint32_t step0 = 0;                                            // CTA's steps before this segment
+        uint32_t step0 = 0, use0 = 0;                                  // CTA's steps, and tiles' steps, before this segment
         for (uint32_t si = 0;; ++si) {
             const SegInfo &seg = segs[si % kSegSlots];
             ok = __all_sync(~0u, wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u));
             if (!ok || seg.take == 0) break;
             const uint32_t take = t == 0 ? seg.take0 : seg.take, key_first = seg.key0;
             const uint32_t tr0 = seg.r0 + t * kTile, r1 = seg.r1;
+            const bool two = r1 - seg.r0 > (uint32_t)kTile;
+            const uint32_t both = two ? seg.take0 : 0;                 // steps that both tiles take part in
             if (tr0 >= r1) {
                 step0 += seg.take;
+                use0 += seg.take;
                 __syncwarp();
                 if (lane == 0) pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
                 continue;
@@ -387,10 +398,13 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             float M = -INFINITY, l = 0.0f;
             for (uint32_t j = 0; j < take; ++j) {
                 const uint32_t key0 = key_first + j * kKeys + hf * 64u;
-                ok = __all_sync(~0u, wait(&bars->s_full[t], n_s & 1u));
+                // buffer and its turn: a tile's own, or all in the order of the products
+                const uint32_t use = use0 + (j < both ? 2 * j + t : both + j);
+                const uint32_t buf = G::kBufs == 2 ? t : use % 3u, turn = G::kBufs == 2 ? n_s : use / 3u, tS = tS0 + buf * 128u;
+                ok = __all_sync(~0u, wait(&bars->s_full[buf], turn & 1u));
                 if (!ok) break;
                 fence_after();
-                const float4 *sc = scales + ((step0 + j) & (kScaleSlots - 1)) * 8 + hf * 4;
+                const float4 *sc = scales + ((step0 + j) & (G::kScaleSlots - 1)) * 8 + hf * 4;
                 const bool all = (int32_t)(key0 + 63) <= pos_first && (int32_t)key0 > floor_last;
                 float top = all ? largest64<false>(tS, sc, fac, key0, pos, floor) : largest64<true>(tS, sc, fac, key0, pos, floor);
                 // and of the other half's
@@ -423,11 +437,12 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) pipe::mbar_arrive(&bars->p_full[t]);
+                if (lane == 0) pipe::mbar_arrive(&bars->p_full[buf]);
                 ++n_s;
             }
             if (!ok) break;
             step0 += seg.take;
+            use0 += both + seg.take;
             ok = __all_sync(~0u, wait(&bars->o_done[t], (n_s - 1) & 1u));
             if (!ok) break;
             fence_after();
@@ -656,7 +671,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     if (it >= 1) ok = wait(raw_empty, (it - 1) & 1u);
                     if (!ok) break;
                     if (keys) {
-                        scales[(it & (kScaleSlots - 1)) * 8 + lane] = b;
+                        scales[(it & (G::kScaleSlots - 1)) * 8 + lane] = b;
                         if (lane == 0) bars->live[it & 1u] = min((uint32_t)kKeys, seg.hi > key0 ? seg.hi - key0 : 1u);
                     } else bars->zero[it & 1u][lane] = zero;
                     if (in) {
@@ -720,17 +735,9 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         } else if (warp == kMmaWarp) {
         const uint32_t one = elect_one();
         // ------------------------------------------------------- products
-        uint32_t it = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
+        uint32_t it = 0, use0 = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
         // descriptors address 16-byte units
         const uint64_t q_desc = desc_sw128(base), k_desc = desc_sw128(base + G::kOffK), v_desc = desc_sw128(base + G::kOffV);
-        auto qk = [&](uint32_t t, uint32_t st) {
-            const uint64_t qa = q_desc + t * (G::kQ >> 4), kb = k_desc + st * (G::kK >> 4);
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-                tc_mma_ss(one, tmem + t * 128u, qa + ((kk >> 2) * (kTile * 8) + (kk & 3) * 2), kb + ((kk >> 2) * (kKeys * 8) + (kk & 3) * 2),
-                          G::kIdescQK, kk != 0);
-            tc_commit(one, &bars->s_full[t]);
-        };
         for (uint32_t si = 0; ok; ++si) {
             ok = __all_sync(~0u, wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u));
             if (!ok) break;
@@ -739,33 +746,54 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             __syncwarp();
             if (one) pipe::mbar_arrive(&bars->seg_empty[si % kSegSlots]);
             if (take == 0) break;
-            ok = __all_sync(~0u, wait(&bars->k_full[it & 1u], (it >> 1) & 1u));
-            for (uint32_t t = 0; ok && t < tiles; ++t) {
-                ok = __all_sync(~0u, wait(&bars->q_full[t], n_q[t]++ & 1u));
+            // the tiles' steps in order: both tiles' while tile 0 has any, then one tile's
+            const uint32_t both = tiles == 2 ? take0 : 0, uses = both + take;
+            auto tile_of = [&](uint32_t u) { return u < 2 * both ? u & 1u : tiles - 1; };
+            auto step_of = [&](uint32_t u) { return u < 2 * both ? u >> 1 : u - both; };
+            uint32_t keys = 0, queries = 0;   // steps and tiles whose operands are there
+            auto qk = [&](uint32_t t, uint32_t j, uint32_t buf) {
+                const uint32_t st = (it + j) & 1u;
+                if (j >= keys) {
+                    ok = __all_sync(~0u, wait(&bars->k_full[st], ((it + j) >> 1) & 1u));
+                    keys = j + 1;
+                }
+                if (ok && !(queries >> t & 1u)) {
+                    ok = __all_sync(~0u, wait(&bars->q_full[t], n_q[t]++ & 1u));
+                    queries |= 1u << t;
+                }
+                if (!ok) return;
+                fence_after();
+                const uint64_t qa = q_desc + t * (G::kQ >> 4), kb = k_desc + st * (G::kK >> 4);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                    tc_mma_ss(one, tmem + buf * 128u, qa + ((kk >> 2) * (kTile * 8) + (kk & 3) * 2), kb + ((kk >> 2) * (kKeys * 8) + (kk & 3) * 2),
+                              G::kIdescQK, kk != 0);
+                tc_commit(one, &bars->s_full[buf]);
+                if (t == 1 || j >= both) tc_commit(one, &bars->k_empty[st]);   // the step's last
+            };
+            for (uint32_t v = 0; ok && v < (uint32_t)G::kBufs && v < uses; ++v) {
+                if (G::kBufs == 3) qk(tile_of(v), step_of(v), (use0 + v) % 3u);
+                else if (v < tiles) qk(v, 0, v);
+            }
+            for (uint32_t u = 0; ok && u < uses; ++u) {
+                const uint32_t t = tile_of(u), j = step_of(u), st = (it + j) & 1u;
+                const uint32_t buf = G::kBufs == 2 ? t : (use0 + u) % 3u, turn = G::kBufs == 2 ? n_p[t]++ : (use0 + u) / 3u;
+                ok = __all_sync(~0u, ((t == 1 && j < both) || wait(&bars->v_full[st], ((it + j) >> 1) & 1u)) && wait(&bars->p_full[buf], turn & 1u));
                 if (!ok) break;
                 fence_after();
-                qk(t, it & 1u);
-            }
-            if (!ok) break;
-            tc_commit(one, &bars->k_empty[it & 1u]);
-            for (uint32_t j = 0; ok && j < take; ++j, ++it) {
-                const uint32_t st = it & 1u, sn = (it + 1) & 1u;
-                ok = __all_sync(~0u, wait(&bars->v_full[st], (it >> 1) & 1u) && (j + 1 >= take || wait(&bars->k_full[sn], ((it + 1) >> 1) & 1u)));
-                for (uint32_t t = j < take0 ? 0 : 1; ok && t < tiles; ++t) {
-                    ok = __all_sync(~0u, wait(&bars->p_full[t], n_p[t]++ & 1u));
-                    if (!ok) break;
-                    fence_after();
-                    const uint64_t vb = v_desc + st * (G::kK >> 4);
+                const uint64_t vb = v_desc + st * (G::kK >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < kKeys / 16; ++kk)
-                        tc_mma_ts(one, tmem + 256u + t * 128u, tmem + t * 128u + (kk >> 2) * 64u + (kk & 3) * 8u, vb + ((kk >> 2) * (D * 8) + (kk & 3) * 2),
-                                  G::kIdescPV, (j | kk) != 0);
-                    tc_commit(one, &bars->o_done[t]);
-                    if (j + 1 < (t == 0 ? take0 : take)) qk(t, sn);
-                }
-                if (ok) tc_commit(one, &bars->v_empty[st]);
-                if (ok && j + 1 < take) tc_commit(one, &bars->k_empty[sn]);
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                    tc_mma_ts(one, tmem + G::kColO + t * D, tmem + buf * 128u + (kk >> 2) * 64u + (kk & 3) * 8u, vb + ((kk >> 2) * (D * 8) + (kk & 3) * 2),
+                              G::kIdescPV, (j | kk) != 0);
+                tc_commit(one, &bars->o_done[t]);
+                if (t == 1 || j >= both) tc_commit(one, &bars->v_empty[st]);   // the step's last
+                if (G::kBufs == 3) {
+                    if (u + 3 < uses) qk(tile_of(u + 3), step_of(u + 3), buf);
+                } else if (j + 1 < (t == 0 ? take0 : take)) qk(t, j + 1, t);
             }
+            it += take;
+            use0 += uses;
         }
         if (!ok) {
             // unwinding: the products in flight end before their memory is given back
