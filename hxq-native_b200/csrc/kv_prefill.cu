@@ -33,7 +33,7 @@
 // weights back, the next scores behind the weights' product (about 4,900 cycles
 // a step of two tiles, where the tensor pipe needs 2,060, the exponentials
 // 2,050 and the conversion's shared memory traffic about 2,500).  Three prompts
-// of up to 4096 rows, 32 heads of 128, int8: 358 us a call, 673 TFLOP/s (39% of
+// of up to 4096 rows, 32 heads of 128, int8: 358-364 us a call, 663 TFLOP/s (39% of
 // the measured matrix rate; tensor pipe active 34% of the time, instructions
 // issued in 61% of the cycles); two chunks of 512 rows x 40 heads of 64 over a
 // window of 4096 keys, e4m3: 106 us.  A second issuing warp, one a
