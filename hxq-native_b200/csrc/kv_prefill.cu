@@ -23,7 +23,7 @@
 // cores work for the other.  Tensor memory, all 512 columns, one CTA an SM:
 // heads of 128 have a buffer of 128 scores for each tile and two accumulators,
 // heads of 64 a third buffer, so that the next scores of a tile are computed
-// while it is at these (chunks below 115 -> 106 us).
+// while it is at these (chunks below 115 -> 107 us).
 //
 // The running maximum is lazy: it is raised, and O rescaled, only where a
 // weight would pass 2^8 (f16 holds 2^16), which after the first keys is rare,
@@ -33,10 +33,10 @@
 // weights back, the next scores behind the weights' product (about 4,900 cycles
 // a step of two tiles, where the tensor pipe needs 2,060, the exponentials
 // 2,050 and the conversion's shared memory traffic about 2,500).  Three prompts
-// of up to 4096 rows, 32 heads of 128, int8: 358-364 us a call, 663 TFLOP/s (39% of
+// of up to 4096 rows, 32 heads of 128, int8: 366 us a call, 659 TFLOP/s (38% of
 // the measured matrix rate; tensor pipe active 34% of the time, instructions
 // issued in 61% of the cycles); two chunks of 512 rows x 40 heads of 64 over a
-// window of 4096 keys, e4m3: 106 us.  A second issuing warp, one a
+// window of 4096 keys, e4m3: 107 us.  A second issuing warp, one a
 // tile, cost (462 -> 490 us at the time).
 //
 // Work is cut and joined as in kv_attention.cu, with granules of 128 keys.
@@ -152,7 +152,7 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 }
 
 struct Bars {
-    uint64_t q_full[2], s_full[3], p_full[3], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_full[2], s_full[2][3], p_full[3], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t rawk_full, rawk_empty, rawv_full, rawv_empty, seg_full[kSegSlots], seg_empty[kSegSlots], drained;
     uint32_t tmem;
     uint32_t live[2], zero[2][8];   // of a raw step (by its parity): keys within the range (0: no more steps), value groups that count as 0
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             pipe::mbar_init(&bars->v_empty[t], 1);
         }
         for (int b = 0; b < 3; ++b) {
-            pipe::mbar_init(&bars->s_full[b], 1);
+            for (int t = 0; t < 2; ++t) pipe::mbar_init(&bars->s_full[t][b], 1);
             pipe::mbar_init(&bars->p_full[b], kSoftWarps / 2);
         }
         pipe::mbar_init(&bars->rawk_full, 8);
@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         float *tops = reinterpret_cast<float *>(smem + G::kOffTop) + t * 2 * kTile;
         const uint32_t qt = base + t * G::kQ;
         uint32_t n_s = 0;                                              // steps of this tile so far
+        uint32_t turns = 0;                                            // of each buffer's barrier, as a parity
         uint32_t step0 = 0, use0 = 0;                                  // CTA's steps, and tiles' steps, before this segment
         for (uint32_t si = 0;; ++si) {
             const SegInfo &seg = segs[si % kSegSlots];
@@ -398,11 +399,13 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             float M = -INFINITY, l = 0.0f;
             for (uint32_t j = 0; j < take; ++j) {
                 const uint32_t key0 = key_first + j * kKeys + hf * 64u;
-                // buffer and its turn: a tile's own, or all in the order of the products
+                // The buffer: the tile's own, or all in the order of the products. Its barrier is one of this tile alone:
+                // a tile that a segment does not have is several turns of the buffers ahead, of its own barriers none.
                 const uint32_t use = use0 + (j < both ? 2 * j + t : both + j);
-                const uint32_t buf = G::kBufs == 2 ? t : use % 3u, turn = G::kBufs == 2 ? n_s : use / 3u, tS = tS0 + buf * 128u;
-                ok = __all_sync(~0u, wait(&bars->s_full[buf], turn & 1u));
+                const uint32_t buf = G::kBufs == 2 ? t : use % 3u, tS = tS0 + buf * 128u;
+                ok = __all_sync(~0u, wait(&bars->s_full[t][buf], turns >> buf & 1u));
                 if (!ok) break;
+                turns ^= 1u << buf;
                 fence_after();
                 const float4 *sc = scales + ((step0 + j) & (G::kScaleSlots - 1)) * 8 + hf * 4;
                 const bool all = (int32_t)(key0 + 63) <= pos_first && (int32_t)key0 > floor_last;
@@ -768,7 +771,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 for (int kk = 0; kk < D / 16; ++kk)
                     tc_mma_ss(one, tmem + buf * 128u, qa + ((kk >> 2) * (kTile * 8) + (kk & 3) * 2), kb + ((kk >> 2) * (kKeys * 8) + (kk & 3) * 2),
                               G::kIdescQK, kk != 0);
-                tc_commit(one, &bars->s_full[buf]);
+                tc_commit(one, &bars->s_full[t][buf]);
                 if (t == 1 || j >= both) tc_commit(one, &bars->k_empty[st]);   // the step's last
             };
             for (uint32_t v = 0; ok && v < (uint32_t)G::kBufs && v < uses; ++v) {

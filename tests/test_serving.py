@@ -864,3 +864,19 @@ def test_lora_infinity(cuda, R):
     assert torch.equal(torch.isnan(out), torch.isnan(want)) and bool(torch.isnan(out[2, 3]))
     assert bool((out[2][torch.isinf(want[2])] == want[2][torch.isinf(want[2])].float()).all())
     assert bool(torch.isfinite(out[[0, 1, 3, 4]]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,lens,heads,group,window,causal", [
+    ([100], [1500], 2, 1, 0, True),                                  # one tile of rows, many steps
+    ([129, 257, 300, 65], [129, 2000, 5000, 4000], 4, 1, 0, True),   # two tiles, the second with fewer rows
+    ([300, 90], [2500, 90], 8, 5, 700, True),
+    ([300, 100], [900, 1000], 2, 3, 0, False),
+    ([150, 70] * 12, [400, 130] * 12, 8, 1, 0, True),                # many units a CTA, of one tile and of two
+])
+def test_attention_tiles_of_rows(cuda, dim, new, lens, heads, group, window, causal):
+    torch = cuda
+    from hxq_b200 import serving as S
+    c, q, starts, sd, ld, table = _attention_case(torch, S, new, lens, heads, group, dim, 32, "e4m3", "bf16", seed=len(new))
+    _check_attention(torch, S, c, q, starts, sd, ld, table, max(new), window, causal)
