@@ -71,8 +71,13 @@ template <int D> struct TcGeo {
     // is done with this one's. Their steps' scales are kept that much longer.
     static constexpr int kBufs = D == 64 ? 3 : 2, kScaleSlots = D == 64 ? 8 : 4, kColO = 128 * kBufs;
     static constexpr int kOffSeg = kOffS + kScaleSlots * 8 * 16, kOffBar = kOffSeg + kSegSlots * 64;
-    static constexpr int kOffTop = kOffBar + 320;      // a float for every row of both tiles and halves
-    static constexpr int kSmem = kOffTop + 2 * 2 * kTile * 4;
+    // A float for every row of both tiles and halves, in which the two warps of a row exchange their maxima. Two of them,
+    // taken in turn, where a tile's next scores may be there before both warps are done with this step's: a warp then
+    // writes the next step's while its partner reads this one's, and the barrier of that next step is what lies between
+    // this read and the write after it. With a buffer a tile the next scores follow all eight warps' weights.
+    static constexpr int kTops = kBufs == 2 ? 1 : 2, kTop = 2 * 2 * kTile;
+    static constexpr int kOffTop = kOffBar + 320;
+    static constexpr int kSmem = kOffTop + kTops * kTop * 4;
     static_assert(kSmem <= 232448, "shared memory");
     static_assert(kOffS - 1024 >= 4 * (HXQ_ATTENTION_MAX_REQUESTS + 1) && sizeof(RangeShared<kWarpsT>) <= 1024, "room for the scan");
     static constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
@@ -411,9 +416,10 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 const bool all = (int32_t)(key0 + 63) <= pos_first && (int32_t)key0 > floor_last;
                 float top = all ? largest64<false>(tS, sc, fac, key0, pos, floor) : largest64<true>(tS, sc, fac, key0, pos, floor);
                 // and of the other half's
-                tops[hf * kTile + rr] = top;
+                float *now = tops + (j & (G::kTops - 1)) * G::kTop;
+                now[hf * kTile + rr] = top;
                 named_sync(pair, 64);
-                top = fmaxf(top, tops[(hf ^ 1u) * kTile + rr]);
+                top = fmaxf(top, now[(hf ^ 1u) * kTile + rr]);
                 if (__any_sync(~0u, top > M + kRaise)) {
                     // raise the maximum (all rows of the warp; the other half's warp does the same), O and l with it
                     const float to = fmaxf(M, top), al = to == -INFINITY ? 1.0f : ex2(M - to);

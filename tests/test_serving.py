@@ -880,3 +880,21 @@ def test_attention_tiles_of_rows(cuda, dim, new, lens, heads, group, window, cau
     from hxq_b200 import serving as S
     c, q, starts, sd, ld, table = _attention_case(torch, S, new, lens, heads, group, dim, 32, "e4m3", "bf16", seed=len(new))
     _check_attention(torch, S, c, q, starts, sd, ld, table, max(new), window, causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens,heads,group,window", [
+    ([256, 100], [6000, 3000], 8, 1, 0), ([130] * 6, [2600] * 6, 4, 5, 700), ([512, 512], [8704, 8192], 4, 5, 4096)])
+def test_attention_maxima_of_a_rows_halves(cuda, new, lens, heads, group, window):
+    """Heads of 64, where the next scores of a tile are there while its warps
+    are at these: keys that grow all the way, so that the maximum of both
+    halves of a row is raised in most steps, and the same bits every time."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    c, q, starts, sd, ld, table = _attention_case(torch, S, new, lens, heads, group, 64, 16, "int8", "bf16", seed=len(new), spread=0.3)
+    for b, n in enumerate(lens):
+        pages = table[b, :-(-n // 16)].long()
+        c.k_scales[pages] *= torch.exp2(torch.arange(len(pages), device="cuda") * (6.0 / len(pages)))[:, None]
+    o, _ = _check_attention(torch, S, c, q, starts, sd, ld, table, max(new), window)
+    for _ in range(30):
+        assert torch.equal(c.attention(q, sd, ld, table, max(new), window=window), o)
