@@ -85,21 +85,6 @@ template <typename QT> __device__ __forceinline__ uint32_t to_f16x2(uint32_t w, 
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Bounded wait for a copy (2^24 tries).
-__device__ __forceinline__ bool arrived(uint64_t *bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
-        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\t"
-        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 16777216;\n\t@q bra AGAIN_%=;\n"
-        "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(pipe::smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 __device__ __forceinline__ uint32_t turn8x8(uint32_t v)
 {
     uint32_t d;
@@ -119,9 +104,13 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
     uint8_t *smem = smem_raw + ((1024u - (pipe::smem_u32(smem_raw) & 1023u)) & 1023u);
     __shared__ RangeShared<kWarpsA> sh;
     __shared__ float sh_m[kWarpsA][kRows], sh_l[kWarpsA][kRows];
+    __shared__ uint32_t gave_up;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q = lane & 3;
     let_next_start();
-    if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0) {
+        a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+        gave_up = 0;
+    }
     Range range;
     if (!find_range<kWarpsA, kRows, kGran, kFixed>(a, sh, reinterpret_cast<uint32_t *>(smem), true, range)) return;
     __syncthreads();   // the sums in front of the requests are read: the ring may be filled
@@ -279,7 +268,8 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
             cp_wait<G::kStages - 2>();
             const bool live = valid >> stage & 1u;
             if (live) {
-                in_time = in_time && arrived(full + stage, phase >> stage & 1u);
+                in_time = __all_sync(~0u, bounded_wait(full + stage, phase >> stage & 1u, &gave_up, a) && a.wait_cycles);
+                if (!in_time) break;
                 phase ^= 1u << stage;
             }
             {
@@ -432,7 +422,8 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
                     sh_l[warp][8 * n + 2 * q + i] = l[n][i];
                 }
             }
-        __syncthreads();
+        in_time = __syncthreads_and(in_time);   // all four warps go on, or none
+        if (!in_time) break;
         float *mine = merge + warp * kRows * (D + G::kPad);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -493,7 +484,10 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
         pipe::async_proxy_fence();
         __syncthreads();   // the ring is free again
     }
-    if (!in_time && lane == 0) flag(a.status, HXQ_SERVING_TIMEOUT);
+    if (!in_time) {
+        if (lane == 0) flag(a.status, HXQ_SERVING_TIMEOUT);
+        let_copies_end();
+    }
 }
 
 template <int D, typename QT, int NT> __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a)
@@ -597,6 +591,9 @@ struct AttnLayout {
     size_t part, tc_desc, tc_part, bytes;
 };
 
+// What a wait inside a kernel may take: about a second.
+std::atomic<uint32_t> wait_cycles{2000000000u};
+
 // Requests with more rows than this go to the tcgen05 kernel.
 constexpr uint32_t kFewRows = 64;
 
@@ -620,6 +617,10 @@ AttnLayout attn_layout(uint32_t D, uint64_t most_rows)   // most_rows: of a requ
 using namespace hxq::serving;
 
 extern "C" {
+
+// Not part of the API: lets a test see the waits of the attention kernels run
+// out. Returns the limit there was.
+uint32_t hxq_serving_wait_cycles(uint32_t cycles) { return wait_cycles.exchange(cycles); }
 
 size_t hxq_cuda_kv_attention_workspace(const hxq_kv_cache_t *cache, const hxq_kv_attention_t *args)
 {
@@ -670,6 +671,7 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     a.causal = args->causal != 0;
     a.row_min = 0;
     a.row_max = 0xffffffffu;
+    a.wait_cycles = wait_cycles.load(std::memory_order_relaxed);
     a.scale_log2 = args->scale * 1.4426950408889634f;
     uint8_t *ws = static_cast<uint8_t *>(d_workspace);
     a.desc = reinterpret_cast<int4 *>(ws);

@@ -4,6 +4,8 @@
 
 #include "serving_common.cuh"
 
+#include "tc_pipe.cuh"
+
 namespace hxq {
 namespace serving {
 
@@ -24,7 +26,35 @@ struct AttnArgs {
     float scale_log2;            // scale * log2(e)
     float *part;                 // partial results
     int4 *desc;                  // one per CTA
+    uint32_t wait_cycles;        // most that a wait inside the kernel takes
 };
+
+// Wait for an mbarrier's phase, for at most a.wait_cycles cycles; false if
+// they ran out, which is noted in gave_up (a word of shared memory), or if
+// another wait of the CTA has noted it.
+__device__ __forceinline__ bool bounded_wait(uint64_t *bar, uint32_t parity, uint32_t *gave_up, const AttnArgs &a)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .u32 t0, t1;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\tmov.u32 t0, %%clock;\n"
+        "AGAIN_%=:\n\tmov.u32 t1, %%clock;\n\tsub.u32 t1, t1, t0;\n\tsetp.ge.u32 q, t1, %4;\n\t@q bra LATE_%=;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\t"
+        "ld.volatile.shared.u32 t1, [%3];\n\tsetp.ne.u32 q, t1, 0;\n\t@q bra DONE_%=;\n\tbra AGAIN_%=;\n"
+        "LATE_%=:\n\tst.volatile.shared.u32 [%3], 1;\n"
+        "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(pipe::smem_u32(bar)), "r"(parity), "r"(pipe::smem_u32(gave_up)), "r"(a.wait_cycles)
+        : "memory");
+    return ok != 0;
+}
+
+// For a thread that gave up on copies of its own: they end before the CTA does.
+__device__ __forceinline__ void let_copies_end()
+{
+    const uint64_t t0 = clock64();
+    while (clock64() - t0 < 20000000ull) {}
+}
 
 // One request: first q row, rows, keys; rows of a (request, cache head) are
 // numbered token * G + group member.

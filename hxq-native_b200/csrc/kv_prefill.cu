@@ -40,7 +40,8 @@
 // tile, cost (462 -> 490 us at the time).
 //
 // Work is cut and joined as in kv_attention.cu, with granules of 128 keys.
-// Every wait is bounded; one that runs out is recorded and the CTA unwinds.
+// Every wait is bounded by the clock; one that runs out is recorded and the CTA
+// unwinds.
 #include "kv_attention.cuh"
 
 #include "tc_pipe.cuh"
@@ -159,7 +160,7 @@ __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint3
 struct Bars {
     uint64_t q_full[2], s_full[2][3], p_full[3], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t rawk_full, rawk_empty, rawv_full, rawv_empty, seg_full[kSegSlots], seg_empty[kSegSlots], drained;
-    uint32_t tmem;
+    uint32_t tmem, gave_up;
     uint32_t live[2], zero[2][8];   // of a raw step (by its parity): keys within the range (0: no more steps), value groups that count as 0
 };
 static_assert(sizeof(Bars) <= 320, "room for the barriers");
@@ -174,25 +175,20 @@ struct SegInfo {
 };
 static_assert(sizeof(SegInfo) == 64, "a slot");
 
-// Bounded wait (2^24 tries, each of which the hardware suspends for a while);
-// false if it ran out.
-__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
-        "AGAIN_%=:\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t@p bra DONE_%=;\n\t"
-        "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, 16777216;\n\t@q bra AGAIN_%=;\n"
-        "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(pipe::smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
 __device__ __forceinline__ void named_sync(uint32_t id, uint32_t threads)
 {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// The same, and whether `ok` holds in every one of the threads.
+__device__ __forceinline__ bool named_all(uint32_t id, uint32_t threads, bool ok)
+{
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.and.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(all)
+                 : "r"(id), "r"(threads), "r"((uint32_t)ok)
+                 : "memory");
+    return all != 0;
 }
 
 // Largest of 16 scores.
@@ -290,6 +286,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         return;
     }
     if (tid == 0) {
+        bars->gave_up = 0;
         for (int t = 0; t < 2; ++t) {
             pipe::mbar_init(&bars->q_full[t], kSoftWarps / 2);   // one arrival a warp
             pipe::mbar_init(&bars->o_done[t], 1);
@@ -322,6 +319,9 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
     fence_after();
     const uint32_t tmem = bars->tmem;
 
+    // Where a wait runs out, the CTA unwinds: the other waits follow (gave_up), a warp takes a wait's outcome as one, and the
+    // warps of the rows meet at every barrier of theirs first, so that they leave the loops together.
+    auto wait = [&](uint64_t *bar, uint32_t parity) { return bounded_wait(bar, parity, &bars->gave_up, a); };
     bool ok = true;
     if (warp < kSoftWarps) {
         // ------------------------------------------------------- rows
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
         uint32_t step0 = 0, use0 = 0;                                  // CTA's steps, and tiles' steps, before this segment
         for (uint32_t si = 0;; ++si) {
             const SegInfo &seg = segs[si % kSegSlots];
-            ok = __all_sync(~0u, wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u));
+            ok = named_all(whole_tile, 2 * kTile, wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u));
             if (!ok || seg.take == 0) break;
             const uint32_t take = t == 0 ? seg.take0 : seg.take, key_first = seg.key0;
             const uint32_t tr0 = seg.r0 + t * kTile, r1 = seg.r1;
@@ -408,18 +408,21 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 // a tile that a segment does not have is several turns of the buffers ahead, of its own barriers none.
                 const uint32_t use = use0 + (j < both ? 2 * j + t : both + j);
                 const uint32_t buf = G::kBufs == 2 ? t : use % 3u, tS = tS0 + buf * 128u;
-                ok = __all_sync(~0u, wait(&bars->s_full[t][buf], turns >> buf & 1u));
-                if (!ok) break;
+                ok = ok && __all_sync(~0u, wait(&bars->s_full[t][buf], turns >> buf & 1u));
                 turns ^= 1u << buf;
                 fence_after();
                 const float4 *sc = scales + ((step0 + j) & (G::kScaleSlots - 1)) * 8 + hf * 4;
                 const bool all = (int32_t)(key0 + 63) <= pos_first && (int32_t)key0 > floor_last;
-                float top = all ? largest64<false>(tS, sc, fac, key0, pos, floor) : largest64<true>(tS, sc, fac, key0, pos, floor);
-                // and of the other half's
+                // and of the other half's; NaN, which no maximum is, from a warp whose wait ran out
+                float top = __uint_as_float(0x7fffffffu);
+                if (ok) top = all ? largest64<false>(tS, sc, fac, key0, pos, floor) : largest64<true>(tS, sc, fac, key0, pos, floor);
                 float *now = tops + (j & (G::kTops - 1)) * G::kTop;
                 now[hf * kTile + rr] = top;
                 named_sync(pair, 64);
-                top = fmaxf(top, now[(hf ^ 1u) * kTile + rr]);
+                const float others = now[(hf ^ 1u) * kTile + rr];
+                ok = ok && others == others;
+                if (!ok) break;
+                top = fmaxf(top, others);
                 if (__any_sync(~0u, top > M + kRaise)) {
                     // raise the maximum (all rows of the warp; the other half's warp does the same), O and l with it
                     const float to = fmaxf(M, top), al = to == -INFINITY ? 1.0f : ex2(M - to);
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     l *= al;
                     if (j > 0) {
                         ok = __all_sync(~0u, wait(&bars->o_done[t], (n_s - 1) & 1u));
-                        if (!ok) break;
+                        if (!ok) continue;   // the partner learns of it in the next step, or behind the last
                         fence_after();
 #pragma unroll 1
                         for (int c = 0; c < D / 32; ++c) {
@@ -449,10 +452,9 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 if (lane == 0) pipe::mbar_arrive(&bars->p_full[buf]);
                 ++n_s;
             }
-            if (!ok) break;
             step0 += seg.take;
             use0 += both + seg.take;
-            ok = __all_sync(~0u, wait(&bars->o_done[t], (n_s - 1) & 1u));
+            ok = named_all(whole_tile, 2 * kTile, ok && wait(&bars->o_done[t], (n_s - 1) & 1u));
             if (!ok) break;
             fence_after();
             // the products are done: Q's place takes the halves' sums, then the rows on their way out
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             uint8_t *dst = smem + G::kOffRaw + (keys ? 0 : G::kRaw) + lane * 16 * D;
             uint32_t it = 0;
             for (uint32_t si = 0; ok; ++si) {
-                ok = wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u);
+                ok = __all_sync(0xffu, wait(&bars->seg_full[si % kSegSlots], si / kSegSlots & 1u));
                 if (!ok) break;
                 const SegInfo seg = segs[si % kSegSlots];
                 __syncwarp(0xffu);
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                         b.x = ks;
                         value_scale(vs, b.y, b.z, zero);
                     }
-                    if (it >= 1) ok = wait(raw_empty, (it - 1) & 1u);
+                    if (it >= 1) ok = __all_sync(0xffu, wait(raw_empty, (it - 1) & 1u));
                     if (!ok) break;
                     if (keys) {
                         scales[(it & (G::kScaleSlots - 1)) * 8 + lane] = b;
@@ -700,18 +702,12 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 }
             }
             // the end of the work
-            if (keys) {
-                if (ok && it >= 1) ok = wait(raw_empty, (it - 1) & 1u);
-                if (ok) {
-                    if (lane == 0) bars->live[it & 1u] = 0;
-                    pipe::mbar_arrive(raw_full);
-                }
+            if (ok && it >= 1) ok = __all_sync(0xffu, wait(raw_empty, (it - 1) & 1u));
+            if (keys && ok) {
+                if (lane == 0) bars->live[it & 1u] = 0;
+                pipe::mbar_arrive(raw_full);
             }
-            // copies under way end before the CTA does
-            if (!ok) {
-                const uint64_t t0 = clock64();
-                while (clock64() - t0 < 20000000ull) {}
-            }
+            if (!ok) let_copies_end();
         } else if (warp == kPlanWarp && lane == 0) {
             // --------------------------------------------------- segments
             Segment seg;

@@ -898,3 +898,31 @@ def test_attention_maxima_of_a_rows_halves(cuda, new, lens, heads, group, window
     o, _ = _check_attention(torch, S, c, q, starts, sd, ld, table, max(new), window)
     for _ in range(30):
         assert torch.equal(c.attention(q, sd, ld, table, max(new), window=window), o)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cycles", [0, 300, 1500, 4000, 10000, 25000])
+@pytest.mark.parametrize("dim,new,lens", [
+    (64, [1, 1], [2500, 1200]), (128, [1, 3], [2500, 1200]), (64, [300, 90], [2500, 1200]), (128, [300, 90], [2500, 1200]),
+    (64, [1, 1], [200000, 150000]), (128, [2, 1], [200000, 150000])])
+def test_attention_waits_that_run_out(H, L, cuda, dim, new, lens, cycles):
+    """A wait inside the kernels that runs out ends the call with a status,
+    wherever it is, and the next call is as if nothing had been."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    c, q, starts, sd, ld, table = _attention_case(torch, S, new, lens, 4, 2, dim, 16, "int8", "bf16")
+    clean = c.attention(q, sd, ld, table, max(new))
+    torch.cuda.synchronize()
+    L.hxq_serving_wait_cycles.argtypes, L.hxq_serving_wait_cycles.restype = [C.c_uint32], C.c_uint32
+    before = L.hxq_serving_wait_cycles(cycles)
+    try:
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        o = c.attention(q, sd, ld, table, max(new), status=status)
+        torch.cuda.synchronize()
+    finally:
+        assert L.hxq_serving_wait_cycles(before) == cycles
+    assert before > 10 ** 9 and int(status) in (0, 64)
+    assert int(status) == 64 or torch.equal(o, clean)
+    assert int(status) == 64 or cycles   # without any patience no call ends as it should
+    status.zero_()
+    assert torch.equal(c.attention(q, sd, ld, table, max(new), status=status), clean) and int(status) == 0
