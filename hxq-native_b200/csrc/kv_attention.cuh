@@ -182,7 +182,7 @@ __device__ __forceinline__ bool find_range(const AttnArgs &a, RangeShared<WARPS>
     uint64_t tiles;
     {
         const uint32_t per = (a.B + N - 1) / N, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-        uint32_t mine = 0;
+        uint64_t mine = 0;
         for (uint32_t i = b0; i < b1; ++i) {
             mine += (load_req(a, i).rows + ROWS - 1) / ROWS;
             if (record && blockIdx.x == 0) flag_req(a, i);
@@ -195,7 +195,9 @@ __device__ __forceinline__ bool find_range(const AttnArgs &a, RangeShared<WARPS>
         if (tid == 0) { pre[a.B] = (uint32_t)tiles; sh.b = a.B; }
         __syncthreads();
     }
-    if (tiles == 0) return false;
+    // More than the rows there are make: starts that descend, so that requests overlap (recorded by flag_req). Their tiles
+    // may be more than 32 bits count, and no program wants their work.
+    if (tiles == 0 || tiles > (uint64_t)a.T * a.G / ROWS + a.B) return false;
     const uint32_t per = ((uint32_t)tiles + N - 1) / N, p0 = min(tid * per, (uint32_t)tiles), p1 = min(p0 + per, (uint32_t)tiles);
     uint32_t lo = 0, most = 1, first;
     uint64_t mine = 0;

@@ -109,7 +109,8 @@ hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots
  * over i <= position of t (causal; every i < d_lens[b] otherwise) and, with a
  * window, i > position - window.  A row that sees nothing (d_lens[b] = 0, or
  * more rows than d_lens[b]) becomes 0 and its lse -infinity.  Rows outside
- * every request are left as they were.
+ * every request are left as they were; where starts descend, rows that two
+ * requests claim get either one's result, or all rows are left (recorded).
  * q and out are bf16 or f16 (elem), head_dim consecutive elements, strides in
  * elements, q rows 16-byte aligned.  Codes enter the products exactly, sums
  * and the softmax are fp32, softmax weights are rounded to f16 for the second

@@ -926,3 +926,22 @@ def test_attention_waits_that_run_out(H, L, cuda, dim, new, lens, cycles):
     assert int(status) == 64 or cycles   # without any patience no call ends as it should
     status.zero_()
     assert torch.equal(c.attention(q, sd, ld, table, max(new), status=status), clean) and int(status) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,T,heads,max_new", [(64, 40, 4, 1), (64, 40, 4, 40), (8192, 1 << 17, 64, 1), (8192, 1 << 17, 64, 1 << 17)])
+def test_attention_overlapping_requests(cuda, B, T, heads, max_new):
+    """Starts 0, T, 0, T, ..: far more rows than there are (in the last two
+    shapes 2^32 tiles and more), recorded and not worked off."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    c = S.KvCache.allocate(4, 1, 64)
+    q = torch.ones((T, heads, 64), dtype=torch.bfloat16, device="cuda")
+    starts = torch.tensor([T * (b & 1) for b in range(B + 1)], dtype=torch.int32, device="cuda")
+    lens = torch.full((B,), 17, dtype=torch.int32, device="cuda")
+    table = torch.zeros((B, 2), dtype=torch.int32, device="cuda")
+    out, status = torch.full_like(q, 9.0), torch.zeros(1, dtype=torch.int32, device="cuda")
+    c.attention(q, starts, lens, table, max_new, causal=False, out=out, status=status)
+    torch.cuda.synchronize()
+    # a cache of zeros: a request's result is 0
+    assert int(status) == 4 and bool(((out == 9) | (out == 0)).all()) and (B < 8192 or bool((out == 9).all()))
