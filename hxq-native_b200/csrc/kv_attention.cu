@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
     Segment seg;
     while (next_segment<kRows, kGran, kFixed>(a, range, seg)) {
         const Req &r = seg.r;
-        const uint32_t h = seg.h, take = seg.take, hi = seg.hi, r0 = seg.r0, r1 = seg.r1;
+        const uint32_t h = seg.h, take = seg.take, lo = seg.lo, hi = seg.hi, r0 = seg.r0, r1 = seg.r1;
         const uint32_t key0 = seg.key0 + warp * 16;   // this warp's first 16 keys
         const int32_t before = (int32_t)r.len - (int32_t)r.n;
         auto position = [&](uint32_t row) { return a.causal ? before + (int32_t)token_of(a, row) : (int32_t)r.len - 1; };
@@ -158,11 +158,11 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
         auto entry = [&](uint32_t j) -> int32_t {
             const uint32_t key = key0 + j * kGran;
             uint32_t slot;
-            return j < take && key < hi ? __ldg(table + block_of(a, key, slot)) : -1;
+            return j < take && key < hi && key + 16 > lo ? __ldg(table + block_of(a, key, slot)) : -1;
         };
         auto issue = [&](uint32_t j, uint32_t stage, int32_t blk) {
             const uint32_t key = key0 + j * kGran;
-            const bool wanted = j < take && key < hi, ok = wanted && (uint32_t)blk < a.n_blocks;
+            const bool wanted = j < take && key < hi && key + 16 > lo, ok = wanted && (uint32_t)blk < a.n_blocks;
             if (wanted && !ok && lane == 0) flag(a.status, HXQ_SERVING_BAD_BLOCK);
             valid = ok ? valid | 1u << stage : valid & ~(1u << stage);
             if (ok) {
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
                         p[n][i] = zero ? 0u : v;
                     }
                 }
-                const bool tail = key + 16 > hi;
+                const bool tail = key + 16 > hi || key < lo;
 #pragma unroll
                 for (int c = 0; c < G::kVC; ++c) {
                     uint32_t vw[4][4];
@@ -386,10 +386,10 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
                         }
                     }
                     if (tail) {
-                        // slots behind the last key may hold anything
+                        // slots behind the last key and in front of the first may hold anything
 #pragma unroll
                         for (int ts = 0; ts < 4; ++ts)
-                            if (key + 2 * q + (ts & 1) + (ts >> 1) * 8 >= hi) vw[ts][0] = vw[ts][1] = vw[ts][2] = vw[ts][3] = 0;
+                            if (key + 2 * q + (ts & 1) + (ts >> 1) * 8 - lo >= hi - lo) vw[ts][0] = vw[ts][1] = vw[ts][2] = vw[ts][3] = 0;
                     }
 #pragma unroll
                     for (int i = 0; i < G::kVB / 4; ++i)

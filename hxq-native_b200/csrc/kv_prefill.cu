@@ -161,7 +161,9 @@ struct Bars {
     uint64_t q_full[2], s_full[2][3], p_full[3], o_done[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t rawk_full, rawk_empty, rawv_full, rawv_empty, seg_full[kSegSlots], seg_empty[kSegSlots], drained;
     uint32_t tmem, gave_up;
-    uint32_t live[2], zero[2][8];   // of a raw step (by its parity): keys within the range (0: no more steps), value groups that count as 0
+    // of a raw step (by its parity): keys up to the range's last (0: no more steps) and, in the upper half, those in front
+    // of its first; value groups that count as 0
+    uint32_t live[2], zero[2][8];
 };
 static_assert(sizeof(Bars) <= 320, "room for the barriers");
 
@@ -170,7 +172,8 @@ struct SegInfo {
     uint32_t take, take0;            // steps, and those that tile 0 takes part in
     uint32_t key0, hi, r0, r1, q0, h, b;
     int32_t before;                  // position of the request's first row
-    uint32_t len, whole;
+    uint32_t len;
+    uint16_t whole, front;           // front: keys of the first step that no row sees, a window being behind them
     int4 cut;                        // for the joining kernel, where the segment begins a unit and doesn't end it
 };
 static_assert(sizeof(SegInfo) == 64, "a slot");
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
             const uint32_t st = it & 1u, par = (it >> 1) & 1u;
             ok = __all_sync(~0u, wait(&bars->rawk_full, it & 1u));
             if (!ok) break;
-            const uint32_t live = bars->live[st];
+            const uint32_t range = bars->live[st], live = range & 0xffffu, front = range >> 16;
             if (live == 0) break;
             if (it >= 2) ok = __all_sync(~0u, wait(&bars->k_empty[st], par ^ 1u));
             if (!ok) break;
@@ -581,7 +584,8 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
 #pragma unroll 4
             for (int i = 0; i < kNK; ++i) {
                 uint2 w = pipe::lds64(k_src + i * (4 * kRowsK * D));
-                if (live < kKeys && ((kr + i * 4 * kRowsK) & ~15u) >= live) w = make_uint2(0, 0);   // not copied
+                const uint32_t r16 = (kr + i * 4 * kRowsK) & ~15u;
+                if (range != kKeys && (r16 >= live || r16 + 16 <= front)) w = make_uint2(0, 0);   // not copied
                 uint32_t h[4];
                 codes_to_f16<FMT>(w.x, h[0], h[1]);
                 codes_to_f16<FMT>(w.y, h[2], h[3]);
@@ -605,11 +609,11 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
 #pragma unroll
                 for (int u = 0; u < 8; ++u) w[u] = pipe::lds32(v_src + i * (kStepV * 8 * D) + (D == 64 ? u ^ swap : u) * D);
                 const bool drop = bars->zero[st][grp >> 1] != 0;
-                if (drop || grp * 8 + 8 > live) {
-                    // blocks that count as 0, and slots behind the last key, which may hold anything
+                if (drop || grp * 8 + 8 > live || grp * 8 < front) {
+                    // blocks that count as 0, and slots behind the last key or in front of the first, which may hold anything
 #pragma unroll
                     for (int u = 0; u < 8; ++u)
-                        if (drop || grp * 8 + (D == 64 ? u ^ swap : u) >= live) w[u] = 0;
+                        if (drop || grp * 8 + (D == 64 ? u ^ swap : u) - front >= live - front) w[u] = 0;
                 }
                 uint32_t o[4][4];
 #pragma unroll
@@ -650,7 +654,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 auto entry = [&](uint32_t j) -> int32_t {
                     const uint32_t key = seg.key0 + j * kKeys + lane * 16;
                     uint32_t slot;
-                    return j < seg.take && key < seg.hi ? __ldg(row + block_of(a, key, slot)) : -1;
+                    return j < seg.take && key < seg.hi && (j > 0 || lane * 16 + 16 > seg.front) ? __ldg(row + block_of(a, key, slot)) : -1;
                 };
                 auto scales_of = [&](int32_t blk, float &ks, float &vs) {
                     ks = vs = 0.0f;
@@ -668,8 +672,8 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     const int32_t blk2 = entry(j + 2);
                     float ks1, vs1;
                     scales_of(blk1, ks1, vs1);
-                    const bool in = key < seg.hi && (uint32_t)blk < a.n_blocks;
-                    if (keys && key < seg.hi && !in) flag(a.status, HXQ_SERVING_BAD_BLOCK);
+                    const bool wanted = key < seg.hi && (j > 0 || lane * 16 + 16 > seg.front), in = wanted && (uint32_t)blk < a.n_blocks;
+                    if (keys && wanted && !in) flag(a.status, HXQ_SERVING_BAD_BLOCK);
                     uint32_t slot;
                     block_of(a, key, slot);
                     const size_t src = (((size_t)(in ? (uint32_t)blk : 0u) * a.H + seg.h) * a.P + slot) * D;
@@ -683,13 +687,14 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     if (!ok) break;
                     if (keys) {
                         scales[(it & (G::kScaleSlots - 1)) * 8 + lane] = b;
-                        if (lane == 0) bars->live[it & 1u] = min((uint32_t)kKeys, seg.hi > key0 ? seg.hi - key0 : 1u);
+                        if (lane == 0)
+                            bars->live[it & 1u] = min((uint32_t)kKeys, seg.hi > key0 ? seg.hi - key0 : 1u) | (j == 0 ? (uint32_t)seg.front << 16 : 0u);
                     } else bars->zero[it & 1u][lane] = zero;
                     if (in) {
                         pipe::mbar_expect_tx(raw_full, 16 * D);
                         pipe::bulk_g2s(dst, codes + src, 16 * D, raw_full);
                     } else {
-                        if (key < seg.hi) {   // in place of a block outside the cache
+                        if (wanted) {   // in place of a block outside the cache
                             for (int i = 0; i < D; ++i) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0, 0, 0, 0);
                             pipe::async_proxy_fence();
                         }
@@ -732,6 +737,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                     d.before = (int32_t)seg.r.len - (int32_t)seg.r.n;
                     d.len = seg.r.len;
                     d.whole = seg.begins && seg.take == seg.n;
+                    d.front = (uint16_t)(seg.lo > seg.key0 ? seg.lo - seg.key0 : 0u);
                     d.cut = seg.begins && seg.take < seg.n ? cut_unit(range, seg) : make_int4(0, 0, 0, 0);
                 }
                 pipe::mbar_arrive(&bars->seg_full[si % kSegSlots]);

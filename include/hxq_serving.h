@@ -107,7 +107,8 @@ hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots
  * cache (G = n_heads / cache->n_heads):
  *     out[t, j] = sum_i softmax_i(scale * q[t, j] . k_i) v_i
  * over i <= position of t (causal; every i < d_lens[b] otherwise) and, with a
- * window, i > position - window.  A row that sees nothing (d_lens[b] = 0, or
+ * window, i > position - window; table entries of blocks that no row of the
+ * request sees are not looked at, and what their slots hold does not matter.  A row that sees nothing (d_lens[b] = 0, or
  * more rows than d_lens[b]) becomes 0 and its lse -infinity.  Rows outside
  * every request are left as they were; where starts descend, rows that two
  * requests claim get either one's result, or all rows are left (recorded).

@@ -945,3 +945,30 @@ def test_attention_overlapping_requests(cuda, B, T, heads, max_new):
     torch.cuda.synchronize()
     # a cache of zeros: a request's result is 0
     assert int(status) == 4 and bool(((out == 9) | (out == 0)).all()) and (B < 8192 or bool((out == 9).all()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new,lens,heads,group,dim,P,window", [
+    ([1, 2], [300, 77], 2, 4, 128, 16, 40), ([1], [1000], 1, 1, 64, 16, 3), ([1, 3], [500, 129], 1, 8, 256, 32, 100),
+    ([5, 4], [90, 400], 2, 3, 64, 16, 1), ([100, 90], [700, 400], 2, 3, 64, 16, 50), ([300, 70], [1000, 1111], 1, 2, 128, 16, 333),
+    ([129], [129 + 640], 2, 1, 128, 128, 511), ([150, 80] * 4, [900, 700] * 4, 4, 2, 64, 64, 130)])
+def test_attention_blocks_behind_the_window(cuda, fmt, new, lens, heads, group, dim, P, window):
+    """A program frees blocks that a window has passed: their entries are no
+    blocks, and slots that no row sees hold anything, NaN codes among it."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    c, q, starts, sd, ld, table = _attention_case(torch, S, new, lens, heads, group, dim, P, fmt, "bf16", seed=window)
+    clean, _ = _check_attention(torch, S, c, q, starts, sd, ld, table, max(new), window)
+    for b, (m, n) in enumerate(zip(new, lens)):
+        first = max(n - m - window + 1, 0)   # the first key that a row sees
+        for j in range(first // P):
+            c.k_scales[table[b, j].long()] = math.nan
+            c.v_scales[table[b, j].long()] = math.nan
+            table[b, j] = (-1, c.n_blocks, 2 ** 31 - 1)[j % 3]
+        if first % P:
+            c.k.view(torch.uint8)[table[b, first // P].long(), :, :first % P] = 0x7f
+            c.v.view(torch.uint8)[table[b, first // P].long(), :, :first % P] = 0xff
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    o = c.attention(q, sd, ld, table, max(new), window=window, status=status)
+    assert int(status) == 0 and torch.equal(o, clean)
