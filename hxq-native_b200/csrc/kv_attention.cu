@@ -6,9 +6,9 @@
 // lv = log2 vs, the weights exp2(s_j + lv_j - M) with M = max_j (s_j + lv_j)
 // make both products run on codes alone:
 //     out = sum_j w_j code_j / sum_j (w_j / vs_j),   0 <= w_j <= 1.
-// Codes are exact in f16; w is rounded to f16 relative to the largest weighted
-// contribution, so a block with large values and no weight costs the others
-// nothing.  q is scaled per row by a power of two into f16's range (bf16
+// Codes are exact in f16; w (times 2^7) is rounded to f16 relative to the
+// largest weighted contribution, so a block with large values and no weight
+// costs the others nothing.  q is scaled per row by a power of two into f16's range (bf16
 // values down to 2^-39 of the row's largest are exact).
 //
 // A CTA of four warps takes 8 or 16 rows (tokens x heads of a group) of one
@@ -23,7 +23,7 @@
 // product is free as long as Q has the same, so a lane reads 16 consecutive
 // bytes of a key and brings them through a byte permute
 // into the fragments; the weights turn round with movmatrix.  The maximum is
-// raised only where a weight would pass 2^8 (f16 holds 2^16): a vote a step
+// raised only where a weight would grow by more than 2^8: a vote a step
 // instead of a reduction.
 //
 // The keys of all (request, head, tile of rows) are laid end to end in granules of
@@ -51,7 +51,7 @@ constexpr int kGran = 64;        // keys of a granule
 constexpr int kFixed = 2;        // granules that a unit costs by itself
 constexpr int kWarpsA = 4;
 constexpr int kThreadsA = kWarpsA * 32;
-constexpr float kRaiseA = 8.0f;  // log2 of the largest weight before the maximum is raised
+constexpr float kRaiseA = 8.0f;  // log2 of the largest weight (less the lift) before the maximum is raised
 
 template <int D> struct Geo {
     static constexpr int kVB = D >= 128 ? 16 : 8;      // bytes of a lane's load of a value row
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
                     float w[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float ms = m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1];
+                        const float ms = (m[n][e & 1] == -INFINITY ? 0.0f : m[n][e & 1]) - kLift;
                         w[e] = ex2(s[n][e] - ms);
                     }
 #pragma unroll
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
                 dst[2] = Elem<QT>::from(v.z * f);
                 dst[3] = Elem<QT>::from(v.w * f);
                 if (a.lse && d == 0)
-                    a.lse[(size_t)tok * a.Hq + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+                    a.lse[(size_t)tok * a.Hq + head] = sum == 0.0f ? -INFINITY : (top - kLift + log2f(sum)) * 0.69314718055994531f;
             } else {
                 *reinterpret_cast<float4 *>(part + rr * D + d) = v;
                 if (d == 0) {

@@ -389,12 +389,21 @@ template <int FMT> __device__ __forceinline__ void codes_to_f16(uint32_t w, uint
     }
 }
 
-// Weight of a value block: log2 of its scale (at least 2^-100), its inverse,
+// Weights are held times 2^kLift: f16 rounds below 2^-14 by 2^-25 whatever the
+// size, which a lift of 7 puts at 2^-32 of a row's largest contribution.  With
+// the largest at 2^0 a key that takes nearly all of the weight and has a small
+// value left the others few bits (131,000 of them, 0.01 of the weight: a fifth
+// of the output).  The largest weight before the maximum is raised is 2^15, f16
+// holds 2^16.  Sums carry the factor, which the quotient drops.
+constexpr float kLift = 7.0f;
+
+// Weight of a value block: log2 of its scale (at least 2^-80), its inverse,
 // and 0 or 1 for blocks that count as 0 or not.  NaN and infinity go through.
+// The floor keeps 2^31 keys' 2^15 / vs within fp32.
 __device__ __forceinline__ void value_scale(float vs, float &lv, float &inv, bool &zero)
 {
-    zero = vs < 7.8886090522101181e-31f;   // 2^-100
-    const float c = zero ? 7.8886090522101181e-31f : vs;
+    zero = vs < 8.271806125530277e-25f;   // 2^-80
+    const float c = zero ? 8.271806125530277e-25f : vs;
     lv = lg2(c);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(c));   // within an ulp
 }
@@ -496,7 +505,7 @@ __device__ __forceinline__ void join_row(const AttnArgs &a, const int4 *desc, co
         for (int j = 0; j < N; ++j) dst[j] = o[j];
     }
     if (a.lse && lane == 0)
-        a.lse[(size_t)tok * a.Hq + head] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+        a.lse[(size_t)tok * a.Hq + head] = sum == 0.0f ? -INFINITY : (top - kLift + log2f(sum)) * 0.69314718055994531f;
 }
 
 // Tensor-core kernel for many rows (kv_prefill.cu): launched behind the mma

@@ -26,7 +26,7 @@
 // while it is at these (chunks below 115 -> 107 us).
 //
 // The running maximum is lazy: it is raised, and O rescaled, only where a
-// weight would pass 2^8 (f16 holds 2^16), which after the first keys is rare,
+// weight would grow by more than 2^8, which after the first keys is rare,
 // so that the rescale needs no warps of its own.
 //
 // Bound by what passes between the warps in a step: scores to the rows' threads,
@@ -60,7 +60,7 @@ constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups
 constexpr int kRegsSoft = 88, kRegsConv = 64, kRegsRest = 64;
 constexpr int kThreadsT = kWarpsT * 32;
 constexpr int kSegSlots = 2;
-constexpr float kRaise = 8.0f;             // log2 of the largest weight before the maximum is raised
+constexpr float kRaise = 8.0f;             // log2 of the largest weight (less the lift) before the maximum is raised
 
 template <int D> struct TcGeo {
     static constexpr int kQ = kTile * D * 2;           // bytes of a tile of Q
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                         wait_st();
                     }
                 }
-                const float ms = M == -INFINITY ? 0.0f : M;
+                const float ms = (M == -INFINITY ? 0.0f : M) - kLift;
                 l += all ? weigh64<false>(tS, sc, fac, ms, key0, pos, floor) : weigh64<true>(tS, sc, fac, ms, key0, pos, floor);
                 wait_st();
                 fence_before();
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
                 if (hf == 0 && a.lse && tr0 + rr < tr1) {
                     const uint32_t tk = token_of(a, tr0 + rr);
                     a.lse[(size_t)(q0 + tk) * a.Hq + head0 + (tr0 + rr - tk * a.G)] =
-                        l == 0.0f ? -INFINITY : (M + log2f(l)) * 0.69314718055994531f;
+                        l == 0.0f ? -INFINITY : (M - kLift + log2f(l)) * 0.69314718055994531f;
                 }
             } else {
                 float *part = a.part + (size_t)(2 * blockIdx.x + (seg.cut.x ? 1 : 0)) * part_floats<kTcRows, D>();

@@ -114,9 +114,12 @@ hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots
  * requests claim get either one's result, or all rows are left (recorded).
  * q and out are bf16 or f16 (elem), head_dim consecutive elements, strides in
  * elements, q rows 16-byte aligned.  Codes enter the products exactly, sums
- * and the softmax are fp32, softmax weights are rounded to f16 for the second
- * product (2^-12 of each), out is rounded once.  Value blocks with a scale
- * below 2^-100 count as 0.  Codes of e4m3 caches are finite (hxq_cuda_kv_append
+ * and the softmax are fp32; for the second product a softmax weight times its
+ * block's value scale is rounded to f16: by up to 2^-11 of it, and below 2^-21
+ * of the row's largest by up to 2^-32 of that.  out is rounded once.  Value
+ * blocks with a scale below 2^-80 count as 0.  Keys whose value scale is 2^-130
+ * of the largest that the row sees, or less, are not counted in the softmax's
+ * sum (with those that count as 0: where a scale is above 2^50).  Codes of e4m3 caches are finite (hxq_cuda_kv_append
  * writes no others; slots that no request reads may hold anything).
  * d_lse (optional): [n_rows, n_heads] fp32, natural log of the softmax sums.
  * max_new: the most rows of any request; it only chooses the kernel, results

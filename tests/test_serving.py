@@ -972,3 +972,44 @@ def test_attention_blocks_behind_the_window(cuda, fmt, new, lens, heads, group, 
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     o = c.attention(q, sd, ld, table, max(new), window=window, status=status)
     assert int(status) == 0 and torch.equal(o, clean)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("new,n,B,heads,dim", [(1, 8192, 74, 8, 64), (1, 8192, 74, 8, 128), (130, 16384, 5, 32, 64), (130, 16384, 5, 32, 128)])
+def test_attention_key_that_takes_the_weight(cuda, new, n, B, heads, dim, fmt):
+    """A first key with nearly all of the weight and a value of 0, as trained
+    models have it: what is left is a sum over the others, each 2^-23 of it."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    g = torch.Generator("cuda").manual_seed(dim)
+    P, top = 64, QMAX[fmt]
+    n_blocks = B * n // P
+    c = S.KvCache.allocate(n_blocks, heads, dim, P, _types(torch)[fmt])
+    sign = torch.randint(0, 2, (dim,), generator=g, device="cuda") * 2.0 - 1
+    for t in (c.k, c.v):
+        x = torch.randn(t.shape, generator=g, device="cuda").mul_(0.3).clamp_(-1, 1) * top
+        t.view(torch.int8).copy_((x.round() if fmt == "int8" else x).to(t.dtype).view(torch.int8))
+    table = torch.arange(n_blocks, dtype=torch.int32, device="cuda").view(B, -1)
+    c.k.view(torch.int8)[table[:, 0].long(), :, 0] = (sign * top).to(c.k.dtype).view(torch.int8)
+    c.v.view(torch.int8)[table[:, 0].long(), :, 0] = 0
+    c.k_scales.fill_(1 / top)
+    c.v_scales.fill_(1 / top)
+    # score of the first key: log of (number of keys x 999) above the others' mean
+    beta = math.log(n * 999) / math.sqrt(dim)
+    q = (sign * beta * (1 + 0.002 * torch.randn((B * new, heads, 1), generator=g, device="cuda"))).to(torch.float16)
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    lse = torch.zeros(q.shape[:2], device="cuda")
+    o = c.attention(q, i([b * new for b in range(B + 1)]), i([n] * B), table, new, causal=False, lse=lse)
+    for b, h, t in ((0, 0, 0), (B - 1, heads - 1, new - 1), (B // 2, 3, new // 2)):
+        k, v = (x[table[b].long(), h].double().reshape(-1, dim) / float(torch.tensor(top)) for x in (c.k, c.v))
+        sc = k @ q[b * new + t, h].double() / math.sqrt(dim)
+        p = torch.softmax(sc, 0)
+        assert 0.99 < float(p[0]) < 0.9999
+        want = p @ v
+        # A weight is rounded by up to 2^-11 of it or 2^-32 of the first key's, evenly spread, so the deviation of the sum
+        # over values of mean 0 is at most 2^-11 / sqrt(3) + (2^-32 / sqrt(3)) / (0.0001 / n) of its own: 0.03% + 0.22% and,
+        # for 16,384 keys of which p[0] leaves least, + 0.44%; out is rounded by 2^-12. Three deviations: 1.5%.
+        rms = float((o[b * new + t, h].double() - want).norm() / want.norm())
+        assert rms < 0.015, (b, h, t, rms)
+        assert abs(float(lse[b * new + t, h]) - float(torch.logsumexp(sc, 0))) < 1e-4
