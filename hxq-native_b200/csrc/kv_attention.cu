@@ -9,7 +9,7 @@
 // Codes are exact in f16; w (times 2^7) is rounded to f16 relative to the
 // largest weighted contribution, so a block with large values and no weight
 // costs the others nothing.  q is scaled per row by a power of two into f16's range (bf16
-// values down to 2^-39 of the row's largest are exact).
+// values down to 2^-31 of the row's largest are exact).
 //
 // A CTA of four warps takes 8 or 16 rows (tokens x heads of a group) of one
 // (request, cache head) against 64 keys at a time, 16 keys a warp, every warp
@@ -228,9 +228,10 @@ __global__ void __launch_bounds__(kThreadsA, ctas_per_sm(D, NT == 1)) attn_mma_k
                 }
             top = max(top, __shfl_xor_sync(~0u, top, 1));
             top = max(top, __shfl_xor_sync(~0u, top, 2));
-            // 2^(14 - exponent of the largest): into [2^14, 2^15); 0 and non-finite rows as they are
+            // 2^(14 - exponent of the largest): into [2^14, 2^15) (below 2^-112: as far as a factor of 2^126 goes);
+            // 0 and non-finite rows as they are
             const int32_t e = (int32_t)(top >> 23) - 127;
-            const int32_t shift = (top == 0 || e == 128) ? 0 : max(-100, min(100, 14 - e));
+            const int32_t shift = (top == 0 || e == 128) ? 0 : max(-113, min(126, 14 - e));
             const float m = __uint_as_float((uint32_t)(127 + shift) << 23);
             const float f = a.scale_log2 * __uint_as_float((uint32_t)(127 - shift) << 23);
 #pragma unroll

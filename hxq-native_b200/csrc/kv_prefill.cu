@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreadsT, 1) attn_tc_kernel(const __grid_cons
 #pragma unroll
                     for (uint32_t d = 1; d < kLanes; d <<= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
                     const int32_t e2 = (int32_t)(top >> 23) - 127;
-                    const int32_t shift = (top == 0 || e2 == 128) ? 0 : max(-100, min(100, 14 - e2));
+                    const int32_t shift = (top == 0 || e2 == 128) ? 0 : max(-113, min(126, 14 - e2));
                     const float m = __uint_as_float((uint32_t)(127 + shift) << 23);
                     uint32_t w[4];
 #pragma unroll

@@ -1013,3 +1013,22 @@ def test_attention_key_that_takes_the_weight(cuda, new, n, B, heads, dim, fmt):
         rms = float((o[b * new + t, h].double() - want).norm() / want.norm())
         assert rms < 0.015, (b, h, t, rms)
         assert abs(float(lse[b * new + t, h]) - float(torch.logsumexp(sc, 0))) < 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [[1, 1, 1], [100, 80, 90]])
+@pytest.mark.parametrize("exponent", [127, 120, 116, 115, -86, -100, -118])
+def test_attention_queries_near_the_ends_of_bf16(cuda, exponent, new, dim):
+    """Rows of q that f16 cannot hold by far, with scales that bring the scores
+    back to the ordinary."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    c, q, starts, sd, ld, table = _attention_case(torch, S, new, [200, 333, 150], 2, 3, dim, 16, "int8", "bf16", spread=0.3)
+    q = (q.float() / q.float().abs().amax(-1, keepdim=True) * 1.98).to(torch.bfloat16)
+    q = (q.float() * 2.0 ** (exponent // 2) * 2.0 ** (exponent - exponent // 2)).to(torch.bfloat16)
+    assert bool(q.isfinite().all())
+    to_keys = min(exponent, 100)   # the rest, which key scales cannot take, to the factor of the scores
+    c.k_scales.mul_(2.0 ** -to_keys)
+    assert bool((c.k_scales > 2.0 ** -126).all()) and bool(c.k_scales.isfinite().all())
+    _check_attention(torch, S, c, q, starts, sd, ld, table, max(new), scale=dim ** -0.5 * 2.0 ** (to_keys - exponent))
