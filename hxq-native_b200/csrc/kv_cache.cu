@@ -478,7 +478,7 @@ hxq_error_t hxq_cuda_kv_plan(const int32_t *d_new, const int32_t *d_cached, uint
                   B, table_width, block_tokens, n_free, n_slots};
     const size_t smem = (size_t)(B + 1) * 2 * sizeof(uint32_t);
     static std::atomic<uint64_t> ready{0};
-    if (smem > 48u * 1024u &&
+    if (smem > 40u * 1024u &&   // 48 KB with the kernel's static part need no permission
         allow_smem(plan_kernel, (HXQ_PLAN_MAX_REQUESTS + 1) * 2 * sizeof(uint32_t), ready) != cudaSuccess) {
         cudaGetLastError();
         return HXQ_ERR_CUDA;

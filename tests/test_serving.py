@@ -1032,3 +1032,33 @@ def test_attention_queries_near_the_ends_of_bf16(cuda, exponent, new, dim):
     c.k_scales.mul_(2.0 ** -to_keys)
     assert bool((c.k_scales > 2.0 ** -126).all()) and bool(c.k_scales.isfinite().all())
     _check_attention(torch, S, c, q, starts, sd, ld, table, max(new), scale=dim ** -0.5 * 2.0 ** (to_keys - exponent))
+
+
+_FIRST_CALL = """
+import sys
+sys.path.insert(0, {pkg!r})
+import torch
+from hxq_b200 import serving as S
+B, n = {B}, {n}
+i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+status = i([0])
+if {op!r} == "plan":
+    p = S.kv_plan(i([1] * B), i([0] * B), i([-1] * B).view(B, 1), i(list(range(B))), 16, B, status=status)
+    assert p.slots.tolist() == [16 * b for b in range(B)] and int(p.taken) == B
+else:
+    p = S.lora_plan(i(list(range(B + 1))), i([b % n for b in range(B)]), n, B, status=status)
+    assert p.order.tolist() == sorted(range(B), key=lambda b: b % n)
+assert int(status) == 0
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [6109, 6110, 6143, 6144])
+def test_plan_as_a_process_first_call(cuda, B):
+    """Sizes about the limit of shared memory that needs no permission, which
+    an earlier and larger call would have raised."""
+    import subprocess
+    import sys
+
+    from conftest import PKG
+    subprocess.run([sys.executable, "-c", _FIRST_CALL.format(pkg=PKG, B=B, n=0, op="plan")], check=True, timeout=120)
