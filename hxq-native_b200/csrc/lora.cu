@@ -104,7 +104,6 @@ __global__ void __launch_bounds__(kLoraPlanThreads) lora_plan_kernel(const LoraP
         if (tid == kLoraPlanThreads - 1) { carry[0] = x; carry[1] = y; }
         __syncthreads();
     }
-    wait_previous();   // nothing is written before the kernel in front has ended
     const uint32_t used = carry[1];
     const uint32_t me = blockIdx.x * kLoraPlanThreads + tid, step = gridDim.x * kLoraPlanThreads;
     for (uint32_t i = me; i < a.n_tiles; i += step) {
@@ -564,7 +563,7 @@ hxq_error_t hxq_cuda_lora_plan(const int32_t *d_starts, const int32_t *d_adapter
     const size_t smem = ((size_t)(n_adapters + 1) * 3 + (size_t)B * 2) * sizeof(uint32_t);
     const size_t most = ((size_t)(HXQ_LORA_MAX_ADAPTERS + 1) * 3 + (size_t)HXQ_LORA_MAX_REQUESTS * 2) * sizeof(uint32_t);
     static std::atomic<uint64_t> ready{0};
-    if (smem > 48u * 1024u && allow_smem(lora_plan_kernel, most, ready) != cudaSuccess) {
+    if (smem > 40u * 1024u && allow_smem(lora_plan_kernel, most, ready) != cudaSuccess) {
         cudaGetLastError();
         return HXQ_ERR_CUDA;
     }

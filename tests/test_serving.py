@@ -1062,3 +1062,13 @@ def test_plan_as_a_process_first_call(cuda, B):
 
     from conftest import PKG
     subprocess.run([sys.executable, "-c", _FIRST_CALL.format(pkg=PKG, B=B, n=0, op="plan")], check=True, timeout=120)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,n", [(6109, 1), (6110, 1), (6141, 1), (6142, 1), (300, 3894)])
+def test_lora_plan_as_a_process_first_call(cuda, B, n):
+    import subprocess
+    import sys
+
+    from conftest import PKG
+    subprocess.run([sys.executable, "-c", _FIRST_CALL.format(pkg=PKG, B=B, n=n, op="lora_plan")], check=True, timeout=120)
