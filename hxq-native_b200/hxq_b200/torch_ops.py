@@ -127,9 +127,11 @@ def _(k_codes, v_codes, k_scales, v_scales, k, v, slots):
 def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
                  starts: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, max_new: int, scale: float, window: int,
                  causal: bool) -> torch.Tensor:
-    """Attention of q [rows, heads, head_dim] over an 8-bit cache."""
+    """Attention of q [rows, heads, head_dim] over an 8-bit cache; rows of no
+    request are 0."""
     from .serving import KvCache
-    return KvCache(k_codes, v_codes, k_scales, v_scales).attention(q, starts, lens, table, max_new, scale, window, causal)
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    return KvCache(k_codes, v_codes, k_scales, v_scales).attention(q, starts, lens, table, max_new, scale, window, causal, out=out)
 
 
 @kv_attention.register_fake
@@ -140,9 +142,10 @@ def _(q, k_codes, v_codes, k_scales, v_scales, starts, lens, table, max_new, sca
 @torch.library.custom_op("hxq::lora", mutates_args=())
 def lora(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, starts: torch.Tensor,
          adapters: torch.Tensor) -> torch.Tensor:
-    """y + scale (x A^T) B^T of each request's adapter."""
+    """y + scale (x A^T) B^T of each request's adapter, y for rows of none."""
     from .serving import LoraAdapters, lora_plan
-    return LoraAdapters(a, b, scales).add(y, x, lora_plan(starts, adapters, a.shape[0], x.shape[0]))
+    out = y.clone(memory_format=torch.contiguous_format)
+    return LoraAdapters(a, b, scales).add(out, x, lora_plan(starts, adapters, a.shape[0], x.shape[0]), out=out)
 
 
 @lora.register_fake

@@ -125,3 +125,34 @@ def test_serving_ops_match_the_calls(H, L, cuda):
     got = torch.ops.hxq.lora(y, x, a, b, s, starts, i(0, -1))
     assert torch.equal(got, S.LoraAdapters(a, b, s).add(y, x, S.lora_plan(starts, i(0, -1), 1, 23)))
     assert torch.equal(got[20:], y[20:]) and not torch.equal(got[:20], y[:20])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts,new", [([0, 4, 9], 5), ([0], 1), ([0, 0, 0], 1), ([3, 80, 150], 80)])
+def test_serving_ops_rows_of_no_request(H, L, cuda, starts, new):
+    """A padded step: an operator's result is its own memory, so rows that no
+    request covers are defined too, whatever the allocator held before."""
+    torch = cuda
+    import hxq_b200.torch_ops  # noqa: F401
+    from hxq_b200 import serving as S
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    T, B = 160, len(starts) - 1
+    c = S.KvCache.allocate(12, 2, 64)
+    k = torch.randn((192, 2, 64), device="cuda")
+    c.append(k, k.flip(0), torch.arange(192, dtype=torch.int32, device="cuda"))
+    lens, table = i(*[96] * B), torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)[:B].contiguous()
+    q, y = torch.randn((T, 4, 64), device="cuda").to(torch.bfloat16), torch.randn((T, 32), device="cuda")
+    x = torch.randn((T, 64), device="cuda").to(torch.bfloat16)
+    a, b = torch.randn((2, 8, 64), device="cuda").to(torch.bfloat16), torch.randn((2, 32, 8), device="cuda").to(torch.bfloat16)
+    none = torch.ones(T, dtype=torch.bool, device="cuda")
+    none[starts[0]:starts[-1]] = False
+    s = torch.ones(2, device="cuda")
+    for _ in range(3):   # what the allocator hands out again
+        del_me = [torch.full((T, 4, 64), float("nan"), dtype=torch.bfloat16, device="cuda"), torch.full((T, 32), float("nan"), device="cuda")]
+        del del_me
+        o = torch.ops.hxq.kv_attention(q, c.k, c.v, c.k_scales, c.v_scales, i(*starts), lens, table, new, 0.125, 0, True)
+        assert bool(o.isfinite().all()) and bool((o[none] == 0).all()) and bool((o[~none] != 0).any(-1).all())
+        for yy in (y, y.t().contiguous().t()):
+            got = torch.ops.hxq.lora(yy, x, a, b, s, i(*starts), i(*range(B)))
+            assert torch.equal(got[none], y[none]) and bool(got.isfinite().all()) and bool((got[~none] != y[~none]).any(-1).all())
+            assert got.data_ptr() != yy.data_ptr()
