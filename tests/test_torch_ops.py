@@ -156,3 +156,26 @@ def test_serving_ops_rows_of_no_request(H, L, cuda, starts, new):
             got = torch.ops.hxq.lora(yy, x, a, b, s, i(*starts), i(*range(B)))
             assert torch.equal(got[none], y[none]) and bool(got.isfinite().all()) and bool((got[~none] != y[~none]).any(-1).all())
             assert got.data_ptr() != yy.data_ptr()
+
+
+def test_makefile_builds_the_binding_against_pytorch_with_cuda(tmp_path):
+    import os
+    import subprocess
+
+    from conftest import PKG
+    torch_dir, out = tmp_path / "torch", tmp_path / "out"
+    (torch_dir / "lib").mkdir(parents=True)
+    out.mkdir()
+    (torch_dir / "version.py").write_text("cuda = None")
+
+    def plan():
+        r = subprocess.run(["make", "-n", "-C", PKG, f"TORCH={torch_dir}", f"PYDIR={out}"], capture_output=True, text=True, check=True)
+        return str(out / "_serving.so") in r.stdout
+    assert not plan()                                    # a PyTorch without CUDA: the C library alone
+    (torch_dir / "lib" / "libc10_cuda.so").touch()
+    assert plan()
+    (out / "_serving.so").touch()
+    assert not plan()
+    later = os.stat(out / "_serving.so").st_mtime + 10
+    os.utime(torch_dir / "version.py", (later, later))   # another PyTorch
+    assert plan()
