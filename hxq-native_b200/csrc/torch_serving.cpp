@@ -141,25 +141,12 @@ public:
         : k_(std::move(k)), v_(std::move(v)), ks_(std::move(k_scales)), vs_(std::move(v_scales)), dev_(k_.device())
     {
         on_cuda(k_, "k");
-        const bool i8 = k_.scalar_type() == at::kChar, f8 = k_.scalar_type() == at::kFloat8_e4m3fn;
-        need((i8 || f8) && v_.scalar_type() == k_.scalar_type(), "codes must be torch.int8 or torch.float8_e4m3fn");
-        need(k_.dim() == 4 && v_.sizes() == k_.sizes(), "codes must be [n_blocks, n_heads, block_tokens, head_dim]");
-        const int64_t blocks = k_.size(0), heads = k_.size(1), tokens = k_.size(2), dim = k_.size(3);
-        need(dim == 64 || dim == 128 || dim == 256, "head_dim must be 64, 128 or 256");
-        need(tokens % 16 == 0 && tokens > 0 && tokens <= 256, "block_tokens must be a multiple of 16, at most 256");
-        need(blocks > 0 && heads > 0 && heads < 65536 && blocks * tokens < (int64_t(1) << 31), "cache too large or empty");
-        for (const at::Tensor *t : {&ks_, &vs_})
-            need(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == blocks && t->size(1) == heads,
-                 "scales must be fp32 [n_blocks, n_heads]");
-        for (const at::Tensor *t : {&k_, &v_, &ks_, &vs_})
-            need(t->device() == dev_ && t->is_contiguous(), "the cache's tensors must be contiguous and on one device");
-        need((((uintptr_t)k_.data_ptr() | (uintptr_t)v_.data_ptr()) & 15u) == 0, "codes must be 16-byte aligned");
-        desc_ = {k_.data_ptr(), v_.data_ptr(), static_cast<float *>(ks_.data_ptr()), static_cast<float *>(vs_.data_ptr()),
-                 (uint32_t)blocks, (uint32_t)heads, (uint32_t)tokens, (uint32_t)dim, (uint32_t)(i8 ? HXQ_KV_INT8 : HXQ_KV_E4M3)};
+        look();
     }
 
     void append(at::Tensor k, at::Tensor v, const at::Tensor &slots, const MaybeTensor &status)
     {
+        look();
         rows(k, "k and v must be [tokens, n_heads, head_dim] in fp32, bf16 or f16 on the cache's device");
         rows(v, "k and v must be [tokens, n_heads, head_dim] in fp32, bf16 or f16 on the cache's device");
         ints(slots, "slots", dev_);
@@ -172,6 +159,7 @@ public:
 
     py::tuple read(const at::Tensor &slots, at::ScalarType dtype, const MaybeTensor &status)
     {
+        look();
         ints(slots, "slots", dev_);
         need(dtype == at::kFloat || dtype == at::kBFloat16 || dtype == at::kHalf, "dtype must be fp32, bf16 or f16");
         const c10::cuda::OptionalCUDAGuard guard(dev_);
@@ -187,6 +175,7 @@ public:
                          std::optional<double> scale, int64_t window, bool causal, const MaybeTensor &out_or, const MaybeTensor &lse,
                          const MaybeTensor &status)
     {
+        look();
         need(q.device() == dev_ && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && q.dim() == 3 &&
                  q.size(2) == desc_.head_dim && q.size(1) > 0 && q.size(1) % desc_.n_heads == 0,
              "q must be [rows, a multiple of the cache's heads, head_dim] in bf16 or f16 on the cache's device");
@@ -234,6 +223,29 @@ public:
     }
 
 private:
+    // The tensors as they are now: they may have been given other memory since the last call.
+    void look()
+    {
+        const bool i8 = k_.scalar_type() == at::kChar, f8 = k_.scalar_type() == at::kFloat8_e4m3fn;
+        need((i8 || f8) && v_.scalar_type() == k_.scalar_type(), "codes must be torch.int8 or torch.float8_e4m3fn");
+        need(k_.dim() == 4 && v_.sizes() == k_.sizes(), "codes must be [n_blocks, n_heads, block_tokens, head_dim]");
+        const int64_t blocks = k_.size(0), heads = k_.size(1), tokens = k_.size(2), dim = k_.size(3);
+        need(dim == 64 || dim == 128 || dim == 256, "head_dim must be 64, 128 or 256");
+        need(tokens % 16 == 0 && tokens > 0 && tokens <= 256, "block_tokens must be a multiple of 16, at most 256");
+        need(blocks > 0 && heads > 0 && heads < 65536 && blocks * tokens < (int64_t(1) << 31), "cache too large or empty");
+        for (const at::Tensor *t : {&ks_, &vs_})
+            need(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == blocks && t->size(1) == heads,
+                 "scales must be fp32 [n_blocks, n_heads]");
+        for (const at::Tensor *t : {&k_, &v_, &ks_, &vs_})
+            need(t->device() == dev_ && t->is_contiguous(), "the cache's tensors must be contiguous and on one device");
+        need((((uintptr_t)k_.data_ptr() | (uintptr_t)v_.data_ptr()) & 15u) == 0, "codes must be 16-byte aligned");
+        need(desc_.k == nullptr || (desc_.n_blocks == blocks && desc_.n_heads == heads && desc_.block_tokens == tokens &&
+                                    desc_.head_dim == dim && desc_.format == (i8 ? HXQ_KV_INT8 : HXQ_KV_E4M3)),
+             "the cache's tensors have another shape or type than it was made with");
+        desc_ = {k_.data_ptr(), v_.data_ptr(), static_cast<float *>(ks_.data_ptr()), static_cast<float *>(vs_.data_ptr()),
+                 (uint32_t)blocks, (uint32_t)heads, (uint32_t)tokens, (uint32_t)dim, (uint32_t)(i8 ? HXQ_KV_INT8 : HXQ_KV_E4M3)};
+    }
+
     void rows(at::Tensor &t, const char *what) const
     {
         need(t.device() == dev_ && elem_of(t) >= 0 && t.dim() == 3 && t.size(1) == desc_.n_heads && t.size(2) == desc_.head_dim, what);
@@ -273,24 +285,13 @@ public:
         : a_(std::move(a)), b_(std::move(b)), s_(std::move(scales)), dev_(a_.device())
     {
         on_cuda(a_, "a");
-        need(a_.scalar_type() == at::kBFloat16 && b_.scalar_type() == at::kBFloat16 && a_.dim() == 3 && b_.dim() == 3,
-             "a and b must be bf16 with three dimensions");
-        const int64_t n = a_.size(0), r = a_.size(1), in = a_.size(2), out = b_.size(1);
-        need(b_.size(0) == n && b_.size(2) == r, "b must be [n_adapters, out_features, rank]");
-        need(r % 8 == 0 && r > 0 && r <= 128, "rank must be a multiple of 8, at most 128");
-        need(in % 8 == 0 && in > 0 && out > 0 && in < 0x7fffff00 && out < 0x7fffff00, "in_features must be a multiple of 8");
-        need(n > 0 && n <= HXQ_LORA_MAX_ADAPTERS, "between 1 and 4096 adapters");
-        need(s_.scalar_type() == at::kFloat && s_.dim() == 1 && s_.size(0) == n, "scales must be fp32 [n_adapters]");
-        for (const at::Tensor *t : {&a_, &b_, &s_})
-            need(t->device() == dev_ && t->is_contiguous(), "the adapters' tensors must be contiguous and on one device");
-        need((((uintptr_t)a_.data_ptr() | (uintptr_t)b_.data_ptr()) & 15u) == 0, "a and b must be 16-byte aligned");
-        desc_ = {static_cast<const uint16_t *>(a_.data_ptr()), static_cast<const uint16_t *>(b_.data_ptr()),
-                 static_cast<const float *>(s_.data_ptr()), (uint32_t)n, (uint32_t)r, (uint32_t)in, (uint32_t)out};
+        look();
     }
 
     at::Tensor add(at::Tensor y, at::Tensor x, const at::Tensor &plan, int64_t n_tiles, int64_t n_tokens, int64_t n_requests,
                    int64_t n_adapters, const MaybeTensor &out_or)
     {
+        look();
         need(x.device() == dev_ && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.size(1) == desc_.in_features,
              "x must be bf16 [tokens, in_features] on the adapters' device");
         const int64_t T = x.size(0);
@@ -318,6 +319,26 @@ public:
     }
 
 private:
+    // The tensors as they are now: they may have been given other memory since the last call.
+    void look()
+    {
+        need(a_.scalar_type() == at::kBFloat16 && b_.scalar_type() == at::kBFloat16 && a_.dim() == 3 && b_.dim() == 3,
+             "a and b must be bf16 with three dimensions");
+        const int64_t n = a_.size(0), r = a_.size(1), in = a_.size(2), out = b_.size(1);
+        need(b_.size(0) == n && b_.size(2) == r, "b must be [n_adapters, out_features, rank]");
+        need(r % 8 == 0 && r > 0 && r <= 128, "rank must be a multiple of 8, at most 128");
+        need(in % 8 == 0 && in > 0 && out > 0 && in < 0x7fffff00 && out < 0x7fffff00, "in_features must be a multiple of 8");
+        need(n > 0 && n <= HXQ_LORA_MAX_ADAPTERS, "between 1 and 4096 adapters");
+        need(s_.scalar_type() == at::kFloat && s_.dim() == 1 && s_.size(0) == n, "scales must be fp32 [n_adapters]");
+        for (const at::Tensor *t : {&a_, &b_, &s_})
+            need(t->device() == dev_ && t->is_contiguous(), "the adapters' tensors must be contiguous and on one device");
+        need((((uintptr_t)a_.data_ptr() | (uintptr_t)b_.data_ptr()) & 15u) == 0, "a and b must be 16-byte aligned");
+        need(desc_.d_a == nullptr || (desc_.n_adapters == n && desc_.rank == r && desc_.in_features == in && desc_.out_features == out),
+             "the adapters' tensors have another shape than they were made with");
+        desc_ = {static_cast<const uint16_t *>(a_.data_ptr()), static_cast<const uint16_t *>(b_.data_ptr()),
+                 static_cast<const float *>(s_.data_ptr()), (uint32_t)n, (uint32_t)r, (uint32_t)in, (uint32_t)out};
+    }
+
     at::Tensor a_, b_, s_;
     at::Device dev_;
     hxq_lora_t desc_{};

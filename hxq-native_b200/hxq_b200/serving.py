@@ -69,13 +69,19 @@ class KvCache:
     """An 8-bit KV cache: codes [n_blocks, n_heads, block_tokens, head_dim]
     (torch.int8 or torch.float8_e4m3fn) and fp32 scales [n_blocks, n_heads]
     for keys and for values.  The tensors are the caller's and are used in
-    place."""
+    place, at whatever memory they have when a call is made; the cache is of
+    these tensors for good (k, v, k_scales and v_scales cannot be assigned)."""
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scales = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
         self._cache = _serving.Cache(k, v, k_scales, v_scales)
         self.device = k.device
         self.n_blocks, self.n_heads, self.block_tokens, self.head_dim = k.shape
-        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self._tensors = (k, v, k_scales, v_scales)
 
     @classmethod
     def allocate(cls, n_blocks: int, n_heads: int, head_dim: int, block_tokens: int = 16, dtype: torch.dtype = torch.int8,
@@ -140,14 +146,19 @@ def lora_plan(starts: torch.Tensor, adapters: torch.Tensor, n_adapters: int, n_t
 class LoraAdapters:
     """Low-rank adapters of one projection: a [n_adapters, rank, in_features]
     and b [n_adapters, out_features, rank] in bf16, scales [n_adapters] fp32.
-    Smaller ranks are padded with zeros."""
+    Smaller ranks are padded with zeros.  The tensors are the caller's, as a
+    KvCache's are."""
+
+    a = property(lambda self: self._tensors[0])
+    b = property(lambda self: self._tensors[1])
+    scales = property(lambda self: self._tensors[2])
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor):
         self._adapters = _serving.Adapters(a, b, scales)
         self.device = a.device
         self.n_adapters, self.rank, self.in_features = a.shape
         self.out_features = b.shape[1]
-        self.a, self.b, self.scales = a, b, scales
+        self._tensors = (a, b, scales)
 
     def add(self, y: torch.Tensor, x: torch.Tensor, plan: LoraPlan, out: torch.Tensor | None = None) -> torch.Tensor:
         """y + scale (x A^T) B^T of each token's adapter: x [tokens,

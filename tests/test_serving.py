@@ -1072,3 +1072,50 @@ def test_lora_plan_as_a_process_first_call(cuda, B, n):
 
     from conftest import PKG
     subprocess.run([sys.executable, "-c", _FIRST_CALL.format(pkg=PKG, B=B, n=n, op="lora_plan")], check=True, timeout=120)
+
+
+@pytest.mark.gpu
+def test_tensors_that_move(cuda):
+    """Calls use the memory that the tensors have then, not what they had."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    c = S.KvCache.allocate(4, 2, 64)
+    before = [t.detach() for t in (c.k, c.v, c.k_scales, c.v_scales)]
+    c.k.data = torch.zeros_like(c.k)
+    c.v.set_(torch.zeros_like(c.v))
+    c.k_scales.data = torch.zeros_like(c.k_scales)
+    c.v_scales.data = torch.zeros_like(c.v_scales)
+    x = torch.randn((2, 16, 2, 64), device="cuda")
+    c.append(x[0], x[1], torch.arange(16, 32, dtype=torch.int32, device="cuda"))
+    assert all(bool((t.float() == 0).all()) for t in before)
+    k, v = c.read(torch.arange(16, 32, dtype=torch.int32, device="cuda"), torch.float32)
+    assert float((k - x[0]).abs().max()) < 0.03 and float((v - x[1]).abs().max()) < 0.03
+    q = torch.randn((1, 2, 64), device="cuda").to(torch.bfloat16)
+    o = c.attention(q, i(0, 1), i(16), i(1).view(1, 1), 1)
+    want = torch.softmax(torch.einsum("hd,thd->ht", q[0].float(), k) / 8, -1)
+    assert float((o[0].float() - torch.einsum("ht,thd->hd", want, v)).abs().max()) < 0.02
+    for bad in (lambda: c.k.data.new_zeros((3, 2, 16, 64)), lambda: c.k.data.new_zeros((4, 2, 16, 64)).transpose(0, 1).contiguous().transpose(0, 1),
+                lambda: c.k.data.cpu(), lambda: c.k.data.view(torch.float8_e4m3fn)):
+        keep, c.k.data = c.k.data, bad()
+        for call in (lambda: c.append(x[0], x[1], i(*range(16))), lambda: c.read(i(0)), lambda: c.attention(q, i(0, 1), i(16), i(1).view(1, 1), 1)):
+            with pytest.raises(ValueError):
+                call()
+        c.k.data = keep
+    assert torch.equal(c.read(torch.arange(16, 32, dtype=torch.int32, device="cuda"), torch.float32)[0], k)
+    with pytest.raises(AttributeError):
+        c.k = torch.zeros_like(c.k)
+
+    a, b = torch.randn((2, 8, 64), device="cuda").bfloat16(), torch.randn((2, 32, 8), device="cuda").bfloat16()
+    h = S.LoraAdapters(a, b, torch.ones(2, device="cuda"))
+    plan = S.lora_plan(i(0, 5), i(1), 2, 5)
+    y, xx = torch.zeros((5, 32), device="cuda"), torch.randn((5, 64), device="cuda").bfloat16()
+    one = h.add(y, xx, plan)
+    a.data, b.data, h.scales.data = a * 2, b * 2, torch.full((2,), 2.0, device="cuda")
+    assert torch.equal(h.add(y, xx, plan), one * 8)
+    keep, h.b.data = h.b.data, torch.zeros((2, 40, 8), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        h.add(y, xx, plan)
+    h.b.data = keep
+    with pytest.raises(AttributeError):
+        h.a = a
