@@ -7,6 +7,7 @@
 // libhxq.so are handed over by address (bind), so that there is one library in
 // the process, whichever the binding loaded.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -72,6 +73,26 @@ void need(bool ok, const char *what)
     if (!ok) throw py::value_error(what);
 }
 
+// None of the operators has a gradient: where one would be expected, the call
+// is refused rather than its part of the gradient left out.
+void without_grad(std::initializer_list<const at::Tensor *> tensors)
+{
+    if (!at::GradMode::is_enabled()) return;
+    for (const at::Tensor *t : tensors)
+        if (t->requires_grad())
+            throw std::runtime_error("the serving operators have no gradient, and a tensor given requires one: call under torch.no_grad()");
+}
+
+// A tensor that a call writes: autograd and others who keep it see that it changed.
+void changed(const at::Tensor &t)
+{
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void changed(const MaybeTensor &t)
+{
+    if (t) changed(*t);
+}
+
 void on_cuda(const at::Tensor &t, const char *name)
 {
     if (!t.is_cuda()) throw py::value_error(std::string(name) + " must be a CUDA tensor");
@@ -131,6 +152,8 @@ py::tuple kv_plan(const at::Tensor &fresh, const at::Tensor &cached, const at::T
                    (uint32_t)block_tokens, i32(free_blocks), (uint32_t)free_blocks.numel(), at0, at0 + B + 1, at0 + 2 * B + 2,
                    at0 + 2 * B + 2 + n_slots, (uint32_t)n_slots, at0 + 2 * B + 1, word(status, dev), stream_of(dev)),
           "hxq_cuda_kv_plan");
+    changed(table);
+    changed(status);
     const auto part = buf.split_with_sizes({B + 1, B, 1, n_slots, n_slots});
     return py::make_tuple(part[0], part[1], part[3], part[4], part[2]);
 }
@@ -151,10 +174,13 @@ public:
         rows(v, "k and v must be [tokens, n_heads, head_dim] in fp32, bf16 or f16 on the cache's device");
         ints(slots, "slots", dev_);
         need(k.scalar_type() == v.scalar_type() && k.size(0) == v.size(0) && k.size(0) == slots.numel(), "k, v and slots must go together");
+        without_grad({&k, &v, &ks_, &vs_});
         const c10::cuda::OptionalCUDAGuard guard(dev_);
         check(api.append(&desc_, k.data_ptr(), v.data_ptr(), elem_of(k), k.stride(0), k.stride(1), v.stride(0), v.stride(1), i32(slots),
                          (uint32_t)slots.numel(), word(status, dev_), stream_of(dev_)),
               "hxq_cuda_kv_append");
+        for (const at::Tensor *t : {&k_, &v_, &ks_, &vs_}) changed(*t);
+        changed(status);
     }
 
     py::tuple read(const at::Tensor &slots, at::ScalarType dtype, const MaybeTensor &status)
@@ -162,12 +188,14 @@ public:
         look();
         ints(slots, "slots", dev_);
         need(dtype == at::kFloat || dtype == at::kBFloat16 || dtype == at::kHalf, "dtype must be fp32, bf16 or f16");
+        without_grad({&ks_, &vs_});
         const c10::cuda::OptionalCUDAGuard guard(dev_);
         const at::Tensor out = make({2, slots.numel(), desc_.n_heads, desc_.head_dim}, dtype, dev_);
         at::Tensor k = out.select(0, 0), v = out.select(0, 1);
         check(api.read(&desc_, i32(slots), (uint32_t)slots.numel(), k.data_ptr(), v.data_ptr(), elem_of(out), word(status, dev_),
                        stream_of(dev_)),
               "hxq_cuda_kv_read");
+        changed(status);
         return py::make_tuple(k, v);
     }
 
@@ -179,6 +207,9 @@ public:
         need(q.device() == dev_ && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && q.dim() == 3 &&
                  q.size(2) == desc_.head_dim && q.size(1) > 0 && q.size(1) % desc_.n_heads == 0,
              "q must be [rows, a multiple of the cache's heads, head_dim] in bf16 or f16 on the cache's device");
+        without_grad({&q, &ks_, &vs_});
+        if (out_or) without_grad({&*out_or});
+        if (lse) without_grad({&*lse});
         if (q.stride(2) != 1 || ((q.stride(0) | q.stride(1)) & 7) != 0 || ((uintptr_t)q.data_ptr() & 15u) != 0)
             q = q.clone(at::MemoryFormat::Contiguous);
         ints(starts, "starts", dev_);
@@ -219,6 +250,9 @@ public:
         const size_t size = api.attention_workspace(&desc_, &a);
         const at::Tensor ws = make({(int64_t)size}, at::kByte, dev_);
         check(api.attention(&desc_, &a, ws.data_ptr(), size, word(status, dev_), stream_of(dev_)), "hxq_cuda_kv_attention");
+        changed(out_or);
+        changed(lse);
+        changed(status);
         return out;
     }
 
@@ -276,6 +310,7 @@ std::pair<at::Tensor, int64_t> lora_plan(const at::Tensor &starts, const at::Ten
     check(api.lora_plan(i32(starts), i32(adapters), (uint32_t)B, (uint32_t)n_adapters, (uint32_t)n_tokens, at0 + 4 * tiles,
                         reinterpret_cast<hxq_lora_tile_t *>(at0), word(status, dev), stream_of(dev)),
           "hxq_cuda_lora_plan");
+    changed(status);
     return {buf, tiles};
 }
 
@@ -301,6 +336,8 @@ public:
                  plan.is_contiguous() && plan.numel() == 4 * n_tiles + n_tokens &&
                  n_tiles == api.lora_tiles((uint32_t)n_requests, desc_.n_adapters, (uint32_t)T),
              "the plan was made for other adapters or tokens");
+        without_grad({&x, &y, &a_, &b_, &s_});
+        if (out_or) without_grad({&*out_or});
         if (x.stride(1) != 1 || (x.stride(0) & 7) != 0 || ((uintptr_t)x.data_ptr() & 15u) != 0) x = x.clone(at::MemoryFormat::Contiguous);
         const c10::cuda::OptionalCUDAGuard guard(dev_);
         need(!out_or || (out_or->device() == dev_ && out_or->scalar_type() == at::kFloat && out_or->sizes() == y.sizes() &&
@@ -315,6 +352,7 @@ public:
                        y.stride(0), static_cast<float *>(out.data_ptr()), out.stride(0), (uint32_t)n_requests, (uint32_t)T,
                        at0 + 4 * n_tiles, reinterpret_cast<const hxq_lora_tile_t *>(at0), ws.data_ptr(), size, stream_of(dev_)),
               "hxq_cuda_lora");
+        changed(out_or);
         return out;
     }
 

@@ -16,7 +16,8 @@ outputs and workspace from PyTorch's allocator, and can be captured in a CUDA
 graph.  Lengths, tables, slots and adapter numbers are int32 CUDA tensors and
 are not read on the host; `status`, an int32 CUDA tensor of one element, takes
 the HXQ_SERVING_* bits of what the device found out of range (see `problems`).
-There is no CPU implementation.
+There is no CPU implementation, and no gradient: with grad mode on, tensors
+that require one are refused.
 """
 from __future__ import annotations
 

@@ -189,7 +189,8 @@ class HxqLinear(torch.nn.Module):
     def forward(self, x: torch.Tensor, adapters=None, plan=None) -> torch.Tensor:
         """x @ W.T in fp32; with `adapters` (a hxq_b200.serving.LoraAdapters of
         this projection's rows) and the step's plan (lora_plan), plus each
-        token's adapter."""
+        token's adapter.  Adapters have no gradient: with them, x may not
+        require one while grad mode is on."""
         if self.fused:
             y = vq_matmul(x.to(torch.bfloat16), self.image, self.out_features)
         else:

@@ -1119,3 +1119,65 @@ def test_tensors_that_move(cuda):
     h.b.data = keep
     with pytest.raises(AttributeError):
         h.a = a
+
+
+@pytest.mark.gpu
+def test_no_gradient_is_lost(H, L, cuda):
+    """Calls that would leave their part out of a gradient are refused, and
+    what calls write in place counts as changed."""
+    torch = cuda
+    from hxq_b200 import serving as S, synth
+    from hxq_b200.torch_ops import HxqLinear
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    c = S.KvCache.allocate(4, 2, 64)
+    kv, table, status = torch.randn((3, 2, 64), device="cuda"), i(-1).view(1, 1), i(0)
+    q = torch.randn((3, 2, 64), device="cuda").to(torch.bfloat16)
+    out, lse = torch.zeros_like(q), torch.zeros((3, 2), device="cuda")
+    a, b = torch.randn((1, 8, 64), device="cuda").bfloat16(), torch.randn((1, 32, 8), device="cuda").bfloat16()
+    scales = torch.ones(1, device="cuda")
+    h = S.LoraAdapters(a, b, scales)
+    x, y = torch.randn((3, 64), device="cuda").bfloat16(), torch.randn((3, 32), device="cuda")
+    plan = S.kv_plan(i(3), i(0), table, i(2), 16, 3, status=status)
+    lp = S.lora_plan(plan.starts, i(0), 1, 3)
+    attend = lambda q, **kw: c.attention(q, plan.starts, plan.lens, table, 3, **kw)  # noqa: E731
+
+    def grad(t):
+        return t.detach().clone().requires_grad_()
+    calls = [lambda: c.append(grad(kv), kv, plan.slots), lambda: c.append(kv, grad(kv), plan.slots), lambda: attend(grad(q)),
+             lambda: attend(q, lse=grad(lse)), lambda: h.add(grad(y), x, lp), lambda: h.add(y, grad(x), lp),
+             lambda: S.LoraAdapters(grad(a), b, scales).add(y, x, lp), lambda: S.LoraAdapters(a, grad(b), scales).add(y, x, lp),
+             lambda: S.LoraAdapters(a, b, grad(scales)).add(y, x, lp)]
+    wide = HxqLinear(synth.scalar(32, 64, 3)), HxqLinear(synth.vq12(32, 64, 4))
+    assert [w.fused for w in wide] == [False, True]
+    calls += [lambda w=w: w(grad(x), adapters=h, plan=lp) for w in wide]
+    before = [t.clone() for t in (c.k, c.k_scales, y)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+    assert all(torch.equal(t, w) for t, w in zip((c.k, c.k_scales, y), before))
+    with torch.no_grad():
+        for call in calls:
+            call()
+    # the projection by itself keeps its gradient
+    xg = grad(x)
+    wide[0](xg).sum().backward()
+    assert torch.allclose(xg.grad.float(), wide[0].weight().sum(0).expand(3, -1), rtol=2.0 ** -8, atol=1e-3)
+
+    written = (table, c.k, c.v, c.k_scales, c.v_scales, out, lse, status, y)
+    v0 = [t._version for t in written]
+    S.kv_plan(i(3), i(0), table, i(2), 16, 3)
+    c.append(kv, kv, plan.slots)
+    attend(q, out=out, lse=lse, status=status)
+    h.add(y, x, lp, out=y)
+    assert all(t._version > v for t, v in zip(written, v0))
+    w = torch.randn_like(y).requires_grad_()
+    z = (w * y).sum()
+    h.add(y, x, lp, out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z.backward()
+    # under inference mode, whose tensors count nothing
+    with torch.inference_mode():
+        ci = S.KvCache.allocate(4, 2, 64)
+        ci.append(kv, kv, plan.slots)
+    ci.append(kv, kv, plan.slots)
+    assert torch.equal(ci.k, c.k)
