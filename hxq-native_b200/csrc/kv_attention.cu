@@ -640,6 +640,9 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     if ((((uintptr_t)args->d_q | (uintptr_t)d_workspace) & 15u) != 0 || ((args->q_stride_t | args->q_stride_h) & 7) != 0 ||
         ((uintptr_t)args->d_out & 1u) != 0)
         return HXQ_ERR_INVALID_ARG;
+    const Runs out = {(uintptr_t)args->d_out, {args->n_rows, args->n_heads}, {args->out_stride_t, args->out_stride_h}, cache->head_dim, 2},
+               q = {(uintptr_t)args->d_q, {args->n_rows, args->n_heads}, {args->q_stride_t, args->q_stride_h}, cache->head_dim, 2};
+    if (!out.apart() || !out.may_overwrite(q)) return HXQ_ERR_INVALID_ARG;
     const AttnLayout lay = attn_layout(cache->head_dim, (uint64_t)args->max_new * (args->n_heads / cache->n_heads));
     if (workspace_bytes < lay.bytes) return HXQ_ERR_INVALID_ARG;
     AttnArgs a;

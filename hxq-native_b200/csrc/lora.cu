@@ -593,6 +593,9 @@ hxq_error_t hxq_cuda_lora(const hxq_lora_t *adapters, const uint16_t *d_x, int64
     if ((((uintptr_t)adapters->d_a | (uintptr_t)adapters->d_b | (uintptr_t)d_x | (uintptr_t)d_tiles | (uintptr_t)d_workspace) & 15u) != 0 ||
         (((uintptr_t)d_y | (uintptr_t)d_out) & 3u) != 0 || (ldx & 7) != 0)
         return HXQ_ERR_INVALID_ARG;
+    const Runs out = {(uintptr_t)d_out, {n_tokens, 1}, {ldo, 0}, adapters->out_features, 4},
+               y = {(uintptr_t)d_y, {n_tokens, 1}, {ldy, 0}, adapters->out_features, 4};
+    if (!out.apart() || !out.may_overwrite(y)) return HXQ_ERR_INVALID_ARG;
     if (workspace_bytes < hxq_cuda_lora_workspace(adapters, n_requests, n_tokens)) return HXQ_ERR_INVALID_ARG;
     const uint32_t tiles = hxq_lora_tiles(n_requests, adapters->n_adapters, n_tokens);
     LoraArgs a;

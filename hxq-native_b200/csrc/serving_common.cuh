@@ -118,6 +118,57 @@ cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, size_t sm
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Host side: runs of `width` consecutive elements, n[0] x n[1] of them,
+// stride[] elements apart.
+struct Runs {
+    uintptr_t at;
+    int64_t n[2], stride[2];
+    int64_t width, size;   // elements of a run, bytes of an element
+
+    static __int128 far(__int128 v) { return v < 0 ? -v : v; }
+    bool longer0() const { return n[1] == 1 || (n[0] > 1 && far(stride[0]) >= far(stride[1])); }
+
+    // Whether every element has its own place, one stride being beyond all that
+    // the other one spans.
+    bool apart() const
+    {
+        const int o = longer0() ? 0 : 1, i = 1 - o;
+        const __int128 inner = n[i] > 1 ? (n[i] - 1) * far(stride[i]) + width : width;
+        return (n[i] == 1 || far(stride[i]) >= width) && (n[o] == 1 || far(stride[o]) >= inner);
+    }
+    void range(__int128 &lo, __int128 &hi) const
+    {
+        lo = hi = (__int128)at;
+        for (int d = 0; d < 2; ++d) ((stride[d] < 0) ? lo : hi) += (__int128)(n[d] - 1) * stride[d] * size;
+        hi += (__int128)width * size;
+    }
+    // Whether a call may write these (which are apart) and read the others: if
+    // they are the same elements in the same places, or share none. Where the
+    // strides differ that is told by the ranges alone.
+    bool may_overwrite(const Runs &r) const
+    {
+        __int128 a0, a1, b0, b1;
+        range(a0, a1);
+        r.range(b0, b1);
+        if (a1 <= b0 || b1 <= a0) return true;
+        for (int d = 0; d < 2; ++d)
+            if (n[d] > 1 && stride[d] != r.stride[d]) return false;
+        const __int128 bytes = (__int128)at - (__int128)r.at;
+        if (bytes == 0) return true;
+        if (bytes % size) return false;
+        const int o = longer0() ? 0 : 1, i = 1 - o;
+        auto below = [](__int128 v, __int128 by) { return v >= 0 ? v / by : -((-v + by - 1) / by); };
+        const __int128 so = n[o] > 1 ? stride[o] : 1, si = n[i] > 1 ? stride[i] : 1, delta = bytes / size;
+        for (int u = 0; u < 2; ++u)
+            for (int v = 0; v < 2; ++v) {
+                const __int128 x = n[o] > 1 ? below(delta, far(so)) + u : 0, rest = delta - x * far(so);
+                const __int128 y = n[i] > 1 ? below(rest, far(si)) + v : 0;
+                if (far(x) < n[o] && far(y) < n[i] && far(rest - y * far(si)) < width) return false;
+            }
+        return true;
+    }
+};
+
 // Host checks of a cache descriptor.
 inline hxq_error_t check_cache(const hxq_kv_cache_t *c)
 {

@@ -113,8 +113,8 @@ class KvCache:
         over its lens[b] keys in blocks table[b] (hxq_cuda_kv_attention).
         scale: head_dim ** -0.5 by default; window: how many keys back a row
         sees (0: all); max_new: the most rows of a request.  `lse` [rows,
-        heads] fp32 takes the log of the softmax sums.  Rows outside every
-        request are not written."""
+        heads] fp32 takes the log of the softmax sums.  `out` may be q.  Rows
+        outside every request are not written."""
         return self._cache.attention(q, starts, lens, table, max_new, scale, window, causal, out, lse, status)
 
 

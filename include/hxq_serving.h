@@ -113,7 +113,8 @@ hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots
  * every request are left as they were; where starts descend, rows that two
  * requests claim get either one's result, or all rows are left (recorded).
  * q and out are bf16 or f16 (elem), head_dim consecutive elements, strides in
- * elements, q rows 16-byte aligned.  Codes enter the products exactly, sums
+ * elements, q rows 16-byte aligned.  Elements of out have a place each, and it
+ * shares none with q unless it is q, strides and all.  Codes enter the products exactly, sums
  * and the softmax are fp32; for the second product a softmax weight times its
  * block's value scale is rounded to f16: by up to 2^-11 of it, and below 2^-21
  * of the row's largest by up to 2^-32 of that.  out is rounded once.  Value
@@ -172,7 +173,8 @@ typedef struct {
 } hxq_lora_t;
 /* x: bf16 [n_tokens] rows of in_features, ldx elements apart (a multiple of
  * 8, 16-byte aligned); y, out: fp32 rows of out_features, ldy and ldo apart;
- * out may be y.  n_requests is the B of the plan.  x A^T is summed in fp32 and
+ * out may be y, ldo then being ldy, and shares no element with it otherwise;
+ * rows of out do not overlap.  n_requests is the B of the plan.  x A^T is summed in fp32 and
  * enters the second product as three bf16 parts (together its 24 bits).
  * workspace: hxq_cuda_lora_workspace bytes, 16-byte aligned, contents don't
  * matter; calls that may overlap in time need one each. */

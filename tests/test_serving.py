@@ -1181,3 +1181,135 @@ def test_no_gradient_is_lost(H, L, cuda):
         ci.append(kv, kv, plan.slots)
     ci.append(kv, kv, plan.slots)
     assert torch.equal(ci.k, c.k)
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(out_stride_t=0), 34), (dict(out_stride_h=0), 34), (dict(out_stride_t=255), 34), (dict(out_stride_h=63), 34),
+    (dict(out_stride_t=64, out_stride_h=64), 34), (dict(out_stride_t=64, out_stride_h=9 * 64 - 1), 34),
+    (dict(out=FAKE + 2), 34), (dict(out=FAKE + 2 * 256 * 3), 34), (dict(out=FAKE - 2 * (256 + 64)), 34),
+    (dict(out=FAKE, out_stride_t=512), 34), (dict(out_stride_t=-200), 34),
+    (dict(q_stride_t=1024, out_stride_t=1024, out=FAKE + 2 * 255), 34), (dict(q_stride_t=1024, out_stride_t=1024, out=FAKE + 2 * (1024 * 3 - 255)), 34)])
+def test_attention_out_has_places_of_its_own(H, L, kw, code):
+    d = dict(q=FAKE, out=FAKE + (1 << 30), starts=FAKE, lens=FAKE, table=FAKE, n_requests=1, n_rows=9, n_heads=4, table_width=1,
+             max_new=1, scale=1.0, elem=1, causal=1, q_stride_t=256, q_stride_h=64, out_stride_t=256, out_stride_h=64)
+    a = H.KvAttention(**{**d, **kw})
+    assert L.hxq_cuda_kv_attention(C.byref(_cache(H)), C.byref(a), FAKE, 1 << 40, None, None) == code
+
+
+def test_overlaps_against_every_element(H, L, tmp_path):
+    """The host's arithmetic about strides against the elements themselves."""
+    import os
+    import subprocess
+
+    from conftest import PKG, REPO
+    src = tmp_path / "t.cu"
+    src.write_text(r"""
+#include "serving_common.cuh"
+#include <cstdio>
+#include <map>
+#include <random>
+#include <set>
+using hxq::serving::Runs;
+int main()
+{
+    std::mt19937 g(1);
+    auto pick = [&](int lo, int hi) { return (int64_t)(lo + (int)(g() % (unsigned)(hi - lo + 1))); };
+    long seen[4] = {0, 0, 0, 0};
+    for (int k = 0; k < 300000; ++k) {
+        Runs w = {(uintptr_t)(1000 + 2 * pick(0, 120)), {pick(1, 4), pick(1, 4)}, {pick(-30, 30), pick(-30, 30)}, pick(1, 6), 2};
+        Runs r = w;
+        r.at = (uintptr_t)(1000 + 2 * pick(0, 120));
+        if (pick(0, 2) == 0) { r.stride[0] = pick(-30, 30); r.stride[1] = pick(-30, 30); }
+        auto elements = [](const Runs &x, bool &twice) {
+            std::map<long, int> e;
+            int at = 0;
+            for (int64_t i = 0; i < x.n[0]; ++i)
+                for (int64_t j = 0; j < x.n[1]; ++j)
+                    for (int64_t d = 0; d < x.width; ++d)
+                        if (!e.emplace((long)x.at + 2 * (i * x.stride[0] + j * x.stride[1] + d), at++).second) twice = true;
+            return e;
+        };
+        bool twice = false, ignore = false;
+        const auto a = elements(w, twice), b = elements(r, ignore);
+        if (w.apart()) {
+            if (twice) { std::printf("apart, but twice\n"); return 1; }
+            bool share = false, same = a == b;
+            for (auto &x : a) share |= b.count(x.first) != 0;
+            const bool ok = w.may_overwrite(r);
+            if (ok && share && !same) { std::printf("shared and not the same\n"); return 2; }
+            bool strides = true;
+            for (int d = 0; d < 2; ++d) strides &= w.n[d] == 1 || w.stride[d] == r.stride[d];
+            if (!ok && strides && (!share || same)) { std::printf("refused without need\n"); return 3; }
+            ++seen[ok ? (share ? 0 : 1) : 2];
+        } else ++seen[3];
+    }
+    for (long s : seen) if (s < 100) { std::printf("too few of a kind\n"); return 4; }
+    return 0;
+}
+""")
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    if not os.path.exists(nvcc):
+        pytest.skip("no nvcc")
+    exe = tmp_path / "t"
+    subprocess.run([nvcc, "-std=c++17", "-arch=sm_100a", "-I", os.path.join(REPO, "include"), "-I", os.path.join(PKG, "csrc"), str(src), "-o", str(exe)],
+                   check=True, capture_output=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
+
+
+def test_lora_out_has_places_of_its_own(H, L):
+    def call(y=FAKE, ldy=48, out=FAKE + (1 << 30), ldo=48):
+        l = H.LoraDesc(a=FAKE, b=FAKE, scales=FAKE, n_adapters=2, rank=16, in_features=64, out_features=48)
+        return L.hxq_cuda_lora(C.byref(l), FAKE, 64, y, ldy, out, ldo, 2, 4, FAKE, FAKE, FAKE, 1 << 40, None)
+    for kw in (dict(ldo=0), dict(ldo=47), dict(out=FAKE + 4), dict(out=FAKE + 4 * 48), dict(out=FAKE, ldo=96), dict(out=FAKE - 4 * 48 * 3),
+               dict(ldy=100, ldo=100, out=FAKE + 4 * 47), dict(ldo=-40)):
+        assert call(**kw) == 34, kw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,lens", [([1, 2], [900, 70]), ([200, 90], [900, 300])])
+def test_attention_out_in_other_places(cuda, new, lens):
+    torch = cuda
+    from hxq_b200 import serving as S
+    c, q, starts, sd, ld, table = _attention_case(torch, S, new, lens, 2, 3, 64, 16, "int8", "bf16")
+    want, T = c.attention(q, sd, ld, table, max(new)), q.shape[0]
+    same = q.clone()
+    assert c.attention(same, sd, ld, table, max(new), out=same).data_ptr() == same.data_ptr() and torch.equal(same, want)
+    wide = torch.randn((T, 18, 64), device="cuda").to(torch.bfloat16)   # q and out in one buffer, as projections leave them
+    wide[:, 6:12] = q
+    for at in (0, 12, 6):
+        c.attention(wide[:, 6:12], sd, ld, table, max(new), out=wide[:, at:at + 6])
+        assert torch.equal(wide[:, at:at + 6], want)
+    heads_first = torch.zeros((6, T, 64), dtype=q.dtype, device="cuda").transpose(0, 1)
+    assert torch.equal(c.attention(q, sd, ld, table, max(new), out=heads_first), want)
+    row = q[:1].expand(T, -1, -1)   # one row for all
+    assert torch.equal(c.attention(row, sd, ld, table, max(new)), c.attention(row.contiguous(), sd, ld, table, max(new)))
+    for bad in (q[:1].clone().expand(T, -1, -1), q[:, :1].clone().expand(-1, 6, -1), torch.as_strided(q.clone(), q.shape, (64, 64, 1))):
+        with pytest.raises(RuntimeError):
+            c.attention(q, sd, ld, table, max(new), out=bad)
+    long = torch.randn((T + 1, 6, 64), device="cuda").to(torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        c.attention(long[:T], sd, ld, table, max(new), out=long[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("O", [48, 50])
+def test_lora_out_in_other_places(cuda, O):
+    torch = cuda
+    from hxq_b200 import serving as S
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    a, b = torch.randn((2, 8, 64), device="cuda").bfloat16(), torch.randn((2, O, 8), device="cuda").bfloat16()
+    h, T = S.LoraAdapters(a, b, torch.ones(2, device="cuda")), 90
+    x, y = torch.randn((T, 64), device="cuda").bfloat16(), torch.randn((T, O), device="cuda")
+    plan = S.lora_plan(i(0, 70, 80, 90), i(0, -1, 1), 2, T)
+    want = h.add(y, x, plan)
+    both = torch.zeros((T, 2 * O), device="cuda")
+    both[:, :O] = y
+    assert torch.equal(h.add(both[:, :O], x, plan, out=both[:, O:]), want) and torch.equal(both[:, :O], y)
+    assert torch.equal(h.add(both[:, :O], x, plan, out=both[:, :O]), want)
+    bias = y[:1].expand(T, -1)
+    assert torch.equal(h.add(bias, x, plan), h.add(bias.contiguous(), x, plan))
+    long = torch.randn((T + 1, O), device="cuda")
+    for yy, out in ((y, y[:1].clone().expand(T, -1)), (long[:T], long[1:]), (both[:, :O], both[:, 4:O + 4])):
+        with pytest.raises(RuntimeError):
+            h.add(yy, x, plan, out=out)
