@@ -433,11 +433,15 @@ template <int KS, bool WIDE> __global__ void __launch_bounds__(128, KS == 8 ? 2 
             float4 v = sums[r];
             if (m * 16 + g + 8 * r >= count || c >= a.R) v = make_float4(0, 0, 0, 0);
             float f[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+            // (bf16 ends before fp32 does: what would round to an infinity, but is none, leaves the rest to the next parts)
+            constexpr float kTopBf16 = 3.38953139e38f;
+            auto top_of = [&](float x) { return fabsf(x) <= 3.402823466e38f ? fminf(fmaxf(x, -kTopBf16), kTopBf16) : x; };
 #pragma unroll
             for (int part = 0; part < 3; ++part)
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    const __nv_bfloat162 top = __floats2bfloat162_rn(f[2 * w], f[2 * w + 1]);
+                    const __nv_bfloat162 top = part == 0 ? __floats2bfloat162_rn(top_of(f[2 * w]), top_of(f[2 * w + 1]))
+                                                         : __floats2bfloat162_rn(f[2 * w], f[2 * w + 1]);
                     const float2 back = __bfloat1622float2(top);
                     // (nothing is left of an infinity)
                     f[2 * w] = fabsf(back.x) <= 3.402823466e38f ? f[2 * w] - back.x : 0.0f;

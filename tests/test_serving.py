@@ -1313,3 +1313,23 @@ def test_lora_out_in_other_places(cuda, O):
     for yy, out in ((y, y[:1].clone().expand(T, -1)), (long[:T], long[1:]), (both[:, :O], both[:, 4:O + 4])):
         with pytest.raises(RuntimeError):
             h.add(yy, x, plan, out=out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R", [8, 32])
+def test_lora_near_the_top_of_fp32(cuda, R):
+    """s x A^T between bf16's largest and fp32's: no infinity comes of it."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    x, a, b = (torch.zeros(n, device="cuda") for n in ((3, 64), (1, R, 64), (1, 16, R)))
+    x[:, 7] = torch.tensor([1.0, -1.0, math.inf], device="cuda")
+    a[0, :, 7], b[0] = 255 / 128, 2.0 ** -40
+    b[0, :, 1:] = 0
+    scale = torch.tensor([1.7065e38], device="cuda")
+    f = float(scale.double()) * 255 / 128
+    assert 3.3962e38 < f < 3.4028e38
+    out = S.LoraAdapters(a.bfloat16(), b.bfloat16(), scale).add(torch.zeros((3, 16), device="cuda"), x.bfloat16(), S.lora_plan(i(0, 3), i(0), 1, 3))
+    want = f * 2.0 ** -40
+    assert bool(((out[0].double() - want).abs() <= want * 2.0 ** -21).all()) and bool(((out[1].double() + want).abs() <= want * 2.0 ** -21).all())
+    assert not bool(out[2].isfinite().any())
