@@ -1316,6 +1316,30 @@ def test_lora_out_in_other_places(cuda, O):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 9, 70])
+@pytest.mark.parametrize("R", [8, 40, 128])
+def test_lora_keeps_24_bits(cuda, R, T):
+    """x A^T of 24 significant bits by its making, through a B that picks one:
+    all of them arrive."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    g = torch.Generator().manual_seed(R + T)
+    I, O = 320, 64
+    x, a, b = torch.zeros((T, I)), torch.zeros((1, R, I)), torch.zeros((1, O, R))
+    x[:, 3], x[:, 100], x[:, 300] = 1.0, 2.0 ** -8, 2.0 ** -16
+    for k in (3, 100, 300):   # 8 bits each: products and their sum are exact
+        a[0, :, k] = (torch.randint(128, 256, (R,), generator=g) / 128) * (torch.randint(0, 2, (R,), generator=g) * 2 - 1)
+    pick = torch.randint(0, R, (O,), generator=g)
+    b[0, torch.arange(O), pick] = 1.0
+    h = (x.double() @ a[0].double().T)[:, pick]
+    out = S.LoraAdapters(a.bfloat16().cuda(), b.bfloat16().cuda(), torch.ones(1, device="cuda")).add(
+        torch.zeros((T, O), device="cuda"), x.bfloat16().cuda(), S.lora_plan(i(0, T), i(0), 1, T))
+    # eight additions at most that may truncate, 2^-23 each; without the third part of h 2^-17 and more is lost
+    assert bool(((out.double().cpu() - h).abs() <= h.abs() * 2.0 ** -20).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("R", [8, 32])
 def test_lora_near_the_top_of_fp32(cuda, R):
     """s x A^T between bf16's largest and fp32's: no infinity comes of it."""
