@@ -474,6 +474,15 @@ hxq_error_t hxq_cuda_kv_plan(const int32_t *d_new, const int32_t *d_cached, uint
     if (B > HXQ_PLAN_MAX_REQUESTS || block_tokens == 0 || block_tokens > 65536u || n_slots > 0x7fffffffu ||
         n_free > 0x7fffffffu)
         return HXQ_ERR_INVALID_ARG;
+    // CTAs read the lengths, the free list and the table while others write
+    const struct { const void *at; uint64_t words; } parts[] = {
+        {d_starts, (uint64_t)B + 1}, {d_lens, B}, {d_slots, n_slots}, {d_positions, n_slots}, {d_taken, 1},   // written
+        {d_table, (uint64_t)B * table_width}, {d_new, B}, {d_cached, B}, {d_free, n_free}};
+    for (int i = 0; i < 6; ++i)
+        for (int j = i + 1; j < 9; ++j) {
+            const uint64_t x = (uint64_t)(uintptr_t)parts[i].at, y = (uint64_t)(uintptr_t)parts[j].at;
+            if (parts[i].words && parts[j].words && x < y + 4 * parts[j].words && y < x + 4 * parts[i].words) return HXQ_ERR_INVALID_ARG;
+        }
     PlanArgs a = {d_new, d_cached, d_free, d_table, d_starts, d_lens, d_slots, d_positions, d_taken, d_status,
                   B, table_width, block_tokens, n_free, n_slots};
     const size_t smem = (size_t)(B + 1) * 2 * sizeof(uint32_t);

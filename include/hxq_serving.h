@@ -53,7 +53,8 @@ extern "C" {
  *                    read (a request's last, partly filled block) or left,
  *   d_taken[1]       how many of d_free were taken.
  * When the free list ends, the entries behind it become -1 and so do their
- * tokens' slots (HXQ_SERVING_NO_BLOCKS).  1 <= block_tokens <= 65536,
+ * tokens' slots (HXQ_SERVING_NO_BLOCKS).  No array that is written overlaps
+ * another one (d_lens is not d_cached).  1 <= block_tokens <= 65536,
  * B <= HXQ_PLAN_MAX_REQUESTS.  B = 0 writes d_starts[0] = 0 and the map. */
 #define HXQ_PLAN_MAX_REQUESTS 8192
 hxq_error_t hxq_cuda_kv_plan(const int32_t *d_new, const int32_t *d_cached, uint32_t B, int32_t *d_table,

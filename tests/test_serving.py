@@ -1357,3 +1357,39 @@ def test_lora_near_the_top_of_fp32(cuda, R):
     want = f * 2.0 ** -40
     assert bool(((out[0].double() - want).abs() <= want * 2.0 ** -21).all()) and bool(((out[1].double() + want).abs() <= want * 2.0 ** -21).all())
     assert not bool(out[2].isfinite().any())
+
+
+def test_plan_arrays_that_overlap(H, L):
+    """While some CTAs write the plan others still read the lengths."""
+    names = ["starts", "lens", "slots", "pos", "taken", "table", "new", "cached", "free"]
+    size = dict(new=3, cached=3, table=12, free=5, starts=4, lens=3, slots=8, pos=8, taken=1)
+    place = {n: FAKE + 4096 * k for k, n in enumerate(names)}
+
+    def call(**kw):
+        d = dict(place, **kw)
+        return L.hxq_cuda_kv_plan(d["new"], d["cached"], 3, d["table"], 4, 16, d["free"], 5, d["starts"], d["lens"], d["slots"], d["pos"], 8,
+                                  d["taken"], None, None)
+    for i, written in enumerate(names[:6]):
+        for other in names[i + 1:]:
+            assert call(**{written: place[other]}) == 34, (written, other)
+            assert call(**{written: place[other] + 4 * size[other] - 4}) == 34, (written, other)
+            assert call(**{written: place[other] - 4 * size[written] + 4}) == 34, (written, other)
+
+
+@pytest.mark.gpu
+def test_plan_arrays_side_by_side(H, L, cuda):
+    """In one buffer without a gap, as the PyTorch calls lay them out, and the
+    lengths read twice."""
+    torch = cuda
+    buf = torch.zeros(64, dtype=torch.int32, device="cuda")
+    at, sizes = {}, dict(new=3, table=6, free=4, starts=4, lens=3, slots=8, pos=8, taken=1)
+    k = 0
+    for n, size in sizes.items():
+        at[n], k = buf[k:k + size], k + size
+    at["new"].copy_(torch.tensor([2, 17, 1]))
+    at["free"].copy_(torch.tensor([5, 6, 7, 8]))
+    p = {n: t.data_ptr() for n, t in at.items()}
+    assert L.hxq_cuda_kv_plan(p["new"], p["new"], 3, p["table"], 2, 16, p["free"], 4, p["starts"], p["lens"], p["slots"], p["pos"], 8, p["taken"],
+                              None, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert at["starts"].tolist() == [0, 2, 19, 20] and at["lens"].tolist() == [4, 34, 2] and at["pos"].tolist() == [2, 3, 17, 18, 19, 20, 21, 22]
