@@ -93,6 +93,13 @@ void changed(const MaybeTensor &t)
     if (t) changed(*t);
 }
 
+// Sizes go to the library in 32 bits.
+void fits(std::initializer_list<int64_t> sizes)
+{
+    for (const int64_t n : sizes)
+        if (n >= (int64_t(1) << 31)) throw py::value_error("a size of 2^31 or more");
+}
+
 void on_cuda(const at::Tensor &t, const char *name)
 {
     if (!t.is_cuda()) throw py::value_error(std::string(name) + " must be a CUDA tensor");
@@ -142,6 +149,7 @@ py::tuple kv_plan(const at::Tensor &fresh, const at::Tensor &cached, const at::T
     ints(free_blocks, "free", dev);
     ints(table, "table", dev, 2);
     const int64_t B = fresh.numel();
+    fits({B, table.size(1), free_blocks.numel()});
     need(cached.numel() == B && table.size(0) == B, "new, cached and table must have one entry per request");
     need(block_tokens > 0 && block_tokens <= 65536 && n_slots >= 0 && n_slots < (int64_t(1) << 31), "block_tokens or n_slots out of range");
     const c10::cuda::OptionalCUDAGuard guard(dev);
@@ -173,6 +181,7 @@ public:
         rows(k, "k and v must be [tokens, n_heads, head_dim] in fp32, bf16 or f16 on the cache's device");
         rows(v, "k and v must be [tokens, n_heads, head_dim] in fp32, bf16 or f16 on the cache's device");
         ints(slots, "slots", dev_);
+        fits({slots.numel()});
         need(k.scalar_type() == v.scalar_type() && k.size(0) == v.size(0) && k.size(0) == slots.numel(), "k, v and slots must go together");
         without_grad({&k, &v, &ks_, &vs_});
         const c10::cuda::OptionalCUDAGuard guard(dev_);
@@ -187,6 +196,7 @@ public:
     {
         look();
         ints(slots, "slots", dev_);
+        fits({slots.numel()});
         need(dtype == at::kFloat || dtype == at::kBFloat16 || dtype == at::kHalf, "dtype must be fp32, bf16 or f16");
         without_grad({&ks_, &vs_});
         const c10::cuda::OptionalCUDAGuard guard(dev_);
@@ -216,6 +226,7 @@ public:
         ints(lens, "lens", dev_);
         ints(table, "table", dev_, 2);
         const int64_t B = lens.numel(), T = q.size(0);
+        fits({B, T, q.size(1), table.size(1)});
         need(starts.numel() == B + 1 && table.size(0) == B, "starts must have one entry more than lens, table as many");
         need(window >= 0 && (causal || window == 0), "a window needs causal attention");
         need(max_new >= 0, "max_new must not be negative");
@@ -330,6 +341,7 @@ public:
         need(x.device() == dev_ && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.size(1) == desc_.in_features,
              "x must be bf16 [tokens, in_features] on the adapters' device");
         const int64_t T = x.size(0);
+        fits({T, n_requests});
         need(y.device() == dev_ && y.scalar_type() == at::kFloat && y.dim() == 2 && y.size(0) == T && y.size(1) == desc_.out_features,
              "y must be fp32 [tokens, out_features] on the adapters' device");
         need(n_adapters == desc_.n_adapters && n_tokens == T && plan.device() == dev_ && plan.scalar_type() == at::kInt &&

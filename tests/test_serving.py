@@ -1393,3 +1393,25 @@ def test_plan_arrays_side_by_side(H, L, cuda):
                               None, torch.cuda.current_stream().cuda_stream) == 0
     torch.cuda.synchronize()
     assert at["starts"].tolist() == [0, 2, 19, 20] and at["lens"].tolist() == [4, 34, 2] and at["pos"].tolist() == [2, 3, 17, 18, 19, 20, 21, 22]
+
+
+@pytest.mark.gpu
+def test_sizes_past_32_bits(cuda):
+    """Refused, and not cut to their lower half."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    N = (1 << 32) + 1
+    long = torch.empty(N, dtype=torch.int32, device="cuda")
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    c = S.KvCache.allocate(4, 1, 64)
+    rows = torch.ones((1, 1, 64), device="cuda").expand(N, -1, -1)
+    q = torch.ones((1, 1, 64), dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: c.append(rows, rows, long), lambda: c.read(long), lambda: S.kv_plan(i(1), i(0), long.view(1, -1), i(2), 16, 1),
+                 lambda: S.kv_plan(i(1), i(0), i(0).view(1, 1), long, 16, 1), lambda: S.kv_plan(long, long, long.view(-1, 1), i(2), 16, 1),
+                 lambda: c.attention(q.expand(N, -1, -1), i(0, 1), i(1), i(0).view(1, 1), 1),
+                 lambda: c.attention(q, i(0, 1), i(1), long.view(1, -1), 1)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
+    assert bool((c.k == 0).all())
