@@ -1415,3 +1415,38 @@ def test_sizes_past_32_bits(cuda):
         with pytest.raises(ValueError, match="2\\^31"):
             call()
     assert bool((c.k == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_prompts_replayed_with_other_lengths(cuda, dim):
+    """Two graphs over the kernel for many rows, replayed at once."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    lens = [900, 130, 2000]
+    c, q, _, _, ld, table = _attention_case(torch, S, [300, 130, 80], lens, 2, 2, dim, 16, "e4m3", "bf16")
+    sd = torch.tensor([0, 300, 430, 510], dtype=torch.int32, device="cuda")
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.attention(q, sd, ld, table, 300)
+    graphs = []
+    for _ in range(2):
+        g, out = torch.cuda.CUDAGraph(), torch.full_like(q, 9.0)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        with torch.cuda.graph(g, stream=side):
+            c.attention(q, sd, ld, table, 300, window=700, out=out, status=status)
+        graphs.append((g, out, status))
+    for new in ([300, 130, 80], [1, 2, 500], [0, 130, 1], [64, 65, 0], [300, 130, 80]):
+        starts = [0, new[0], new[0] + new[1], sum(new)]
+        sd.copy_(torch.tensor(starts, dtype=torch.int32))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            graphs[0][0].replay()
+        graphs[1][0].replay()
+        torch.cuda.synchronize()
+        want, _, tol, _ = _attention_ref(torch, c, q, starts, lens, table, dim ** -0.5, 700, True)
+        n = starts[-1]
+        for _, out, status in graphs:
+            assert int(status) == 0 and bool(((out[:n].double() - want[:n]).abs() <= tol[:n]).all()), new
+        assert torch.equal(graphs[0][1][:n], graphs[1][1][:n])
