@@ -994,7 +994,7 @@ def test_attention_key_that_takes_the_weight(cuda, new, n, B, heads, dim, fmt):
     c.k.view(torch.int8)[table[:, 0].long(), :, 0] = (sign * top).to(c.k.dtype).view(torch.int8)
     c.v.view(torch.int8)[table[:, 0].long(), :, 0] = 0
     c.k_scales.fill_(1 / top)
-    c.v_scales.fill_(1 / top)
+    c.v_scales.fill_(1024 / top)   # what is left of the sum stays among f16's normal numbers
     # score of the first key: log of (number of keys x 999) above the others' mean
     beta = math.log(n * 999) / math.sqrt(dim)
     q = (sign * beta * (1 + 0.002 * torch.randn((B * new, heads, 1), generator=g, device="cuda"))).to(torch.float16)
@@ -1002,7 +1002,7 @@ def test_attention_key_that_takes_the_weight(cuda, new, n, B, heads, dim, fmt):
     lse = torch.zeros(q.shape[:2], device="cuda")
     o = c.attention(q, i([b * new for b in range(B + 1)]), i([n] * B), table, new, causal=False, lse=lse)
     for b, h, t in ((0, 0, 0), (B - 1, heads - 1, new - 1), (B // 2, 3, new // 2)):
-        k, v = (x[table[b].long(), h].double().reshape(-1, dim) / float(torch.tensor(top)) for x in (c.k, c.v))
+        k, v = (x[table[b].long(), h].double().reshape(-1, dim) * float(s[0, 0]) for x, s in ((c.k, c.k_scales), (c.v, c.v_scales)))
         sc = k @ q[b * new + t, h].double() / math.sqrt(dim)
         p = torch.softmax(sc, 0)
         assert 0.99 < float(p[0]) < 0.9999
