@@ -32,10 +32,12 @@
 // joins the parts of each cut unit in order.  Every CTA derives the cut from
 // the lengths itself, so it follows the lengths of a replayed graph.
 //
-// Bound by memory with four CTAs (16 warps) an SM to hide its latency: 64
-// requests of up to 8192 keys, 8 heads of 128, groups of 4: 116 us a call, 71%
-// of the copy bandwidth; 2 of 131,001 keys: 107.6 us, 76% (cp.async in place of
-// TMA: 130 and 126; 8 rows on the side of 16: 166 and 158).  One request of
+// Bound by instructions, then memory: 64 requests of up to 8192 keys, 8 heads of
+// 128, groups of 4: 113 to 117 us a call, 71 to 73% of the copy bandwidth; 2 of
+// 131,001 keys: 109 us, 75% (cp.async in place of TMA: 130 and 126; 8 rows on
+// the side of 16: 166 and 158).  Instructions are issued in 58% of a scheduler's
+// cycles and shared memory is at 56% of its wavefronts; a warp that waits does
+// so for a fixed latency or shared memory, a seventh as often for device memory.  One request of
 // 1024 keys takes 14.4 us a call, latency: launch, cut, copies, join.
 #include "kv_attention.cuh"
 
@@ -595,13 +597,17 @@ struct AttnLayout {
 // What a wait inside a kernel may take: about a second.
 std::atomic<uint32_t> wait_cycles{2000000000u};
 
-// Requests with more rows than this go to the tcgen05 kernel.
+// Requests with more rows than this go to the tcgen05 kernel.  16 requests of
+// 4096 keys, 8 heads, int8, rows of a request: us a call here (tiles of 16) and
+// there: heads of 128, 32: 87, 105; 48: 120, 105; 64: 153, 107; 96: 214, 107;
+// heads of 64: 65, 89; 87, 89; 109, 87; 155, 89.  (They meet at about 40 and 48.)
 constexpr uint32_t kFewRows = 64;
 
 AttnLayout attn_layout(uint32_t D, uint64_t most_rows)   // most_rows: of a request, as the caller says
 {
     AttnLayout l;
     const uint32_t sms = (uint32_t)sm_count();
+    // tiles of 8 rows or of 16, the same keys: 8 rows 44 and 52 us (heads of 64: 35, 40), 12 rows 69 and 54 (52, 42)
     l.few = D == 256 || most_rows <= 8;
     l.ctas = sms * ctas_per_sm(D, l.few);
     l.tc_ctas = D != 256 && most_rows > kFewRows ? sms : 0;
@@ -680,10 +686,9 @@ hxq_error_t hxq_cuda_kv_attention(const hxq_kv_cache_t *cache, const hxq_kv_atte
     uint8_t *ws = static_cast<uint8_t *>(d_workspace);
     a.desc = reinterpret_cast<int4 *>(ws);
     a.part = reinterpret_cast<float *>(ws + lay.part);
-    // Few rows of a request: this file's kernel. More: the tcgen05 kernel (64
-    // is where tiles of 16 rows read the keys four times over; that kernel
-    // takes 128 rows at a time). Without rows of the other kind a launch ends
-    // after its scan of the lengths.
+    // Few rows of a request: this file's kernel. More: the tcgen05 kernel.
+    // Without rows of the other kind a launch ends after its scan of the
+    // lengths.
     AttnArgs tc = a;
     if (lay.tc_ctas) {
         a.row_max = kFewRows;

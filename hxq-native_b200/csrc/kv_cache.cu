@@ -15,7 +15,7 @@ namespace serving {
 // every CTA sums the lengths (8 bytes a request out of L2, a block scan) and
 // then fills its own part of the slot map and of the table.  Bound by the
 // launch and two dependent loads, not by bytes: 8.5 us a call for 64 decoding
-// requests and 8.3 for 500 prompts of up to 1024 tokens.
+// requests and for 500 prompts of up to 1024 tokens.
 
 constexpr int kPlanThreads = 512;
 

@@ -33,10 +33,10 @@
 // weights back, the next scores behind the weights' product (about 4,900 cycles
 // a step of two tiles, where the tensor pipe needs 2,060, the exponentials
 // 2,050 and the conversion's shared memory traffic about 2,500).  Three prompts
-// of up to 4096 rows, 32 heads of 128, int8: 366 us a call, 659 TFLOP/s (38% of
-// the measured matrix rate; tensor pipe active 34% of the time, instructions
+// of up to 4096 rows, 32 heads of 128, int8: 375 to 382 us a call, 640 TFLOP/s (37%
+// of the measured matrix rate; tensor pipe active 33% of the time, instructions
 // issued in 61% of the cycles); two chunks of 512 rows x 40 heads of 64 over a
-// window of 4096 keys, e4m3: 107 us.  A second issuing warp, one a
+// window of 4096 keys, e4m3: 109 us.  A second issuing warp, one a
 // tile, cost (462 -> 490 us at the time).
 //
 // Work is cut and joined as in kv_attention.cu, with granules of 128 keys.
@@ -51,7 +51,7 @@ namespace serving {
 
 constexpr int kKeys = 128;                 // keys of a step
 constexpr int kTile = 128;                 // rows of a tile
-constexpr int kFixedT = 3;                 // steps that a unit costs by itself (kernel of the prompts above: 2: 390 us, 3: 355, 4: 361)
+constexpr int kFixedT = 3;                 // steps that a unit costs by itself (the prompts above and the chunks: 2: 395, 108.4 us, 3: 375, 108.8, 4: 380, 108.9)
 constexpr int kSoftWarps = 16, kConvWarps = 4;
 constexpr int kMmaWarp = kSoftWarps + kConvWarps, kLoadWarp = kMmaWarp + 1, kPlanWarp = kMmaWarp + 2;
 constexpr int kWarpsT = kMmaWarp + 4;       // six warpgroups

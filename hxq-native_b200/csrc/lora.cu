@@ -11,10 +11,10 @@
 // most of a tcgen05 tile empty.  Bound by memory: the shrink by x
 // (prompts) or A (decode), the expand by reading and writing y and by B; then
 // by how evenly tiles of 1 to 64 tokens fill the SMs.  A call of 40 requests of
-// up to 50 tokens, 24 adapters of rank 64, 4096 to 11008 features: 62.5 us,
-// shrink 14 and expand 38 (bytes: 22); 6 prompts of up to 2048 tokens, rank 32,
-// 11008 to 4096: 108 us, shrink 31 and expand 52 (61); 64 decoding requests,
-// rank 16, 4096 to 4096: 14.2 us, the calls and two launches.
+// up to 50 tokens, 24 adapters of rank 64, 4096 to 11008 features: 63 us,
+// shrink 15 and expand 40 (bytes: 22; its warps wait for the loads of y and B); 6 prompts of up to 2048 tokens, rank 32,
+// 11008 to 4096: 109 us, shrink 32 and expand 54 with 120 MB of x and y left in
+// L2 by the call before (61); 64 decoding requests, rank 16, 4096 to 4096: 14 to 15 us, the calls and two launches.
 #include "serving_common.cuh"
 
 #include "tc_pipe.cuh"
@@ -29,7 +29,8 @@ constexpr int kShrinkRanks = 32;   // rows of A a CTA takes
 // ---------------------------------------------------------------------------
 // The plan: groups' sizes (one warp over the requests in order, so that tokens
 // keep theirs), their tiles (block scans), then tiles and order, found by
-// binary search.  Every CTA does the first two itself: one launch, 5 us.
+// binary search.  Every CTA does the first two itself: one launch, 6 to 7 us for
+// up to 64 requests; one warp takes 32 more of them a turn.
 struct LoraPlanArgs {
     const int32_t *starts, *ids;
     int32_t *order;

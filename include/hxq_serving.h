@@ -95,7 +95,7 @@ typedef struct {
 hxq_error_t hxq_cuda_kv_append(const hxq_kv_cache_t *cache, const void *d_k, const void *d_v, int elem,
                                int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h,
                                const int32_t *d_slots, uint32_t n_tokens, uint32_t *d_status, void *stream);
-/* code * scale at the given slots, rounded once to elem: contiguous
+/* code * scale (in fp32, then rounded to elem) at the given slots: contiguous
  * [n_tokens, n_heads, head_dim] into d_k and d_v (either may be NULL).
  * Negative slots give rows of zeros, slots outside the cache also (recorded). */
 hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots, uint32_t n_tokens, void *d_k,
