@@ -119,9 +119,10 @@ hxq_error_t hxq_cuda_kv_read(const hxq_kv_cache_t *cache, const int32_t *d_slots
  * and the softmax are fp32; for the second product a softmax weight times its
  * block's value scale is rounded to f16: by up to 2^-11 of it, and below 2^-21
  * of the row's largest by up to 2^-32 of that.  out is rounded once.  Value
- * blocks with a scale below 2^-80 count as 0.  Keys whose value scale is 2^-130
- * of the largest that the row sees, or less, are not counted in the softmax's
- * sum (with those that count as 0: where a scale is above 2^50).  Codes of e4m3 caches are finite (hxq_cuda_kv_append
+ * blocks with a scale below 2^-80 count as 0.  A key is not counted in the
+ * softmax's sum where its weight times its value scale (2^-80 at least) is less
+ * than 2^-130 of the row's largest such product; while the value scales that a
+ * row sees are below 2^26 that is what fp32 sums do not hold either.  Codes of e4m3 caches are finite (hxq_cuda_kv_append
  * writes no others; slots that no request reads may hold anything).
  * d_lse (optional): [n_rows, n_heads] fp32, natural log of the softmax sums.
  * max_new: the most rows of any request; it only chooses the kernel, results

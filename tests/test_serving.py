@@ -1450,3 +1450,23 @@ def test_attention_of_prompts_replayed_with_other_lengths(cuda, dim):
         for _, out, status in graphs:
             assert int(status) == 0 and bool(((out[:n].double() - want[:n]).abs() <= tol[:n]).all()), new
         assert torch.equal(graphs[0][1][:n], graphs[1][1][:n])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 140])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_value_scales_far_apart(cuda, new, dim):
+    """Values of 0 and of 2^40 times a code, seen with the same weight: those of
+    0 count in the softmax's sum."""
+    torch = cuda
+    from hxq_b200 import serving as S
+    n, P = 320, 16
+    c = S.KvCache.allocate(n // P, 1, dim, P)
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    c.v.fill_(64)
+    c.v_scales.copy_(torch.where(torch.arange(n // P, device="cuda") % 2 == 0, 0.0, 2.0 ** 40)[:, None])
+    q, lse = torch.ones((new, 2, dim), dtype=torch.bfloat16, device="cuda"), torch.zeros((new, 2), device="cuda")
+    o = c.attention(q, i([0, new]), i([n]), torch.arange(n // P, dtype=torch.int32, device="cuda").view(1, -1), new, causal=False, lse=lse)
+    # half of the keys: exact in f16 and fp32 but for the inverses of the scales and the sum (2^-20), and out in bf16
+    assert bool(((o.double() / 2.0 ** 45 - 1).abs() <= 2.0 ** -8).all())
+    assert bool(((lse.double() - math.log(n)).abs() <= 2.0 ** -19 * math.log(n)).all())
